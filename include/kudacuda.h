@@ -566,6 +566,71 @@ KUDACUDA_API int kudacuda_sm100_gqa_decode_batch(void* handle, uint64_t query, u
                                                  int64_t kv_heads, int64_t head_dim, float scale, int shared_cache,
                                                  uint64_t stream);
 
+/* ---- paged KV cache and sampling (no reference counterpart) ----
+ * A cache in pages [num_pages][kv_heads][page_size][head_dim] (f16 or bf16,
+ * page_size 16, 32, 64 or 128, head_dim 64 or 128) and a ragged batch of new
+ * tokens: rows query_start[b] .. query_start[b + 1] - 1 (int32 [batch + 1],
+ * starting at 0) are sequence b's, kv_len[b] (int32) its length with them, so
+ * row i of n_b is at position kv_len[b] - n_b + i; block_table[b][j] (int32,
+ * rows table_stride apart) is the page of its keys j * page_size ...  A
+ * sequence may have no rows.  Entries past a sequence's length are not read;
+ * a position or page out of range that is needed sets bit 2 of the error word
+ * and touches no memory.
+ *
+ * rope_append_paged: rows of qkv (q heads | k heads | v heads, qkv_stride
+ *   elements apart), plus bias (optional, one element per column, rounded to
+ *   the type like a projection's output), rotated over the first rotary_dim
+ *   dims of every q and k head: pairs (i, i + rotary_dim / 2), or (2i, 2i + 1)
+ *   when interleaved, by cos/sin fp32 [max_pos][rotary_dim / 2] (scaled tables
+ *   serve scaled positions); q to q_out [rows][q_stride], k and v to their
+ *   pages.  32-bit arithmetic, one rounding.
+ * paged_attention: out[r][h] = softmax(scale q k^T) V over keys at positions
+ *   <= the row's own, lse (optional, fp32 [rows][q_heads]) the natural log of
+ *   the sum of exponentials; a row without keys gives 0 and -inf.  max_query
+ *   is the largest number of rows of a sequence.  workspace_bytes(max_kv =
+ *   table_width * page_size) once; the contents need no initialisation, and
+ *   calls that may overlap need a workspace each.
+ * kv_pages_copy: page pairs[i][0] -> page pairs[i][1] (int32 device pairs) of
+ *   K and V in every layer (layer_stride bytes apart); no page is both a
+ *   source and a target.  block_table / page_map (both or neither): every
+ *   valid entry e of the tables becomes page_map[e].
+ * sample: per row temperature, top_k, top_p, min_p (device arrays, null: off),
+ *   one uniform number in [0, 1) -> token, and its log-probability in the
+ *   distribution it was drawn from (optional).  Whole-number masses
+ *   rint(2^38 exp((x - max) / T)): the result does not depend on the batch.
+ *   Order (value descending, index ascending): top-k, then the shortest prefix
+ *   of mass >= top_p, then exp(..) >= min_p; drawn in order of index.
+ *   temperature <= 0: the lowest index of the maximum.  NaN counts as -inf; a
+ *   row with nothing above -inf gives -1. */
+KUDACUDA_API int kudacuda_sm100_rope_append_paged(void* handle, int dtype, uint64_t qkv, int64_t qkv_stride,
+                                                  uint64_t bias, uint64_t q_out, int64_t q_stride, uint64_t k_pages,
+                                                  uint64_t v_pages, uint64_t rope_cos, uint64_t rope_sin,
+                                                  int64_t max_pos, int64_t rotary_dim, int interleaved,
+                                                  uint64_t query_start, uint64_t kv_len, uint64_t block_table,
+                                                  int64_t table_stride, int64_t table_width, int64_t batch,
+                                                  int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                  int64_t num_pages, int64_t page_size, uint64_t stream);
+KUDACUDA_API int64_t kudacuda_sm100_paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t max_query,
+                                                                    int64_t q_heads, int64_t kv_heads,
+                                                                    int64_t head_dim, int64_t max_kv);
+KUDACUDA_API int kudacuda_sm100_paged_attention(void* handle, int dtype, uint64_t query, int64_t q_stride,
+                                                uint64_t k_pages, uint64_t v_pages, uint64_t output,
+                                                int64_t out_stride, uint64_t lse, uint64_t workspace,
+                                                int64_t workspace_bytes, uint64_t query_start, uint64_t kv_len,
+                                                uint64_t block_table, int64_t table_stride, int64_t table_width,
+                                                int64_t batch, int64_t rows, int64_t max_query, int64_t q_heads,
+                                                int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                                                int64_t page_size, float scale, uint64_t stream);
+KUDACUDA_API int kudacuda_sm100_kv_pages_copy(void* handle, uint64_t k_pages, uint64_t v_pages, int64_t layers,
+                                              int64_t layer_stride, int64_t num_pages, int64_t page_bytes,
+                                              uint64_t pairs, int64_t count, uint64_t block_table,
+                                              int64_t table_stride, int64_t table_rows, int64_t table_width,
+                                              uint64_t page_map, uint64_t stream);
+KUDACUDA_API int kudacuda_sm100_sample(void* handle, int dtype, uint64_t logits, int64_t row_stride, int64_t rows,
+                                       int64_t vocab, uint64_t temperature, uint64_t top_k, uint64_t top_p,
+                                       uint64_t min_p, uint64_t uniform, uint64_t tokens, uint64_t logprobs,
+                                       uint64_t stream);
+
 /* Library / build identification: "sm_100a". */
 KUDACUDA_API const char* kudacuda_sm100_target_arch(void);
 

@@ -275,6 +275,82 @@ cudaError_t batch_argmax_pairs(const float* partials, int ksplit, int vocab, int
 cudaError_t batch_select_advance(const int32_t* gathered, int world, int batch, int32_t* state, int32_t* history,
                                  int history_len, cudaStream_t s);
 
+// ---- paged KV cache: ragged batches of new tokens (paged.cu, paged_attention.cu) ----
+// Rows query_start[b] .. query_start[b + 1] - 1 are sequence b's new tokens; row
+// i of them is at position kv_len[b] - n_b + i.  Key j of sequence b lies in
+// page table[b * table_stride + j / page_size], slot j % page_size, of
+// [num_pages][kv_heads][page_size][head_dim].
+struct PagedBatch {
+    const int32_t* query_start;  // [batch + 1]
+    const int32_t* kv_len;       // [batch]
+    const int32_t* table;
+    int64_t table_stride;
+    int table_width;
+    int batch, rows;
+    int q_heads, kv_heads, head_dim;
+    int num_pages, page_size;  // page_size 16, 32, 64 or 128
+    int* err;
+};
+struct RopeAppendArgs {
+    PagedBatch p;
+    const void* qkv;  // [rows][qkv_stride]: q heads | k heads | v heads
+    int64_t qkv_stride;
+    const void* bias;  // [(q_heads + 2 kv_heads) * head_dim] or null
+    void* q_out;       // [rows][q_stride]
+    int64_t q_stride;
+    void* k_pages;
+    void* v_pages;
+    const float* cos;  // [max_pos][rotary_dim / 2]
+    const float* sin;
+    int max_pos, rotary_dim, interleaved;
+};
+cudaError_t rope_append_paged(const RopeAppendArgs& a, int dt, cudaStream_t s);
+struct PagedAttentionArgs {
+    PagedBatch p;
+    const void* q;  // [rows][q_stride], heads head_dim apart
+    int64_t q_stride;
+    const void* k_pages;
+    const void* v_pages;
+    void* out;  // [rows][out_stride]
+    int64_t out_stride;
+    float* lse;  // [rows][q_heads] or null
+    void* workspace;
+    int max_query;
+    float scale;
+};
+int64_t paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t max_query, int64_t q_heads,
+                                        int64_t kv_heads, int64_t head_dim, int64_t max_kv);
+cudaError_t paged_attention(const PagedAttentionArgs& a, int dt, cudaStream_t s);
+struct PagesCopyArgs {
+    void* k_pages;
+    void* v_pages;
+    int64_t layer_stride;  // bytes
+    int64_t page_bytes;    // a multiple of 16
+    int layers, num_pages;
+    const int32_t* pairs;  // [count][2]: from, to
+    int count;
+    int32_t* table;  // rewritten through page_map, or null
+    int64_t table_stride;
+    int table_rows, table_width;
+    const int32_t* page_map;  // [num_pages]
+    int* err;
+};
+cudaError_t kv_pages_copy(const PagesCopyArgs& a, cudaStream_t s);
+// ---- sampling (sample.cu) -------------------------------------------------------
+struct SampleArgs {
+    const void* logits;  // [rows][row_stride]
+    int64_t row_stride;
+    int rows, vocab;
+    const float* temperature;  // [rows] or null (1)
+    const int32_t* top_k;      // [rows] or null (off)
+    const float* top_p;
+    const float* min_p;
+    const float* uniform;  // [rows]
+    int32_t* tokens;
+    float* logprobs;  // [rows] or null
+};
+cudaError_t sample_rows(const SampleArgs& a, int dt, cudaStream_t s);
+
 int64_t decode_persistent_scratch_bytes(const PersistDims& d, int sms);
 const char* decode_persistent_check(const PersistDims& d, int sms);
 cudaError_t decode_layers_persistent(const PersistLaunch& p, cudaStream_t stream);

@@ -1715,6 +1715,209 @@ int kudacuda_sm100_gqa_decode_batch(void* raw, uint64_t query, uint64_t key_cach
     return finish(h, "gqa decode (per-sequence lengths)", kc::gqa_decode(a, kc::kBF16, S(stream)));
 }
 
+namespace {
+// The ragged batch and cache arguments that the paged entries share; returns
+// what is wrong with them, or null.  Pointers are 16-byte aligned where the
+// kernels read 16-byte words.
+const char* paged_batch(kc::PagedBatch* p, Handle* h, int dtype, uint64_t k_pages, uint64_t v_pages,
+                        uint64_t query_start, uint64_t kv_len, uint64_t block_table, int64_t table_stride,
+                        int64_t table_width, int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, int64_t num_pages, int64_t page_size) {
+    memset(p, 0, sizeof(*p));
+    if (dtype != kc::kF16 && dtype != kc::kBF16) return "dtype must be 1 (f16) or 2 (bf16)";
+    if (batch < 0 || batch > kc::kMaxGqaBatch || rows < 0 || rows > (int64_t{1} << 24))
+        return "requires 0 <= batch <= 65536 and 0 <= rows <= 2^24";
+    if (kv_heads < 1 || q_heads < kv_heads || q_heads > kc::kMaxGqaHeads || q_heads % kv_heads != 0)
+        return "query_heads must be a multiple of kv_heads, at most 1024";
+    if (head_dim != 64 && head_dim != 128) return "head_dim must be 64 or 128";
+    if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+        return "page_size must be 16, 32, 64 or 128";
+    if (num_pages < 1 || num_pages * kv_heads * page_size > (int64_t{1} << 31) - 1)
+        return "requires num_pages >= 1 and num_pages * kv_heads * page_size < 2^31";
+    if (table_width < 1 || table_width * page_size > (int64_t{1} << 30) || table_stride < table_width)
+        return "requires table_width >= 1, table_width * page_size <= 2^30 and table_stride >= table_width";
+    if (k_pages == 0 || v_pages == 0 || query_start == 0 || kv_len == 0 || block_table == 0)
+        return "requires non-null device pointers";
+    if (k_pages % 16 != 0 || v_pages % 16 != 0) return "the pages must be 16-byte aligned";
+    p->query_start = P<const int32_t>(query_start);
+    p->kv_len = P<const int32_t>(kv_len);
+    p->table = P<const int32_t>(block_table);
+    p->table_stride = table_stride;
+    p->table_width = static_cast<int>(table_width);
+    p->batch = static_cast<int>(batch);
+    p->rows = static_cast<int>(rows);
+    p->q_heads = static_cast<int>(q_heads);
+    p->kv_heads = static_cast<int>(kv_heads);
+    p->head_dim = static_cast<int>(head_dim);
+    p->num_pages = static_cast<int>(num_pages);
+    p->page_size = static_cast<int>(page_size);
+    p->err = h->err_word;
+    return nullptr;
+}
+int refuse(Handle* h, const char* entry, const char* why) {
+    h->set_error(std::string(entry) + ": " + why);
+    return 1;
+}
+}  // namespace
+
+int kudacuda_sm100_rope_append_paged(void* raw, int dtype, uint64_t qkv, int64_t qkv_stride, uint64_t bias,
+                                     uint64_t q_out, int64_t q_stride, uint64_t k_pages, uint64_t v_pages,
+                                     uint64_t rope_cos, uint64_t rope_sin, int64_t max_pos, int64_t rotary_dim,
+                                     int interleaved, uint64_t query_start, uint64_t kv_len, uint64_t block_table,
+                                     int64_t table_stride, int64_t table_width, int64_t batch, int64_t rows,
+                                     int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                                     int64_t page_size, uint64_t stream) {
+    static const char* const kName = "sm100_rope_append_paged";
+    Handle* h = as_handle(raw);
+    if (!ready(h, "kudacuda_sm100_rope_append_paged")) return 1;
+    kc::RopeAppendArgs a;
+    memset(&a, 0, sizeof(a));
+    if (const char* why = paged_batch(&a.p, h, dtype, k_pages, v_pages, query_start, kv_len, block_table, table_stride,
+                                      table_width, batch, rows, q_heads, kv_heads, head_dim, num_pages, page_size))
+        return refuse(h, kName, why);
+    if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0)
+        return refuse(h, kName, "rotary_dim must be a multiple of 16, at most head_dim");
+    if (rotary_dim > 0 && (rope_cos == 0 || rope_sin == 0 || max_pos < 1 || max_pos > (int64_t{1} << 30)))
+        return refuse(h, kName, "rotary_dim > 0 requires cos and sin tables of max_pos >= 1 rows");
+    if (rows > 0 && (qkv == 0 || q_out == 0)) return refuse(h, kName, "requires non-null device pointers");
+    if (qkv_stride < (q_heads + 2 * kv_heads) * head_dim || q_stride < q_heads * head_dim || qkv_stride % 8 != 0 ||
+        q_stride % 8 != 0)
+        return refuse(h, kName, "row strides must hold every head and be multiples of 8 elements");
+    if (qkv % 16 != 0 || q_out % 16 != 0 || bias % 16 != 0 || rope_cos % 16 != 0 || rope_sin % 16 != 0)
+        return refuse(h, kName, "rows, bias and tables must be 16-byte aligned");
+    a.qkv = P<const void>(qkv);
+    a.qkv_stride = qkv_stride;
+    a.bias = P<const void>(bias);
+    a.q_out = P<void>(q_out);
+    a.q_stride = q_stride;
+    a.k_pages = P<void>(k_pages);
+    a.v_pages = P<void>(v_pages);
+    a.cos = P<const float>(rope_cos);
+    a.sin = P<const float>(rope_sin);
+    a.max_pos = static_cast<int>(max_pos);
+    a.rotary_dim = static_cast<int>(rotary_dim);
+    a.interleaved = interleaved != 0 ? 1 : 0;
+    return finish(h, "rope_append_kernel", kc::rope_append_paged(a, dtype, S(stream)));
+}
+
+int64_t kudacuda_sm100_paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t max_query,
+                                                       int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                       int64_t max_kv) {
+    if (batch < 0 || batch > kc::kMaxGqaBatch || rows < 0 || rows > (int64_t{1} << 24) || max_query < 0 ||
+        kv_heads < 1 || q_heads < kv_heads || q_heads > kc::kMaxGqaHeads || q_heads % kv_heads != 0 ||
+        (head_dim != 64 && head_dim != 128) || max_kv < 0 || max_kv > (int64_t{1} << 30))
+        return -1;
+    return kc::paged_attention_workspace_bytes(batch, rows, max_query, q_heads, kv_heads, head_dim, max_kv);
+}
+
+int kudacuda_sm100_paged_attention(void* raw, int dtype, uint64_t query, int64_t q_stride, uint64_t k_pages,
+                                   uint64_t v_pages, uint64_t output, int64_t out_stride, uint64_t lse,
+                                   uint64_t workspace, int64_t workspace_bytes, uint64_t query_start, uint64_t kv_len,
+                                   uint64_t block_table, int64_t table_stride, int64_t table_width, int64_t batch,
+                                   int64_t rows, int64_t max_query, int64_t q_heads, int64_t kv_heads,
+                                   int64_t head_dim, int64_t num_pages, int64_t page_size, float scale,
+                                   uint64_t stream) {
+    static const char* const kName = "sm100_paged_attention";
+    Handle* h = as_handle(raw);
+    if (!ready(h, "kudacuda_sm100_paged_attention")) return 1;
+    kc::PagedAttentionArgs a;
+    memset(&a, 0, sizeof(a));
+    if (const char* why = paged_batch(&a.p, h, dtype, k_pages, v_pages, query_start, kv_len, block_table, table_stride,
+                                      table_width, batch, rows, q_heads, kv_heads, head_dim, num_pages, page_size))
+        return refuse(h, kName, why);
+    if (max_query < 0 || max_query > rows) return refuse(h, kName, "requires 0 <= max_query <= rows");
+    if (rows > 0 && (query == 0 || output == 0 || workspace == 0))
+        return refuse(h, kName, "requires non-null device pointers");
+    if (q_stride < q_heads * head_dim || out_stride < q_heads * head_dim || q_stride % 8 != 0 || out_stride % 8 != 0)
+        return refuse(h, kName, "row strides must hold every head and be multiples of 8 elements");
+    if (query % 16 != 0 || output % 16 != 0 || workspace % 16 != 0)
+        return refuse(h, kName, "query, output and workspace must be 16-byte aligned");
+    if (!(scale > 0.0F) || scale > 3.0e38F) return refuse(h, kName, "requires a positive, finite scale");
+    const int64_t need = kc::paged_attention_workspace_bytes(batch, rows, max_query, q_heads, kv_heads, head_dim,
+                                                             table_width * page_size);
+    if (workspace_bytes < need)
+        return refuse(h, kName, "workspace is smaller than kudacuda_sm100_paged_attention_workspace_bytes()");
+    a.q = P<const void>(query);
+    a.q_stride = q_stride;
+    a.k_pages = P<const void>(k_pages);
+    a.v_pages = P<const void>(v_pages);
+    a.out = P<void>(output);
+    a.out_stride = out_stride;
+    a.lse = P<float>(lse);
+    a.workspace = P<void>(workspace);
+    a.max_query = static_cast<int>(max_query);
+    a.scale = scale;
+    return finish(h, "paged attention", kc::paged_attention(a, dtype, S(stream)));
+}
+
+int kudacuda_sm100_kv_pages_copy(void* raw, uint64_t k_pages, uint64_t v_pages, int64_t layers, int64_t layer_stride,
+                                 int64_t num_pages, int64_t page_bytes, uint64_t pairs, int64_t count,
+                                 uint64_t block_table, int64_t table_stride, int64_t table_rows, int64_t table_width,
+                                 uint64_t page_map, uint64_t stream) {
+    static const char* const kName = "sm100_kv_pages_copy";
+    Handle* h = as_handle(raw);
+    if (!ready(h, "kudacuda_sm100_kv_pages_copy")) return 1;
+    if (layers < 1 || layers > 65536 || num_pages < 1 || num_pages > (int64_t{1} << 30) || page_bytes < 16 ||
+        page_bytes % 16 != 0 || page_bytes > (int64_t{1} << 30) || layer_stride < num_pages * page_bytes ||
+        layer_stride % 16 != 0)
+        return refuse(h, kName, "requires layers, num_pages >= 1, page_bytes a multiple of 16 and layer_stride >= "
+                                "num_pages * page_bytes, a multiple of 16");
+    if (count < 0 || count > num_pages) return refuse(h, kName, "requires 0 <= count <= num_pages");
+    if (k_pages == 0 || v_pages == 0 || (count > 0 && pairs == 0))
+        return refuse(h, kName, "requires non-null device pointers");
+    if (k_pages % 16 != 0 || v_pages % 16 != 0) return refuse(h, kName, "the pages must be 16-byte aligned");
+    if ((block_table != 0) != (page_map != 0))
+        return refuse(h, kName, "a block table and a page map come together");
+    if (block_table != 0 && (table_rows < 0 || table_rows > kc::kMaxGqaBatch || table_width < 0 ||
+                             table_width > (int64_t{1} << 26) || table_stride < table_width))
+        return refuse(h, kName, "requires 0 <= table_rows <= 65536 and table_stride >= table_width >= 0");
+    kc::PagesCopyArgs a;
+    memset(&a, 0, sizeof(a));
+    a.k_pages = P<void>(k_pages);
+    a.v_pages = P<void>(v_pages);
+    a.layer_stride = layer_stride;
+    a.page_bytes = page_bytes;
+    a.layers = static_cast<int>(layers);
+    a.num_pages = static_cast<int>(num_pages);
+    a.pairs = P<const int32_t>(pairs);
+    a.count = static_cast<int>(count);
+    a.table = P<int32_t>(block_table);
+    a.table_stride = table_stride;
+    a.table_rows = static_cast<int>(table_rows);
+    a.table_width = static_cast<int>(table_width);
+    a.page_map = P<const int32_t>(page_map);
+    a.err = h->err_word;
+    return finish(h, "pages_copy_kernel", kc::kv_pages_copy(a, S(stream)));
+}
+
+int kudacuda_sm100_sample(void* raw, int dtype, uint64_t logits, int64_t row_stride, int64_t rows, int64_t vocab,
+                          uint64_t temperature, uint64_t top_k, uint64_t top_p, uint64_t min_p, uint64_t uniform,
+                          uint64_t tokens, uint64_t logprobs, uint64_t stream) {
+    static const char* const kName = "sm100_sample";
+    Handle* h = as_handle(raw);
+    if (!ready(h, "kudacuda_sm100_sample")) return 1;
+    if (dtype != kc::kF32 && dtype != kc::kF16 && dtype != kc::kBF16)
+        return refuse(h, kName, "dtype must be 0 (f32), 1 (f16) or 2 (bf16)");
+    if (rows < 0 || rows > 65535 || vocab < 1 || vocab > (1 << 24) || row_stride < vocab)
+        return refuse(h, kName, "requires 0 <= rows <= 65535, 1 <= vocab <= 2^24 and row_stride >= vocab");
+    if (rows > 0 && (logits == 0 || uniform == 0 || tokens == 0))
+        return refuse(h, kName, "requires non-null logits, uniform and tokens");
+    kc::SampleArgs a;
+    memset(&a, 0, sizeof(a));
+    a.logits = P<const void>(logits);
+    a.row_stride = row_stride;
+    a.rows = static_cast<int>(rows);
+    a.vocab = static_cast<int>(vocab);
+    a.temperature = P<const float>(temperature);
+    a.top_k = P<const int32_t>(top_k);
+    a.top_p = P<const float>(top_p);
+    a.min_p = P<const float>(min_p);
+    a.uniform = P<const float>(uniform);
+    a.tokens = P<int32_t>(tokens);
+    a.logprobs = P<float>(logprobs);
+    return finish(h, "sample_kernel", kc::sample_rows(a, dtype, S(stream)));
+}
+
 const char* kudacuda_sm100_target_arch(void) { return "sm_100a"; }
 
 }  // extern "C"

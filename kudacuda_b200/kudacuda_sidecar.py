@@ -32,6 +32,10 @@ from . import native as _native
 DEFAULT_MANIFEST = Path(__file__).resolve().parent / "manifests" / "b200-sm100.json"
 
 
+# the C ABI's type codes (DType in csrc/kc_launch.h)
+_DTYPE_CODES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+
 class NativeCudaError(RuntimeError):
     """The native library rejected a request or a launch failed."""
 
@@ -1437,6 +1441,196 @@ class KudaCudaBridge:
                    int(workspace.numel()) * int(workspace.element_size()), self._tensor_pointer(tickets, "tickets"),
                    self._tensor_pointer(kv_len, "kv_len"), int(batch), int(kv_stride), int(query_heads),
                    int(kv_heads), int(head_dim), sc, 1 if shared_cache else 0, _normalize_cuda_handle(stream_ptr))
+
+    # ---------------------------------------------------------------- paged KV cache and sampling
+    @staticmethod
+    def _dtype_code(tensor: Any, label: str, allowed: tuple = (1, 2)) -> int:
+        """The C ABI's code of a tensor's type: 0 float32, 1 float16, 2 bfloat16."""
+
+        code = _DTYPE_CODES.get(str(tensor.dtype), -1)
+        if code not in allowed:
+            raise ValueError(f"{label} has an unsupported dtype {tensor.dtype}")
+        return code
+
+    def _int32_array(self, tensor: Any, count: int, label: str) -> int:
+        """Pointer of a contiguous int32 vector of at least ``count`` elements."""
+
+        if str(tensor.dtype) != "torch.int32" or tensor.dim() != 1 or tensor.shape[0] < count or (
+                count > 1 and tensor.stride(0) != 1):
+            raise ValueError(f"{label} must be a contiguous int32 vector of {count} elements")
+        return self._tensor_pointer(tensor, label)
+
+    def _paged_batch(self, k_pages: Any, v_pages: Any, query_start: Any, kv_len: Any, block_table: Any,
+                     code: int) -> tuple[list, tuple[int, int, int, int, int]]:
+        """Checks what the paged entries share; the arguments from query_start to batch, and
+        (batch, num_pages, kv_heads, page_size, head_dim)."""
+
+        shape = tuple(k_pages.shape)
+        if len(shape) != 4 or tuple(v_pages.shape) != shape:
+            raise ValueError("k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
+        if self._dtype_code(k_pages, "k_pages") != code or self._dtype_code(v_pages, "v_pages") != code:
+            raise ValueError("the rows and the pages must have one dtype")
+        if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+            raise ValueError("k_pages and v_pages must be contiguous")
+        if str(block_table.dtype) != "torch.int32" or block_table.dim() != 2:
+            raise ValueError("block_table must be int32 [batch, pages]")
+        batch, width = block_table.shape
+        if width > 1 and block_table.stride(1) != 1:
+            raise ValueError("block_table rows must be contiguous")
+        args = [self._int32_array(query_start, batch + 1, "query_start"), self._int32_array(kv_len, batch, "kv_len"),
+                self._tensor_pointer(block_table, "block_table"),
+                block_table.stride(0) if batch > 1 else width, width, batch]
+        return args, (batch, *shape)
+
+    @staticmethod
+    def _head_rows(tensor: Any, head_dim: int, label: str) -> tuple[int, int, int]:
+        """(rows, columns, row stride) of [rows, heads, head_dim] or [rows, heads * head_dim] with
+        contiguous heads; the row stride is free."""
+
+        shape, stride = tensor.shape, tensor.stride()
+        if len(shape) == 3:
+            cols = shape[1] * shape[2]
+            dense = shape[2] == head_dim and stride[2] == 1 and (shape[1] == 1 or stride[1] == head_dim)
+        elif len(shape) == 2:
+            cols = shape[1]
+            dense = stride[1] == 1
+        else:
+            raise ValueError(f"{label} must be [rows, heads, head_dim] or [rows, heads * head_dim]")
+        if not dense or cols % head_dim:
+            raise ValueError(f"{label} must have contiguous heads of head_dim elements")
+        return shape[0], cols, (stride[0] if shape[0] > 1 else cols)
+
+    def dispatch_rope_append_paged(self, qkv: Any, q_out: Any, k_pages: Any, v_pages: Any, rope_cos: Any,
+                                   rope_sin: Any, query_start: Any, kv_len: Any, block_table: Any, *,
+                                   interleaved: bool = False, bias: Any = None, stream_ptr: int) -> None:
+        """Rotate q and k of a ragged batch of new tokens, write k and v into their pages.
+
+        ``qkv`` [rows, (q_heads + 2 kv_heads) * head_dim], ``q_out`` [rows, q_heads(, *) head_dim],
+        ``rope_cos`` / ``rope_sin`` float32 [max_pos, rotary_dim / 2] (None: no rotation); see
+        kudacuda_sm100_rope_append_paged in include/kudacuda.h."""
+
+        code = self._dtype_code(qkv, "qkv")
+        batch_args, (_, num_pages, kv_heads, page_size, head_dim) = self._paged_batch(
+            k_pages, v_pages, query_start, kv_len, block_table, code)
+        rows, cols, stride = self._head_rows(qkv, head_dim, "qkv")
+        out_rows, out_cols, out_stride = self._head_rows(q_out, head_dim, "q_out")
+        if out_rows != rows or cols != out_cols + 2 * kv_heads * head_dim or self._dtype_code(q_out, "q_out") != code:
+            raise ValueError("q_out must hold the query heads of qkv's rows in its dtype")
+        max_pos = rotary = cos = sin = 0
+        if rope_cos is not None:
+            if (str(rope_cos.dtype) != "torch.float32" or str(rope_sin.dtype) != "torch.float32"
+                    or rope_cos.dim() != 2 or tuple(rope_sin.shape) != tuple(rope_cos.shape)
+                    or not (rope_cos.is_contiguous() and rope_sin.is_contiguous())):
+                raise ValueError("rope_cos and rope_sin must be contiguous float32 [max_pos, rotary_dim / 2]")
+            max_pos, rotary = rope_cos.shape[0], 2 * rope_cos.shape[1]
+            cos, sin = self._tensor_pointer(rope_cos, "rope_cos"), self._tensor_pointer(rope_sin, "rope_sin")
+        if bias is not None and (bias.dim() != 1 or bias.shape[0] != cols or bias.stride(0) != 1
+                                 or self._dtype_code(bias, "bias") != code):
+            raise ValueError("bias must have one element per column of qkv, in its dtype")
+        self._call("kudacuda_sm100_rope_append_paged", code, int(qkv.data_ptr()), stride,
+                   0 if bias is None else int(bias.data_ptr()), int(q_out.data_ptr()), out_stride,
+                   self._tensor_pointer(k_pages, "k_pages"), self._tensor_pointer(v_pages, "v_pages"), cos, sin,
+                   max_pos, rotary, 1 if interleaved else 0, *batch_args, rows, out_cols // head_dim, kv_heads,
+                   head_dim, num_pages, page_size, _normalize_cuda_handle(stream_ptr))
+
+    def paged_attention_workspace(self, query: Any, k_pages: Any, block_table: Any, *, max_query: int) -> Any:
+        """The workspace of dispatch_paged_attention for these shapes (uint8, on the query's device)."""
+
+        import torch
+
+        num_pages, kv_heads, page_size, head_dim = k_pages.shape
+        rows, cols, _ = self._head_rows(query, head_dim, "query")
+        n = int(self.lib.kudacuda_sm100_paged_attention_workspace_bytes(
+            block_table.shape[0], rows, int(max_query), cols // head_dim, kv_heads, head_dim,
+            block_table.shape[1] * page_size))
+        if n < 0:
+            raise NativeCudaError("kudacuda_sm100_paged_attention_workspace_bytes rejected the shape")
+        return torch.empty((max(n, 16),), dtype=torch.uint8, device=query.device)
+
+    def dispatch_paged_attention(self, query: Any, k_pages: Any, v_pages: Any, output: Any, query_start: Any,
+                                 kv_len: Any, block_table: Any, workspace: Any, *, max_query: int,
+                                 scale: float | None = None, lse: Any = None, stream_ptr: int) -> None:
+        """Causal attention of a ragged batch of new tokens over a paged cache that holds them already.
+
+        ``query`` / ``output`` [rows, q_heads, head_dim] (rows may be strided), ``lse`` float32
+        [rows, q_heads] or None; see kudacuda_sm100_paged_attention in include/kudacuda.h."""
+
+        code = self._dtype_code(query, "query")
+        batch_args, (_, num_pages, kv_heads, page_size, head_dim) = self._paged_batch(
+            k_pages, v_pages, query_start, kv_len, block_table, code)
+        rows, cols, stride = self._head_rows(query, head_dim, "query")
+        out_rows, out_cols, out_stride = self._head_rows(output, head_dim, "output")
+        if out_rows != rows or out_cols != cols or self._dtype_code(output, "output") != code:
+            raise ValueError("output must have the query's shape and dtype")
+        if lse is not None and (str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (rows, cols // head_dim)
+                                or not lse.is_contiguous()):
+            raise ValueError("lse must be contiguous float32 [rows, q_heads]")
+        self._call("kudacuda_sm100_paged_attention", code, int(query.data_ptr()), stride,
+                   self._tensor_pointer(k_pages, "k_pages"), self._tensor_pointer(v_pages, "v_pages"),
+                   int(output.data_ptr()), out_stride, 0 if lse is None else int(lse.data_ptr()),
+                   self._tensor_pointer(workspace, "workspace"), workspace.numel() * workspace.element_size(),
+                   *batch_args, rows, int(max_query), cols // head_dim, kv_heads, head_dim, num_pages, page_size,
+                   float(scale) if scale is not None else 1.0 / math.sqrt(head_dim),
+                   _normalize_cuda_handle(stream_ptr))
+
+    def dispatch_kv_pages_copy(self, k_pages: Any, v_pages: Any, pairs: Any, *, block_table: Any = None,
+                               page_map: Any = None, stream_ptr: int) -> None:
+        """Copy pages pairs[:, 0] -> pairs[:, 1] (int32 [n, 2]) of K and V in every layer.
+
+        ``k_pages`` / ``v_pages`` [layers, num_pages, ...]; with ``block_table`` (int32 [rows, pages]) and
+        ``page_map`` (int32 [num_pages]) every valid table entry e becomes page_map[e].  No page may be
+        both a source and a target; see kudacuda_sm100_kv_pages_copy in include/kudacuda.h."""
+
+        shape = tuple(k_pages.shape)
+        if len(shape) < 3 or tuple(v_pages.shape) != shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError("k_pages and v_pages must be [layers, num_pages, ...] of one dtype")
+        if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+            raise ValueError("k_pages and v_pages must be contiguous")
+        if str(pairs.dtype) != "torch.int32" or pairs.dim() != 2 or pairs.shape[1] != 2 or not pairs.is_contiguous():
+            raise ValueError("pairs must be contiguous int32 [n, 2]")
+        layer_bytes = k_pages.stride(0) * k_pages.element_size()
+        table = [0, 0, 0, 0]
+        if (block_table is None) != (page_map is None):
+            raise ValueError("a block table and a page map come together")
+        if block_table is not None:
+            rows, width = block_table.shape
+            if str(block_table.dtype) != "torch.int32" or (width > 1 and block_table.stride(1) != 1):
+                raise ValueError("block_table must be int32 [rows, pages] with contiguous rows")
+            table = [int(block_table.data_ptr()), block_table.stride(0) if rows > 1 else width, rows, width]
+        self._call("kudacuda_sm100_kv_pages_copy", self._tensor_pointer(k_pages, "k_pages"),
+                   self._tensor_pointer(v_pages, "v_pages"), shape[0], layer_bytes, shape[1],
+                   layer_bytes // max(1, shape[1]), int(pairs.data_ptr()), pairs.shape[0], *table,
+                   0 if page_map is None else self._int32_array(page_map, shape[1], "page_map"),
+                   _normalize_cuda_handle(stream_ptr))
+
+    def dispatch_sample(self, logits: Any, tokens: Any, uniform: Any, *, temperature: Any = None, top_k: Any = None,
+                        top_p: Any = None, min_p: Any = None, logprobs: Any = None, stream_ptr: int) -> None:
+        """The next token of every row of ``logits`` [rows, vocab] (float32, float16 or bfloat16; rows may
+        be strided) from one uniform number in [0, 1) per row.
+
+        ``temperature``, ``top_p``, ``min_p`` float32 [rows], ``top_k`` int32 [rows] (None: off);
+        ``tokens`` int32 [rows], ``logprobs`` float32 [rows] or None; see kudacuda_sm100_sample in
+        include/kudacuda.h."""
+
+        if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise ValueError("logits must be [rows, vocab] with contiguous rows")
+        code = self._dtype_code(logits, "logits", (0, 1, 2))
+        rows, vocab = logits.shape
+
+        def column(tensor: Any, dtype: str, label: str, required: bool = False) -> int:
+            if tensor is None and not required:
+                return 0
+            if (str(tensor.dtype) != dtype or tensor.dim() != 1 or tensor.shape[0] != rows
+                    or (rows > 1 and tensor.stride(0) != 1)):
+                raise ValueError(f"{label} must be a contiguous {dtype} vector of {rows} elements")
+            return int(tensor.data_ptr())
+
+        f32, i32 = "torch.float32", "torch.int32"
+        self._call("kudacuda_sm100_sample", code, int(logits.data_ptr()), logits.stride(0) if rows > 1 else vocab,
+                   rows, vocab, column(temperature, f32, "temperature"), column(top_k, i32, "top_k"),
+                   column(top_p, f32, "top_p"), column(min_p, f32, "min_p"), column(uniform, f32, "uniform", True),
+                   column(tokens, i32, "tokens", True), column(logprobs, f32, "logprobs"),
+                   _normalize_cuda_handle(stream_ptr))
 
     def error_word(self, *, clear: bool = True) -> int:
         word = ctypes.c_int(0)

@@ -144,6 +144,22 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "kudacuda_sm100_decode_advance": (_i32, [_p, _u64, _u64, _u64, _i64, _u64]),
     "kudacuda_sm100_graph_step_host": (_i32, [_p, _p, _u64, _i64, _p, _u64, _i64, _u64]),
     "kudacuda_sm100_error_word": (_i32, [_p, ctypes.POINTER(ctypes.c_int), _i32]),
+    # paged KV cache and sampling
+    "kudacuda_sm100_rope_append_paged": (
+        _i32,
+        [_p, _i32, _u64, _i64, _u64, _u64, _i64, _u64, _u64, _u64, _u64, _i64, _i64, _i32, _u64, _u64, _u64]
+        + [_i64] * 9 + [_u64],
+    ),
+    "kudacuda_sm100_paged_attention_workspace_bytes": (_i64, [_i64] * 7),
+    "kudacuda_sm100_paged_attention": (
+        _i32,
+        [_p, _i32, _u64, _i64, _u64, _u64, _u64, _i64, _u64, _u64, _i64, _u64, _u64, _u64] + [_i64] * 10
+        + [_f32, _u64],
+    ),
+    "kudacuda_sm100_kv_pages_copy": (
+        _i32, [_p, _u64, _u64, _i64, _i64, _i64, _i64, _u64, _i64, _u64, _i64, _i64, _i64, _u64, _u64],
+    ),
+    "kudacuda_sm100_sample": (_i32, [_p, _i32, _u64, _i64, _i64, _i64] + [_u64] * 8),
     "kudacuda_sm100_target_arch": (ctypes.c_char_p, []),
     # include/kudacuda_registry.h
     "kudacuda_tactic_count": (_i32, []),

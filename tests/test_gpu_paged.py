@@ -1,0 +1,493 @@
+"""GPU parity of the paged-cache operators and of sampling against plain
+64-bit statements (tests/paged_reference.py).
+
+Tolerances, with u half of the type's spacing at 1 (2^-8 bf16, 2^-11 f16):
+* attention: the output is rounded once (u |o|) and the probabilities that
+  multiply V may be rounded once each (u sum p |v|); 32-bit scores, sums and
+  exponentials add at most 2^-14 sum p |v|.  lse: the scores are 32-bit sums of
+  head_dim products (head_dim 2^-24 sum |q k| scale) plus 2^-18.
+* rotary: one rounding (u |y|) and three 32-bit operations (2^-22 (|x0| + |x1|)).
+* copies and appended values are exact; sampled tokens are equal (the 32-bit
+  exponentials move a boundary by about 1e-6 of the mass, so one of the few
+  hundred fixed draws meets one with probability about 1e-3), log-probabilities
+  within 2^-16 (argument rounding |z| 2^-23, z below 40, and its sum).
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import paged_reference as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def bridge():
+    from kudacuda_b200.kudacuda_sidecar import KudaCudaBridge
+
+    torch.cuda.set_device(0)
+    br = KudaCudaBridge(device_id=0)
+    yield br
+    br.shutdown()
+
+
+def attend(bridge, q, k, v, table, new, lens, *, scale=None, max_query=None, out=None, stream=None):
+    rows, heads, d = q.shape
+    start = R.starts(new, DEV)
+    kv = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    if out is None:
+        out = torch.full((rows, heads, d), 7.0, dtype=q.dtype, device=DEV)
+    lse = torch.full((rows, heads), 7.0, dtype=torch.float32, device=DEV)
+    most = max(new) if max_query is None else max_query
+    ws = bridge.paged_attention_workspace(q, k, table, max_query=most)
+    ws.fill_(0xA5)  # its contents need no initialisation
+    torch.cuda.synchronize()
+    bridge.dispatch_paged_attention(q, k, v, out, start, kv, table, ws, max_query=most, lse=lse, scale=scale,
+                                    stream_ptr=int((stream or torch.cuda.current_stream()).cuda_stream))
+    torch.cuda.synchronize()
+    return out, lse
+
+
+def check_attention(q, new, lens, keys, vals, out, lse, scale):
+    d = q.shape[-1]
+    ref, ref_lse, mag, reach = R.attention(q.cpu(), new, lens, keys, vals, scale)
+    u = R.UNIT[q.dtype]
+    got, got_lse = out.double().cpu(), lse.double().cpu()
+    bound = u * ref.abs() + (u + 2.0**-14) * mag
+    assert torch.isfinite(got).all()
+    bad = (got - ref).abs() > bound
+    assert not bad.any(), f"{int(bad.sum())} outputs off, first at {bad.nonzero()[0].tolist()}"
+    empty = ref_lse == -math.inf
+    assert torch.equal(got_lse == -math.inf, empty)
+    assert (got[empty] == 0).all()
+    lse_bound = d * 2.0**-24 * reach + 2.0**-18
+    diff = torch.where(empty, torch.zeros_like(ref_lse), got_lse - ref_lse).abs()
+    assert (diff <= lse_bound).all(), f"lse off by {float((diff - lse_bound).max())} over its bound"
+
+
+ATTENTION = [
+    # dtype, q_heads, kv_heads, d, page, new tokens, lengths with them
+    (BF16, 16, 2, 128, 16, [1], [1]),
+    (BF16, 16, 2, 128, 16, [1], [509]),
+    (F16, 32, 8, 128, 64, [1, 1, 1], [17, 128, 1000]),
+    (BF16, 16, 2, 128, 32, [1, 1, 0, 1, 1], [0, 5, 33, 2048, 64]),   # an empty sequence, one without new tokens
+    (BF16, 5, 5, 64, 16, [1, 2, 3], [100, 2, 3]),
+    (F16, 7, 1, 64, 128, [1, 1], [300, 129]),
+    (BF16, 28, 4, 128, 16, [3, 1, 5], [257, 600, 5]),
+    (BF16, 16, 2, 128, 64, [4, 2, 9], [1, 2, 400]),                  # more new tokens than the length: empty rows
+    (BF16, 8, 1, 128, 128, [130], [130]),
+    (F16, 32, 8, 128, 16, [77, 1, 31], [77, 333, 200]),
+    (BF16, 2, 2, 64, 32, [65, 200], [129, 260]),
+    (BF16, 15, 3, 128, 16, [40, 0, 27], [50, 10, 411]),              # five heads a group
+    (F16, 24, 2, 64, 16, [19, 33], [97, 64]),                        # twelve heads a group
+    (BF16, 40, 1, 128, 64, [7, 11], [70, 300]),                      # forty heads of one key head
+    (BF16, 16, 16, 128, 64, [129], [515]),
+    (BF16, 4, 1, 128, 64, [300, 1, 60], [1100, 900, 60]),
+    (F16, 160, 1, 64, 16, [2, 1], [40, 19]),                         # more heads a group than a tile has rows
+]
+
+
+@pytest.mark.parametrize("case", range(len(ATTENTION)))
+def test_attention_against_64_bits(bridge, case):
+    dtype, qh, kh, d, page, new, lens = ATTENTION[case]
+    k, v, table, keys, vals = R.make_cache(lens, kh, page, d, dtype, DEV, 100 + case)
+    g = torch.Generator().manual_seed(200 + case)
+    q = (1.5 * torch.randn((sum(new), qh, d), generator=g)).to(dtype).to(DEV)
+    out, lse = attend(bridge, q, k, v, table, new, lens)
+    assert bridge.error_word(clear=True) == 0
+    check_attention(q, new, lens, keys, vals, out, lse, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1], [5000, 9001]), ([70], [3000])])
+def test_attention_scores_far_apart(bridge, new, lens):
+    """Scores to hundreds, the largest at the far end: the running maximum moves late."""
+
+    dtype, qh, kh, d, page = BF16, 8, 2, 128, 64
+    k, v, table, keys, vals = R.make_cache(lens, kh, page, d, dtype, DEV, 31)
+    for b, n in enumerate(lens):  # keys that grow along the sequence
+        gain = torch.linspace(0.1, 6.0, n, dtype=torch.float64)[None, :, None]
+        keys[b] = (keys[b] * gain).to(dtype).double()
+        for j in range((n + page - 1) // page):
+            m = min(page, n - j * page)
+            k[table[b, j], :, :m] = keys[b][:, j * page:j * page + m].to(dtype).to(DEV)
+    g = torch.Generator().manual_seed(32)
+    q = (3.0 * torch.randn((sum(new), qh, d), generator=g)).to(dtype).to(DEV)
+    out, lse = attend(bridge, q, k, v, table, new, lens)
+    assert bridge.error_word(clear=True) == 0
+    check_attention(q, new, lens, keys, vals, out, lse, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [70, 300, 129]), ([90, 3], [200, 77])])
+def test_attention_strided_rows_scale_stream_and_wide_table(bridge, new, lens):
+    """Rows that are a slice of a wider buffer, a table that is a slice of a wider one, a scale of the
+    caller's, a stream other than the current one, no lse."""
+
+    dtype, qh, kh, d, page = BF16, 16, 2, 128, 16
+    k, v, table, keys, vals = R.make_cache(lens, kh, page, d, dtype, DEV, 41, width=40)
+    wide = torch.full((len(lens), 57), 999999, dtype=torch.int32, device=DEV)
+    wide[:, 8:48] = table
+    g = torch.Generator().manual_seed(42)
+    rows = sum(new)
+    full = torch.randn((rows, (qh + 2 * kh) * d), generator=g).to(dtype).to(DEV)
+    q = full[:, :qh * d].view(rows, qh, d)
+    canvas = torch.full((rows, 3 * qh * d), 5.0, dtype=dtype, device=DEV)
+    out = canvas[:, qh * d:2 * qh * d].unflatten(1, (qh, d))
+    stream = torch.cuda.Stream()
+    got, lse = attend(bridge, q, k, v, wide[:, 8:48], new, lens, scale=0.2, out=out, stream=stream)
+    assert bridge.error_word(clear=True) == 0
+    check_attention(q, new, lens, keys, vals, got, lse, 0.2)
+    assert (canvas[:, :qh * d] == 5.0).all() and (canvas[:, 2 * qh * d:] == 5.0).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [60, 1, 17]])
+def test_attention_does_not_depend_on_the_batch_and_repeats(bridge, new):
+    """A second run gives the same bits, and a graph replay too."""
+
+    lens = [600, 77, 1500]
+    k, v, table, keys, vals = R.make_cache(lens, 8, 32, 128, F16, DEV, 51)
+    q = torch.randn((sum(new), 32, 128), generator=torch.Generator().manual_seed(52)).to(F16).to(DEV)
+    first, lse1 = attend(bridge, q, k, v, table, new, lens)
+    second, lse2 = attend(bridge, q, k, v, table, new, lens)
+    assert torch.equal(first, second) and torch.equal(lse1, lse2)
+    start, kv = R.starts(new, DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = torch.zeros_like(first)
+    ws = bridge.paged_attention_workspace(q, k, table, max_query=max(new))
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        bridge.dispatch_paged_attention(q, k, v, out, start, kv, table, ws, max_query=max(new),
+                                        stream_ptr=int(torch.cuda.current_stream().cuda_stream))
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
+    # lengths are device data: the same graph serves shorter ones
+    shorter = [300, 70, 1201]
+    kv.copy_(torch.tensor(shorter, dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    want, _ = attend(bridge, q, k, v, table, new, shorter)
+    assert torch.equal(out, want)
+    assert bridge.error_word(clear=True) == 0
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 3]])
+def test_attention_flags_a_missing_page_and_spares_the_others(bridge, new):
+    lens = [200, 150]
+    k, v, table, keys, vals = R.make_cache(lens, 2, 16, 128, BF16, DEV, 61, junk=0.0)
+    q = torch.randn((sum(new), 16, 128), generator=torch.Generator().manual_seed(62)).to(BF16).to(DEV)
+    good, _ = attend(bridge, q, k, v, table, new, lens)
+    broken = table.clone()
+    broken[0, 3] = k.shape[0] + 5
+    out, _ = attend(bridge, q, k, v, broken, new, lens)
+    assert bridge.error_word(clear=True) == 2
+    assert torch.equal(out[new[0]:], good[new[0]:])
+    # a length past the table
+    out, _ = attend(bridge, q, k, v, table[:, :5], new, lens)
+    assert bridge.error_word(clear=True) == 2
+
+
+def test_attention_no_rows(bridge):
+    k, v, table, _, _ = R.make_cache([5], 2, 16, 128, BF16, DEV, 71)
+    q = torch.empty((0, 16, 128), dtype=BF16, device=DEV)
+    out, _ = attend(bridge, q, k, v, table, [0], [5])
+    assert out.shape[0] == 0 and bridge.error_word(clear=True) == 0
+
+
+def test_attention_offsets_past_32_bits(bridge):
+    """A cache of more than 2^32 elements whose sequences live at its end."""
+
+    page, kh, d = 128, 8, 128
+    num = (1 << 32) // (page * kh * d) + 40
+    if torch.cuda.mem_get_info()[0] < 2.2 * num * page * kh * d * 2:
+        pytest.skip("needs 40 GB of free memory")
+    k = torch.empty((num, kh, page, d), dtype=BF16, device=DEV)
+    v = torch.empty((num, kh, page, d), dtype=BF16, device=DEV)
+    for new, lens in (([1, 1], [700, 300]), ([70, 9], [400, 130])):
+        sk, sv, table, keys, vals = R.make_cache(lens, kh, page, d, BF16, DEV, 81)
+        at = num - sk.shape[0]
+        k[at:], v[at:] = sk, sv
+        q = torch.randn((sum(new), 32, d), generator=torch.Generator().manual_seed(82)).to(BF16).to(DEV)
+        out, lse = attend(bridge, q, k, v, torch.where(table >= 0, table + at, table), new, lens)
+        assert bridge.error_word(clear=True) == 0
+        check_attention(q, new, lens, keys, vals, out, lse, 1 / math.sqrt(d))
+    del k, v
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ rope + append
+def rope_reference(x, cos, sin, interleaved):
+    """x [heads, d] in 64 bits rotated by cos/sin [rot / 2]."""
+
+    y = x.clone()
+    half = cos.shape[0]
+    for i in range(half):
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+        y[:, a] = x[:, a] * cos[i] - x[:, b] * sin[i]
+        y[:, b] = x[:, b] * cos[i] + x[:, a] * sin[i]
+    return y
+
+
+APPEND = [
+    # dtype, q_heads, kv_heads, d, page, rotary, interleaved, bias, new, lengths
+    (BF16, 16, 2, 128, 16, 128, False, True, [1], [1]),
+    (BF16, 16, 2, 128, 64, 128, False, False, [1, 1, 0, 1], [33, 64, 5, 300]),
+    (F16, 5, 5, 64, 32, 32, True, True, [3, 17], [3, 100]),
+    (F16, 7, 1, 64, 16, 64, True, False, [40, 1, 5], [57, 2, 90]),
+    (BF16, 32, 8, 128, 128, 64, False, True, [130, 3], [131, 257]),
+    (BF16, 4, 4, 128, 16, 16, False, False, [9], [20]),
+    (BF16, 3, 3, 128, 16, 0, False, True, [9, 2], [20, 2]),  # no rotation
+]
+
+
+@pytest.mark.parametrize("case", range(len(APPEND)))
+def test_rope_append_against_64_bits(bridge, case):
+    dtype, qh, kh, d, page, rot, inter, has_bias, new, lens = APPEND[case]
+    k, v, table, _, _ = R.make_cache(lens, kh, page, d, dtype, DEV, 300 + case, junk=3.0)
+    g = torch.Generator().manual_seed(400 + case)
+    rows, heads = sum(new), qh + 2 * kh
+    wide = torch.randn((rows, heads * d + 24), generator=g).to(dtype).to(DEV)
+    qkv = wide[:, 8:8 + heads * d]  # strided rows
+    bias = (0.5 * torch.randn((heads * d,), generator=g)).to(dtype).to(DEV) if has_bias else None
+    ang = torch.rand((max(lens) + 2, rot // 2), generator=g, dtype=torch.float64) * 6.28
+    cos, sin = ang.cos().float(), ang.sin().float()
+    q_out = torch.full((rows, qh, d), 9.0, dtype=dtype, device=DEV)
+    start, kv = R.starts(new, DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    before_k, before_v = k.clone(), v.clone()
+    bridge.dispatch_rope_append_paged(qkv, q_out, k, v, cos.to(DEV) if rot else None, sin.to(DEV) if rot else None,
+                                      start, kv, table, interleaved=inter, bias=bias,
+                                      stream_ptr=int(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert bridge.error_word(clear=True) == 0
+    x = qkv.cpu().double()
+    if has_bias:
+        x = (x + bias.cpu().double()).float().to(dtype).double()
+    x = x.view(rows, heads, d)
+    u = R.UNIT[dtype]
+    at = 0
+    for b, (t, n) in enumerate(zip(new, lens)):
+        for i in range(t):
+            pos = n - t + i
+            turned = rope_reference(x[at, :qh + kh], cos[pos].double(), sin[pos].double(), inter)
+            size = rope_reference(x[at, :qh + kh].abs(), torch.ones(rot // 2), -torch.ones(rot // 2), inter).abs()
+            bound = u * turned.abs() + 2.0**-22 * (size + x[at, :qh + kh].abs())
+            assert ((q_out[at].cpu().double() - turned[:qh]).abs() <= bound[:qh]).all()
+            pg, slot = int(table[b, pos // page]), pos % page
+            assert ((k[pg, :, slot].cpu().double() - turned[qh:]).abs() <= bound[qh:]).all()
+            assert torch.equal(v[pg, :, slot].cpu().double(), x[at, qh + kh:])
+            before_k[pg, :, slot] = k[pg, :, slot]
+            before_v[pg, :, slot] = v[pg, :, slot]
+            at += 1
+    # every other slot is as it was
+    assert torch.equal(k, before_k) and torch.equal(v, before_v)
+
+
+def test_rope_append_refuses_positions_and_pages_out_of_range(bridge):
+    new, lens = [2, 1, 1, 3], [40, 17, 16, 2]
+    k, v, table, _, _ = R.make_cache(lens, 2, 16, 64, BF16, DEV, 91, junk=0.0)
+    table[1, 1] = -1            # the page of position 16 is missing
+    qkv = torch.randn((7, 8 * 64), device=DEV).to(BF16)
+    q_out = torch.full((7, 4, 64), 9.0, dtype=BF16, device=DEV)
+    cos = torch.ones((39, 32), device=DEV)  # position 39 has no table row
+    sin = torch.zeros((39, 32), device=DEV)
+    bridge.dispatch_rope_append_paged(qkv, q_out, k, v, cos, sin, R.starts(new, DEV),
+                                      torch.tensor(lens, dtype=torch.int32, device=DEV), table, stream_ptr=0)
+    torch.cuda.synchronize()
+    assert bridge.error_word(clear=True) == 2
+    # written: position 38 of sequence 0, 15 of sequence 2, 0 and 1 of sequence 3
+    for row, ok in enumerate([True, False, False, True, False, True, True]):
+        assert torch.equal(q_out[row].flatten(), qkv[row, :256]) if ok else (q_out[row] == 9.0).all()
+
+
+# ------------------------------------------------------------------ page copies
+@pytest.mark.parametrize("layers,pages,shape,moves,tables", [
+    (1, 5, (2, 16, 64), 1, False), (3, 40, (2, 16, 128), 17, True), (7, 21, (1, 32, 8), 10, True),
+    (2, 9, (3, 128, 128), 4, False), (2, 6, (1, 16, 64), 0, True),
+])
+def test_kv_pages_copy(bridge, layers, pages, shape, moves, tables):
+    g = torch.Generator(device=DEV).manual_seed(pages)
+    k = torch.randn((layers, pages, *shape), generator=g, device=DEV).to(F16)
+    v = torch.randn((layers, pages, *shape), generator=g, device=DEV).to(F16)
+    order = torch.randperm(pages, generator=g, device=DEV).to(torch.int32)
+    pairs = torch.stack([order[:moves], order[moves:2 * moves]], 1).contiguous()
+    want_k, want_v = k.clone(), v.clone()
+    for a, b in pairs.tolist():
+        want_k[:, b] = k[:, a]
+        want_v[:, b] = v[:, a]
+    table = page_map = want = None
+    if tables:
+        wide = torch.randint(-1, pages, (5, 19), generator=g, device=DEV, dtype=torch.int32)
+        wide[0, 3] = pages + 7  # not a page: left alone
+        table = wide[:, 2:13]
+        page_map = torch.arange(pages, dtype=torch.int32, device=DEV)
+        page_map[pairs[:, 0].long()] = pairs[:, 1]
+        want = wide.clone()
+        for r in range(5):
+            for c in range(2, 13):
+                e = int(wide[r, c])
+                want[r, c] = int(page_map[e]) if 0 <= e < pages else e
+    bridge.dispatch_kv_pages_copy(k, v, pairs, block_table=table, page_map=page_map,
+                                  stream_ptr=int(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert bridge.error_word(clear=True) == 0
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+    if tables:
+        assert torch.equal(wide, want)
+
+
+def test_kv_pages_copy_skips_pages_out_of_range(bridge):
+    k = torch.randn((2, 6, 1, 16, 64), device=DEV).to(BF16)
+    v = k + 1
+    want_k, want_v = k.clone(), v.clone()
+    want_k[:, 1], want_v[:, 1] = k[:, 4], v[:, 4]
+    pairs = torch.tensor([[6, 0], [2, -1], [4, 1]], dtype=torch.int32, device=DEV)
+    bridge.dispatch_kv_pages_copy(k, v, pairs, stream_ptr=0)
+    torch.cuda.synchronize()
+    assert bridge.error_word(clear=True) == 2
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
+# ------------------------------------------------------------------ sampling
+def sample(bridge, x, u, t=None, k=None, p=None, low=None):
+    rows = x.shape[0]
+
+    def col(value, dtype):
+        return None if value is None else torch.tensor(value, dtype=dtype, device=DEV)
+
+    tokens = torch.full((rows,), -7, dtype=torch.int32, device=DEV)
+    logp = torch.full((rows,), 7.0, device=DEV)
+    bridge.dispatch_sample(x, tokens, col(u, torch.float32), temperature=col(t, torch.float32),
+                           top_k=col(k, torch.int32), top_p=col(p, torch.float32), min_p=col(low, torch.float32),
+                           logprobs=logp, stream_ptr=int(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    return tokens.tolist(), logp.tolist()
+
+
+def check_rows(bridge, x, u, t, k, p, low):
+    """Against the definition with the parameters as their 32-bit values."""
+
+    tokens, logp = sample(bridge, x, u, t, k, p, low)
+    f32 = lambda v: torch.tensor(v, dtype=torch.float32).double().tolist()  # noqa: E731
+    u, t, p, low = f32(u), f32(t), f32(p), f32(low)
+    for r in range(x.shape[0]):
+        want, want_logp = R.sample_row(x[r].double().tolist(), t[r], k[r], p[r], low[r], u[r])
+        assert tokens[r] == want, f"row {r}: {tokens[r]} for {want}"
+        assert logp[r] == want_logp or abs(logp[r] - want_logp) <= 2.0**-16
+
+
+SETTINGS = [(0.0, 0, 1.0, 0.0), (1.0, 0, 1.0, 0.0), (0.7, 5, 1.0, 0.0), (1.3, 0, 0.6, 0.0), (0.9, 0, 1.0, 0.2),
+            (0.8, 9, 0.8, 0.05), (2.0, 1, 0.5, 0.0), (0.5, 3, 1.0, 1.0), (1.0, 40, 0.999, 0.001), (0.05, 0, 0.9, 0.0),
+            (1.0, 0, 0.0, 0.0), (30.0, 0, 0.95, 0.0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, F16])
+@pytest.mark.parametrize("vocab", [1, 2, 31, 1000, 4097, 33333])
+def test_sample_against_the_definition(bridge, dtype, vocab):
+    g = torch.Generator().manual_seed(vocab)
+    rows = len(SETTINGS) * (2 if vocab > 5000 else 4)
+    wide = (3.0 * torch.randn((rows, vocab + 5), generator=g)).to(dtype).to(DEV)
+    x = wide[:, 3:3 + vocab]  # strided rows at odd offsets
+    u = torch.rand((rows,), generator=g).tolist()
+    cols = [[SETTINGS[r % len(SETTINGS)][c] for r in range(rows)] for c in range(4)]
+    check_rows(bridge, x, u, *cols)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_sample_ties_infinities_and_nan(bridge, dtype):
+    inf, nan = math.inf, math.nan
+    base = [[1.0] * 50, [2.0, 2.0, 1.0, 2.0, 1.0] * 10, [-inf] * 50, [nan] * 50, [-inf] * 49 + [0.5],
+            [nan, 1.0, inf, 0.0, inf] * 10, [0.0, -0.0] * 25, [-inf, 3.0, nan, 3.0, 2.0] * 10,
+            [torch.finfo(dtype).min] * 50, [torch.finfo(dtype).max, torch.finfo(dtype).min] * 25]
+    g = torch.Generator().manual_seed(5)
+    rows, us, cols = [], [], [[], [], [], []]
+    for row in base:
+        for s in SETTINGS:
+            rows.append(row)
+            us.append(float(torch.rand((1,), generator=g)))
+            for c in range(4):
+                cols[c].append(s[c])
+    check_rows(bridge, torch.tensor(rows, dtype=torch.float64).to(dtype).to(DEV), us, *cols)
+
+
+def test_sample_ends_of_the_uniform_range_and_defaults(bridge):
+    x = torch.tensor([[0.0, 1.0, -math.inf, 2.0, -math.inf]] * 4, device=DEV)
+    tokens, logp = sample(bridge, x, [0.0, 1.0 - 2.0**-24, 0.5, 5.0])
+    total = 1 + math.e + math.e**2
+    assert tokens == [0, 3, 3, 3]
+    assert abs(logp[0] + math.log(total)) < 1e-6 and abs(logp[1] - 2 + math.log(total)) < 1e-6
+
+
+def test_sample_follows_the_distribution(bridge):
+    """Uniform numbers on a fine grid give each token its share to within one step of the grid."""
+
+    n, vocab = 4096, 37
+    x = torch.randn((1, vocab), generator=torch.Generator().manual_seed(6)).to(DEV).expand(n, vocab)
+    tokens, _ = sample(bridge, x.contiguous(), [(i + 0.5) / n for i in range(n)])
+    share = torch.bincount(torch.tensor(tokens), minlength=vocab).double() / n
+    assert ((share - torch.softmax(x[0].double().cpu(), 0)).abs() <= 1.01 / n).all()
+
+
+def test_sample_row_does_not_depend_on_its_batch(bridge):
+    g = torch.Generator().manual_seed(7)
+    x = (4.0 * torch.randn((130, 50000), generator=g)).to(BF16).to(DEV)
+    u = torch.rand((130,), generator=g).tolist()
+    cols = [[SETTINGS[r % len(SETTINGS)][c] for r in range(130)] for c in range(4)]
+    whole, lw = sample(bridge, x, u, *cols)
+    for r in (0, 1, 5, 8, 77, 129):
+        one, lo = sample(bridge, x[r:r + 1], u[r:r + 1], *[c[r:r + 1] for c in cols])
+        assert one[0] == whole[r] and lo[0] == lw[r]
+
+
+# ------------------------------------------------------------------ refusals of the C entries
+def test_native_refusals(bridge):
+    from kudacuda_b200.kudacuda_sidecar import NativeCudaError
+
+    k, v, table, _, _ = R.make_cache([40], 2, 16, 128, BF16, DEV, 95)
+    start, kv = R.starts([1], DEV), torch.tensor([40], dtype=torch.int32, device=DEV)
+    q = torch.zeros((1, 16, 128), dtype=BF16, device=DEV)
+    out = torch.empty_like(q)
+    ws = bridge.paged_attention_workspace(q, k, table, max_query=1)
+
+    def attention(**kw):
+        a = dict(q=q, k=k, v=v, out=out, start=start, kv=kv, table=table, ws=ws, max_query=1, scale=None) | kw
+        bridge.dispatch_paged_attention(a["q"], a["k"], a["v"], a["out"], a["start"], a["kv"], a["table"], a["ws"],
+                                        max_query=a["max_query"], scale=a["scale"], stream_ptr=0)
+
+    def pages(shape):
+        return dict(k=torch.zeros(shape, dtype=BF16, device=DEV), v=torch.zeros(shape, dtype=BF16, device=DEV))
+
+    with pytest.raises(NativeCudaError, match="page_size"):
+        attention(**pages((4, 2, 24, 128)))
+    with pytest.raises(NativeCudaError, match="head_dim"):
+        attention(q=torch.zeros((1, 16, 96), dtype=BF16, device=DEV),
+                  out=torch.zeros((1, 16, 96), dtype=BF16, device=DEV), **pages((4, 2, 16, 96)))
+    with pytest.raises(NativeCudaError, match="multiple of kv_heads"):
+        attention(**pages((4, 3, 16, 128)))
+    with pytest.raises(NativeCudaError, match="max_query"):
+        attention(max_query=2)
+    with pytest.raises(NativeCudaError, match="scale"):
+        attention(scale=-1.0)
+    with pytest.raises(NativeCudaError, match="aligned"):
+        attention(q=torch.zeros((2049,), dtype=BF16, device=DEV)[1:].view(1, 16, 128))
+    x = torch.zeros((2, 10), device=DEV)
+    with pytest.raises(NativeCudaError, match="page_bytes"):
+        bridge.dispatch_kv_pages_copy(torch.zeros((1, 4, 3), dtype=BF16, device=DEV),
+                                      torch.zeros((1, 4, 3), dtype=BF16, device=DEV),
+                                      torch.zeros((1, 2), dtype=torch.int32, device=DEV), stream_ptr=0)
+    with pytest.raises(NativeCudaError, match="rotary_dim"):
+        bridge.dispatch_rope_append_paged(torch.zeros((1, 20 * 128), dtype=BF16, device=DEV), out, k, v,
+                                          torch.zeros((64, 20), device=DEV), torch.zeros((64, 20), device=DEV), start,
+                                          kv, table, stream_ptr=0)
+    with pytest.raises(NativeCudaError, match="vocab"):
+        bridge.dispatch_sample(torch.empty((2, 0), device=DEV), torch.zeros((2,), dtype=torch.int32, device=DEV),
+                               x[:, 0].contiguous(), stream_ptr=0)
+    torch.cuda.synchronize()
+    assert bridge.error_word(clear=True) == 0
