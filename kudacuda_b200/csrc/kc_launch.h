@@ -321,6 +321,11 @@ struct PagedAttentionArgs {
 int64_t paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t max_query, int64_t q_heads,
                                         int64_t kv_heads, int64_t head_dim, int64_t max_kv);
 cudaError_t paged_attention(const PagedAttentionArgs& a, int dt, cudaStream_t s);
+// its two kernels (many query rows a key head; few), each with the join of the items it cut
+int64_t paged_chunk_workspace_bytes(int head_dim);
+cudaError_t paged_chunk(const PagedAttentionArgs& a, int dt, cudaStream_t s);
+int64_t paged_decode_workspace_bytes(int head_dim);
+cudaError_t paged_decode(const PagedAttentionArgs& a, int dt, cudaStream_t s);
 struct PagesCopyArgs {
     void* k_pages;
     void* v_pages;

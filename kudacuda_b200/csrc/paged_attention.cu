@@ -66,15 +66,12 @@ __global__ void __launch_bounds__(128) paged_attention_rows_kernel(const PagedAt
 
 int64_t paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t max_query, int64_t q_heads,
                                         int64_t kv_heads, int64_t head_dim, int64_t max_kv) {
-    return 256;
+    return paged_chunk_workspace_bytes(static_cast<int>(head_dim));
 }
 
 cudaError_t paged_attention(const PagedAttentionArgs& a, int dt, cudaStream_t s) {
     if (a.p.rows == 0 || a.p.batch == 0) return cudaSuccess;
-    const int64_t blocks = (static_cast<int64_t>(a.p.rows) * a.p.q_heads + 3) / 4;
-    if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-    return launch_pdl(dt == kBF16 ? paged_attention_rows_kernel<kBF16> : paged_attention_rows_kernel<kF16>,
-                      dim3(static_cast<unsigned>(blocks)), dim3(128), 0, s, a);
+    return paged_chunk(a, dt, s);
 }
 
 }  // namespace kc

@@ -1,0 +1,538 @@
+// paged_chunk.cu -- paged attention with many query rows a key head (chunks of
+// a prompt, mixed steps) on the tcgen05 tensor cores.
+//
+// One CTA per SM takes a stretch of the batch's work (paged_plan.cuh): items
+// of 256 query rows (two tiles of 128: a tile's rows are the tensor memory's
+// lanes) against blocks of 128 keys.  Per block j and tile t
+//   S_t = Q_t K_j^T   (Q, K from shared memory; 128 x 128 fp32 in tensor memory)
+//   P_t = exp2(c S_t - m_t), rounded to the cache's type over S_t's columns
+//   O_t += P_t V_j    (P from tensor memory, V from shared memory, MN-major)
+// with the running maximum m in the log2 domain (c = scale log2 e).  A thread
+// owns one row, so maximum and sum need no exchange.  m only follows the true
+// maximum when that has grown by more than 8 (a factor of 256, far inside fp32
+// and both 16-bit types): O is then rescaled in tensor memory, which is rare.
+// The final O / l does not depend on m.
+//
+// Warps: 0-3 and 4-7 softmax, tile 0 and 1; 8 K/V producer (TMA, one box per
+// page and 64 dims, 128-byte swizzle); 9 MMA issuer; 10 loads Q and clears the
+// rows of the last V block past the item's last key (their P is 0, but 0 times
+// a NaN in an unused slot is not); 11 idle.
+#include <cuda_bf16.h>
+
+#include "kc_common.cuh"
+#include "kc_launch.h"
+#include "kc_tcgen05.cuh"
+#include "kc_tma.h"
+#include "paged_plan.cuh"
+
+namespace kc {
+namespace {
+
+constexpr int kRows = 256;   // query rows of an item
+constexpr int kKeys = 128;   // keys of a block
+constexpr int kThreads = 384;
+constexpr float kLn2 = 0.6931471805599453F;
+constexpr float kLog2E = 1.4426950408889634F;
+constexpr float kLazy = 8.F;  // how far the true maximum may exceed m
+
+template <int D>
+struct ChunkSmem {
+    static constexpr int kHalves = D / 64;
+    static constexpr int kTile = kHalves * 128 * 128;  // 128 rows of Q, K or V: [D / 64][128][128 B]
+    static constexpr int kStages = D == 128 ? 5 : 8;
+    static constexpr int kBytes = 1024 + 2 * kTile + kStages * kTile;
+};
+
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (DT == kBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// the item's last block has rows without a key
+__device__ __forceinline__ bool has_tail(int limit) { return limit % kKeys != 0 || limit == 0; }
+
+struct ChunkBars {
+    uint64_t kv_full[8], kv_empty[8];
+    uint64_t v_tail[8];  // the last V block of an item has landed, rows past its last key not cleared yet
+    uint64_t q_full, q_empty;
+    uint64_t s_full[2], p_ready[2], o_done[2];
+};
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const PagedAttentionArgs a) {
+    using M = ChunkSmem<D>;
+    using W = PagedWalk<kRows, kKeys>;
+    using Part = PagedPartial<kRows, D>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) ChunkBars bars;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    __shared__ int64_t sums[kThreads / 32], place_at;
+    __shared__ int place_seq;
+    const PagedBatch& p = a.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t* const base = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+    uint8_t* const qs = base;
+    uint8_t* const ring = base + 2 * M::kTile;
+
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < M::kStages; ++i) {
+            mbar_init(&bars.kv_full[i], 1);
+            mbar_init(&bars.kv_empty[i], 1);
+            mbar_init(&bars.v_tail[i], 1);
+        }
+        mbar_init(&bars.q_full, 1);
+        mbar_init(&bars.q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_ready[i], 128);
+            mbar_init(&bars.o_done[i], 1);
+        }
+        abort_flag = 0;
+        fence_mbar_init();
+    }
+    tc_fence_before();
+    pdl_wait_on_producer();
+    const int group = p.q_heads / p.kv_heads;
+    const int worker = blockIdx.x, workers = gridDim.x;
+    const int64_t total = paged_places<kRows, kKeys, kThreads>(p, group, worker, 1, workers, sums, &place_seq, &place_at);
+    tc_fence_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = tmem_slot;
+    volatile int* const abort_p = &abort_flag;
+    W w;
+    w.begin(p, group, paged_bound(total, worker, workers), paged_bound(total, worker + 1, workers), place_seq, place_at);
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) {
+            // ---- K/V producer: K_0, V_0, K_1, V_1, ... of every piece through the ring
+            uint32_t seq = 0, tail_use = 0, tail_parity = 0;  // per stage: its last copy was a tail, tails so far
+            bool ok = true;
+            while (ok && w.next(p, group)) {
+                const int32_t* table = p.table + w.piece_b * p.table_stride;
+                for (int j = w.t0; j < w.t1 && ok; ++j) {
+                    const int pages = min(kKeys, w.limit - j * kKeys + p.page_size - 1) / p.page_size;
+                    const int part = lane / M::kHalves, half = lane % M::kHalves;
+                    const bool mine = part < pages;
+                    int row = 0;
+                    if (mine) {
+                        const int page = table[j * (kKeys / p.page_size) + part];
+                        // a missing page reads as zeros: a box that begins before the tensor
+                        row = -p.page_size;
+                        if (page >= 0 && page < p.num_pages) row = (page * p.kv_heads + w.kvh) * p.page_size;
+                        else if (half == 0 && p.err != nullptr) atomicOr(p.err, 2);
+                    }
+                    for (int v = 0; v < 2; ++v, ++seq) {
+                        const int s = seq % M::kStages;
+                        if (seq >= M::kStages) ok = bar_wait(&bars.kv_empty[s], (seq / M::kStages - 1) & 1, abort_p);
+                        if (!ok) break;
+                        // the tail of V goes through warp 10, which then completes kv_full
+                        const bool tail = v == 1 && j == w.tiles - 1 && has_tail(w.limit);
+                        tail_use = tail ? tail_use | 1u << s : tail_use & ~(1u << s);
+                        if (tail) tail_parity ^= 1u << s;
+                        uint64_t* const full = tail ? &bars.v_tail[s] : &bars.kv_full[s];
+                        if (lane == 0) mbar_arrive_expect_tx(full, pages * p.page_size * 128 * M::kHalves);
+                        __syncwarp();
+                        if (mine)
+                            tma_load_2d(ring + s * M::kTile + half * (128 * 128) + part * p.page_size * 128,
+                                        v ? &map_v : &map_k, half * 64, row, full);
+                    }
+                }
+                if (w.piece_len > p.table_width * p.page_size && lane == 0 && p.err != nullptr) atomicOr(p.err, 2);
+            }
+            // every copy has landed before the CTA may exit (normally already true)
+            const uint32_t first = seq > M::kStages ? seq - M::kStages : 0;
+            for (uint32_t i = first; i < seq; ++i) {
+                const uint32_t s = i % M::kStages;
+                if (tail_use >> s & 1) bar_wait(&bars.v_tail[s], ~tail_parity >> s & 1, abort_p, false);
+                else bar_wait(&bars.kv_full[s], (i / M::kStages) & 1, abort_p, false);
+            }
+        } else if (warp == 9) {
+            // ---- MMA issuer
+            if (lane == 0) {
+                constexpr uint32_t kIdescS = umma_idesc(DT == kBF16, 128, 128, false);
+                constexpr uint32_t kIdescO = umma_idesc(DT == kBF16, 128, D, true);
+                uint32_t seq = 0, items = 0, np[2] = {0, 0};
+                const uint32_t q_addr = smem_u32(qs), r_addr = smem_u32(ring);
+                while (w.next(p, group)) {
+                    const int active = w.item_rows > 128 ? 2 : 1;
+                    const int n = w.t1 - w.t0;
+                    bar_wait(&bars.q_full, items & 1, abort_p);
+                    for (int j = 0; j <= n; ++j) {
+                        // O_t += P_t(j - 1) V(j - 1), then S_t = Q_t K(j)^T over P_t(j - 1)'s
+                        // columns: the matrix instructions of one thread run in order
+                        const uint32_t sv = seq + 2 * j - 1, sk = seq + 2 * j;
+                        if (j > 0) bar_wait(&bars.kv_full[sv % M::kStages], (sv / M::kStages) & 1, abort_p);
+                        if (j < n) bar_wait(&bars.kv_full[sk % M::kStages], (sk / M::kStages) & 1, abort_p);
+                        tc_fence_after();
+                        const uint32_t va = r_addr + (sv % M::kStages) * M::kTile;
+                        const uint32_t ka = r_addr + (sk % M::kStages) * M::kTile;
+                        for (int t = 0; t < active; ++t) {
+                            if (j > 0) {
+                                bar_wait(&bars.p_ready[t], np[t]++ & 1, abort_p);
+                                tc_fence_after();
+#pragma unroll
+                                for (int k = 0; k < kKeys / 16; ++k)
+                                    umma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
+                                                 umma_desc_sw128_mn(va + 2048 * k, 128 * 128), kIdescO,
+                                                 (j > 1 || k > 0) ? 1u : 0u);
+                            }
+                            if (j < n) {
+#pragma unroll
+                                for (int k = 0; k < D / 16; ++k) {
+                                    const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
+                                    umma_bf16(tmem + t * 128, umma_desc_sw128(q_addr + t * M::kTile + off),
+                                              umma_desc_sw128(ka + off), kIdescS, k > 0 ? 1u : 0u);
+                                }
+                                umma_commit(&bars.s_full[t]);
+                            } else {
+                                umma_commit(&bars.o_done[t]);
+                            }
+                            if (t == active - 1) {
+                                if (j > 0) umma_commit(&bars.kv_empty[sv % M::kStages]);
+                                if (j < n) umma_commit(&bars.kv_empty[sk % M::kStages]);
+                                if (j == n - 1) umma_commit(&bars.q_empty);
+                            }
+                        }
+                    }
+                    seq += 2 * n;
+                    ++items;
+                }
+            }
+        } else if (warp == 10) {
+            // ---- Q: row R of the item is token R / group, head R % group; rows past the item are zero
+            uint32_t items = 0, seq = 0, tail_parity = 0;
+            const uint16_t* q = static_cast<const uint16_t*>(a.q);
+            constexpr int kChunks = D / 8, kAbreast = 32 / kChunks;  // 16-byte chunks of a row, rows a pass
+            const int c = lane % kChunks, sub = lane / kChunks;
+            while (w.next(p, group)) {
+                // (a long wait: the whole of the piece before)
+                if (items > 0 && !bar_wait(&bars.q_empty, (items - 1) & 1, abort_p, true, 1u << 22)) break;
+                const int r_all = w.item_rows > 128 ? 256 : 128;
+                int token = (w.q * kRows + sub) / group, head = (w.q * kRows + sub) % group;
+                for (int r = sub; r < r_all; r += kAbreast) {
+                    const uint32_t dst = smem_u32(qs) + (r >> 7) * M::kTile + (c >> 3) * (128 * 128) + (r & 127) * 128 +
+                                         (((c & 7) ^ (r & 7)) << 4);
+                    const bool live = r < w.item_rows;
+                    const uint16_t* src =
+                        q + (live ? (w.piece_start + token) * a.q_stride +
+                                        static_cast<int64_t>(w.kvh * group + head) * D + c * 8
+                                  : 0);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                                 "r"(live ? 16 : 0)
+                                 : "memory");
+                    head += kAbreast;
+                    while (head >= group) {
+                        head -= group;
+                        ++token;
+                    }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.q_full);
+                ++items;
+                seq += 2 * (w.t1 - w.t0);
+                if (w.t1 == w.tiles && has_tail(w.limit)) {
+                    const uint32_t sv = (seq - 1) % M::kStages;  // the piece's last V block
+                    if (!bar_wait(&bars.v_tail[sv], tail_parity >> sv & 1, abort_p, true, 1u << 22)) break;
+                    tail_parity ^= 1u << sv;
+                    const int from = w.limit - (w.tiles - 1) * kKeys;  // rows from here on hold no key
+                    uint8_t* v = ring + sv * M::kTile;
+                    for (int i = from * 8 + lane; i < 128 * 8; i += 32)
+#pragma unroll
+                        for (int h = 0; h < M::kHalves; ++h)
+                            *reinterpret_cast<uint4*>(v + h * (128 * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&bars.kv_full[sv]);
+                }
+            }
+        }
+    } else {
+        // ---- softmax: thread = row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int t = warp >> 2;
+        const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
+        const int r = t * 128 + 32 * (warp & 3) + lane;
+        const float c = a.scale * kLog2E;
+        uint32_t ns = 0, no = 0;
+        while (w.next(p, group)) {
+            if (t == 1 && w.item_rows <= 128) continue;
+            const bool live = r < w.item_rows;
+            const int token = (w.q * kRows + r) / group;
+            // this row's keys, relative to the item: never more than the item's
+            const int row_keys = live ? min(max(w.piece_len - w.piece_n + token + 1, 0), w.limit) : w.limit;
+            float m = -INFINITY, l = 0.F;
+            for (int j = w.t0; j < w.t1; ++j) {
+                bar_wait(&bars.s_full[t], ns++ & 1, abort_p);
+                tc_fence_after();
+                float s[kKeys];
+#pragma unroll
+                for (int i = 0; i < kKeys; i += 32) tmem_ld32(ts + i, s + i);
+                tmem_wait_ld();
+                const int keys = row_keys - j * kKeys;
+                if (__any_sync(0xffffffffu, keys < kKeys)) {
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) s[i] = i < keys ? s[i] : -INFINITY;
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < kKeys; i += 4) {
+                    mx[0] = fmaxf(mx[0], s[i]);
+                    mx[1] = fmaxf(mx[1], s[i + 1]);
+                    mx[2] = fmaxf(mx[2], s[i + 2]);
+                    mx[3] = fmaxf(mx[3], s[i + 3]);
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                const bool grow = top > m + kLazy;  // from -inf: any finite maximum
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float mn = grow ? top : m;
+                    const float f = grow ? ex2(m - mn) : 1.F;
+                    l *= f;
+                    m = mn;
+                    if (j > w.t0) {
+                        // S_t(j) is complete, so every earlier matrix instruction on O_t is too
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 32) {
+                            float o[32];
+                            tmem_ld32(to + i, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] *= f;
+                            tmem_st32(to + i, reinterpret_cast<uint32_t*>(o));
+                        }
+                    }
+                }
+                const float sub = m == -INFINITY ? 0.F : m;
+                float sum[4] = {0.F, 0.F, 0.F, 0.F};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float e0 = ex2(fmaf(s[64 * h + 2 * i], c, -sub));
+                        const float e1 = ex2(fmaf(s[64 * h + 2 * i + 1], c, -sub));
+                        sum[(2 * i) & 3] += e0;
+                        sum[(2 * i + 1) & 3] += e1;
+                        pk[i] = pack2<DT>(e0, e1);
+                    }
+                    tmem_st32(ts + 32 * h, pk);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                bar_arrive(&bars.p_ready[t]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            // ---- the piece's end
+            bar_wait(&bars.o_done[t], no++ & 1, abort_p);
+            tc_fence_after();
+            if (w.whole()) {
+                const float inv = l > 0.F ? 1.F / l : 0.F;
+                const int64_t row = w.piece_start + token;
+                const int head = w.kvh * group + (w.q * kRows + r) % group;
+                uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
+#pragma unroll 1
+                for (int i = 0; i < D; i += 32) {
+                    float o[32];
+                    tmem_ld32(to + i, o);
+                    tmem_wait_ld();
+                    if (live) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8)
+                            *reinterpret_cast<uint4*>(out + i + k) =
+                                make_uint4(pack2<DT>(o[k] * inv, o[k + 1] * inv), pack2<DT>(o[k + 2] * inv, o[k + 3] * inv),
+                                           pack2<DT>(o[k + 4] * inv, o[k + 5] * inv), pack2<DT>(o[k + 6] * inv, o[k + 7] * inv));
+                    }
+                }
+                if (live && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
+            } else {
+                float* part = Part::slot(a.workspace, workers, worker, w.t0 > 0 ? 0 : 1);
+                *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, l);
+                float4* acc = reinterpret_cast<float4*>(part + 2 * kRows);
+#pragma unroll 1
+                for (int i = 0; i < D; i += 32) {
+                    float o[32];
+                    tmem_ld32(to + i, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        __stcg(acc + ((i + k) >> 2) * kRows + r, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    // what the combine kernel needs to know of this worker's cut items
+    if (tid == 352) {
+        W v;
+        v.begin(p, group, paged_bound(total, worker, workers), paged_bound(total, worker + 1, workers), place_seq, place_at);
+        PagedCut cut;
+        cut.valid = cut.tail = cut.row0 = cut.r0 = cut.rows = cut.kvh = cut.last = cut.pad = 0;
+        while (v.next(p, group)) {
+            if (v.t0 > 0) cut.tail = 1;
+            else if (v.t1 < v.tiles) {
+                cut.valid = 1;
+                cut.row0 = v.piece_start;
+                cut.r0 = v.q * kRows;
+                cut.rows = v.item_rows;
+                cut.kvh = v.kvh;
+                cut.last = static_cast<int>((v.item_end * workers + total - 1) / total - 1);
+            }
+        }
+        Part::cuts(a.workspace)[worker] = cut;
+    }
+    if (tid == 0 && *abort_p && p.err != nullptr) atomicOr(p.err, 16);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// The join of cut items: with M the largest of the pieces' maxima,
+// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the pieces
+// (the same bits on every run).  One block per worker that began a cut item
+// and 32 of the item's rows: lane = row, warp = a share of the dims.
+template <int DT, int D, int ROWS>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedAttentionArgs a, int workers) {
+    using Part = PagedPartial<ROWS, D>;
+    pdl_launch_dependents();
+    pdl_wait_on_producer();
+    const int owner = blockIdx.x;
+    const PagedCut* cuts = Part::cuts(a.workspace);
+    const PagedCut cut = cuts[owner];
+    constexpr int kLanes = ROWS < 32 ? ROWS : 32, kShares = 256 / kLanes;
+    const int lane = threadIdx.x % kLanes, share = threadIdx.x / kLanes;
+    const int r = blockIdx.y * kLanes + lane;
+    if (!cut.valid || r >= cut.rows) return;
+    constexpr int kVecs = (D / 4 + kShares - 1) / kShares;  // float4 of a thread
+    float m = -INFINITY, l = 0.F;
+    float4 acc[kVecs];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) acc[i] = make_float4(0.F, 0.F, 0.F, 0.F);
+    for (int c = owner; c <= cut.last && c < workers; ++c) {
+        if (c > owner && !cuts[c].tail) continue;
+        const float* part = Part::slot(a.workspace, workers, c, c == owner ? 1 : 0);
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part) + r);
+        const float mn = fmaxf(m, ml.x);
+        const float f = m == -INFINITY ? 0.F : exp2f(m - mn), g = ml.x == -INFINITY ? 0.F : exp2f(ml.x - mn);
+        l = l * f + ml.y * g;
+        const float4* o = reinterpret_cast<const float4*>(part + 2 * ROWS);
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const int v = share + i * kShares;
+            if (v >= D / 4) break;
+            const float4 x = __ldcg(o + v * ROWS + r);
+            acc[i].x = acc[i].x * f + x.x * g;
+            acc[i].y = acc[i].y * f + x.y * g;
+            acc[i].z = acc[i].z * f + x.z * g;
+            acc[i].w = acc[i].w * f + x.w * g;
+        }
+        m = mn;
+    }
+    const PagedBatch& p = a.p;
+    const int group = p.q_heads / p.kv_heads;
+    const int64_t row = cut.row0 + (cut.r0 + r) / group;
+    const int head = cut.kvh * group + (cut.r0 + r) % group;
+    const float inv = l > 0.F ? 1.F / l : 0.F;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+        const int v = share + i * kShares;
+        if (v >= D / 4) break;
+        *reinterpret_cast<uint2*>(out + 4 * v) = make_uint2(pack2<DT>(acc[i].x * inv, acc[i].y * inv),
+                                                            pack2<DT>(acc[i].z * inv, acc[i].w * inv));
+    }
+    if (share == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
+}
+
+namespace {
+constexpr int kMaxWorkers = 148;
+
+template <int DT, int D>
+cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t s) {
+    const PagedBatch& p = a.p;
+    const uint64_t rows = static_cast<uint64_t>(p.num_pages) * p.kv_heads * p.page_size;
+    CUtensorMap mk, mv;
+    const CUtensorMapDataType type =
+        DT == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    cudaError_t st = encode_tmap_2d(&mk, type, a.k_pages, D, rows, D * 2, 64, p.page_size, CU_TENSOR_MAP_SWIZZLE_128B,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (st == cudaSuccess)
+        st = encode_tmap_2d(&mv, type, a.v_pages, D, rows, D * 2, 64, p.page_size, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (st != cudaSuccess) return st;
+    auto kernel = paged_chunk_kernel<DT, D>;
+    static bool opted[64] = {};
+    const int dev = current_device_index();
+    if (dev < 0 || dev >= 64 || !opted[dev]) {
+        st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem<D>::kBytes);
+        if (st != cudaSuccess) return st;
+        if (dev >= 0 && dev < 64) opted[dev] = true;
+    }
+    const int workers = device_sm_count() < kMaxWorkers ? device_sm_count() : kMaxWorkers;
+    st = launch_pdl(kernel, dim3(workers), dim3(kThreads), ChunkSmem<D>::kBytes, s, mk, mv, a);
+    if (st != cudaSuccess) return st;
+    return launch_pdl(paged_combine_kernel<DT, D, kRows>, dim3(workers, kRows / 32), dim3(256), 0, s, a, workers);
+}
+}  // namespace
+
+int64_t paged_chunk_workspace_bytes(int head_dim) {
+    return head_dim == 128 ? PagedPartial<kRows, 128>::bytes(kMaxWorkers) : PagedPartial<kRows, 64>::bytes(kMaxWorkers);
+}
+
+cudaError_t paged_chunk(const PagedAttentionArgs& a, int dt, cudaStream_t s) {
+    if (dt == kBF16) return a.p.head_dim == 128 ? launch_chunk<kBF16, 128>(a, s) : launch_chunk<kBF16, 64>(a, s);
+    return a.p.head_dim == 128 ? launch_chunk<kF16, 128>(a, s) : launch_chunk<kF16, 64>(a, s);
+}
+
+}  // namespace kc

@@ -1,0 +1,210 @@
+// paged_plan.cuh -- how the work of a ragged batch of paged attention is
+// shared out.
+//
+// A sequence with n new tokens and G query heads per key head has n * G query
+// rows per key head (row R: token R / G, head R % G); ROWS of them are a tile,
+// and (sequence, key head, tile) is an item whose keys come in blocks of KT.
+// Every item has a cost (its last row's keys, counted per query row, and one
+// block for its start and end), the items stand in one line, and worker c of N
+// takes the stretch [c U / N, (c + 1) U / N) of the total cost U.  A stretch
+// that ends inside an item is rounded down to a block, by the same formula for
+// both neighbours, so lengths of any mix load every worker alike and an item
+// is cut only where a stretch ends.  A cut item's pieces are left as partial
+// results (accumulator, maximum, sum) and joined by the combine kernel.
+//
+// The costs have a closed form per sequence, so a worker finds its place from
+// the lengths alone: no host work and no plan kernel, and the lengths may
+// change under a captured graph.
+#pragma once
+
+#include "kc_common.cuh"
+#include "kc_launch.h"
+
+namespace kc {
+
+// one per worker: the cut item that this worker began, for the combine kernel
+struct PagedCut {
+    int valid;      // 1: an item is cut and this worker has its first piece
+    int tail;       // 1: this worker has a piece of an item begun earlier (slot 0)
+    int row0;       // first query row of the item in the batch's rows (token row)
+    int r0, rows;   // first tile row R and the number of rows
+    int kvh;
+    int last;       // last worker that may have a piece of the item
+    int pad;
+};
+
+__device__ __forceinline__ int64_t paged_bound(int64_t total, int worker, int workers) {
+    return total * worker / workers;
+}
+
+struct PagedSeq {
+    int start, n, len;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& p, int b) {
+    PagedSeq s;
+    const int a = p.query_start[b], e = p.query_start[b + 1], l = p.kv_len[b];
+    s.start = min(max(a, 0), p.rows);
+    s.n = min(max(e, s.start), p.rows) - s.start;
+    s.len = max(l, 0);
+    return s;
+}
+
+template <int ROWS, int KT>
+struct PagedWalk {
+    // the line
+    int64_t x0, x1;
+    // the sequence at hand
+    int b, start, n, len, rows, tiles_q;
+    int64_t head_cost, head_at;  // cost of one key head of it; where the current one begins
+    int next_kvh, next_q;
+    // the piece at hand
+    int piece_b, piece_start, piece_n, piece_len;
+    int kvh, q, item_rows, limit, t0, t1, tiles;
+    int64_t item_end;
+
+    // cost of the first k tiles of a key head
+    __device__ __forceinline__ int64_t cost(int group, int k) const {
+        const int64_t base = static_cast<int64_t>(max(len - n, 0) + KT) * group;
+        if (k >= tiles_q)
+            return tiles_q * base + static_cast<int64_t>(ROWS / 2) * (tiles_q - 1) * tiles_q + rows;
+        return k * base + static_cast<int64_t>(ROWS / 2) * k * (k + 1);
+    }
+    __device__ __forceinline__ void load(const PagedBatch& p, int group) {
+        const PagedSeq s = paged_seq(p, b);
+        start = s.start;
+        n = s.n;
+        len = s.len;
+        rows = n * group;
+        tiles_q = (rows + ROWS - 1) / ROWS;
+        head_cost = tiles_q > 0 ? cost(group, tiles_q) : 0;
+    }
+    __device__ __forceinline__ void skip_empty(const PagedBatch& p, int group) {
+        while (b < p.batch) {
+            load(p, group);
+            if (tiles_q > 0) return;
+            ++b;
+        }
+    }
+    // the stretch [from, to), which begins in or after sequence `seq`, whose cost begins at `at`
+    __device__ __forceinline__ void begin(const PagedBatch& p, int group, int64_t from, int64_t to, int seq,
+                                          int64_t at) {
+        x0 = from;
+        x1 = to;
+        b = seq;
+        head_at = at;
+        next_kvh = next_q = 0;
+        tiles_q = 0;
+        skip_empty(p, group);
+        if (b >= p.batch || x0 <= at) return;
+        const int64_t rem = x0 - at;
+        next_kvh = static_cast<int>(min(rem / head_cost, static_cast<int64_t>(p.kv_heads - 1)));
+        head_at = at + next_kvh * head_cost;
+        int lo = 0, hi = tiles_q - 1;  // the last tile that begins at or before x0
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (head_at + cost(group, mid) <= x0) lo = mid;
+            else hi = mid - 1;
+        }
+        next_q = lo;
+    }
+    // the next piece with a block in it
+    __device__ __forceinline__ bool next(const PagedBatch& p, int group) {
+        while (b < p.batch) {
+            const int64_t lo = head_at + cost(group, next_q), hi = head_at + cost(group, next_q + 1);
+            if (lo >= x1) return false;
+            kvh = next_kvh;
+            q = next_q;
+            item_end = hi;
+            item_rows = min(ROWS, rows - q * ROWS);
+            const int last_token = (q * ROWS + item_rows - 1) / group;
+            limit = min(max(len - n + last_token + 1, 0), p.table_width * p.page_size);
+            tiles = max((limit + KT - 1) / KT, 1);
+            t0 = x0 <= lo ? 0 : static_cast<int>((x0 - lo) * tiles / (hi - lo));
+            t1 = x1 >= hi ? tiles : static_cast<int>((x1 - lo) * tiles / (hi - lo));
+            piece_b = b;
+            piece_start = start;
+            piece_n = n;
+            piece_len = len;
+            if (++next_q == tiles_q) {
+                next_q = 0;
+                head_at += head_cost;
+                if (++next_kvh == p.kv_heads) {
+                    next_kvh = 0;
+                    ++b;
+                    skip_empty(p, group);
+                }
+            }
+            if (t0 < t1) return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
+};
+
+// Block-wide: the total cost, and for `count` workers first .. first + count - 1
+// of `workers` the sequence in which each one's stretch begins (seq) and that
+// sequence's place (at).  `sums` has one word per warp.  Ends with a barrier.
+template <int ROWS, int KT, int THREADS>
+__device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, int first, int count, int workers,
+                                                int64_t* sums, int* seq, int64_t* at) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int b0 = static_cast<int>(static_cast<int64_t>(p.batch) * tid / THREADS);
+    const int b1 = static_cast<int>(static_cast<int64_t>(p.batch) * (tid + 1) / THREADS);
+    PagedWalk<ROWS, KT> w;
+    int64_t mine = 0;
+    for (w.b = b0; w.b < b1; ++w.b) {
+        w.load(p, group);
+        mine += w.head_cost * p.kv_heads;
+    }
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    if (tid < count) {
+        seq[tid] = p.batch;
+        at[tid] = 0;
+    }
+    __syncthreads();
+    int64_t total = 0, before = 0;
+    for (int i = 0; i < THREADS / 32; ++i) {
+        if (i < warp) before += sums[i];
+        total += sums[i];
+    }
+    int64_t from = before + upto - mine;
+    for (int i = 0; i < count; ++i) {
+        const int64_t x = paged_bound(total, first + i, workers);
+        if (mine == 0 || x < from || x >= from + mine) continue;
+        int64_t c = from;
+        for (w.b = b0; w.b < b1; ++w.b) {
+            w.load(p, group);
+            const int64_t e = c + w.head_cost * p.kv_heads;
+            if (x < e) break;
+            c = e;
+        }
+        seq[i] = w.b;
+        at[i] = c;
+    }
+    __syncthreads();
+    return total;
+}
+
+// Where a worker's partial results lie: slot 0 the end of an item begun by an
+// earlier worker, slot 1 the beginning of an item that later ones end.  A slot
+// is ROWS (maximum, sum) pairs and the accumulator as float4 [D / 4][ROWS].
+template <int ROWS, int D>
+struct PagedPartial {
+    static constexpr int64_t kFloats = static_cast<int64_t>(ROWS) * (D + 2);
+    static __host__ __device__ int64_t bytes(int64_t workers) {
+        return (workers * sizeof(PagedCut) + 255) / 256 * 256 + workers * 2 * kFloats * 4;
+    }
+    static __device__ __forceinline__ PagedCut* cuts(void* ws) { return static_cast<PagedCut*>(ws); }
+    static __device__ __forceinline__ float* slot(void* ws, int workers, int worker, int s) {
+        char* base = static_cast<char*>(ws) + (static_cast<int64_t>(workers) * sizeof(PagedCut) + 255) / 256 * 256;
+        return reinterpret_cast<float*>(base) + (static_cast<int64_t>(worker) * 2 + s) * kFloats;
+    }
+};
+
+}  // namespace kc

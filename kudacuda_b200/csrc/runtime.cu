@@ -1734,8 +1734,8 @@ const char* paged_batch(kc::PagedBatch* p, Handle* h, int dtype, uint64_t k_page
         return "page_size must be 16, 32, 64 or 128";
     if (num_pages < 1 || num_pages * kv_heads * page_size > (int64_t{1} << 31) - 1)
         return "requires num_pages >= 1 and num_pages * kv_heads * page_size < 2^31";
-    if (table_width < 1 || table_width * page_size > (int64_t{1} << 30) || table_stride < table_width)
-        return "requires table_width >= 1, table_width * page_size <= 2^30 and table_stride >= table_width";
+    if (table_width < 1 || table_width * page_size > (int64_t{1} << 27) || table_stride < table_width)
+        return "requires table_width >= 1, table_width * page_size <= 2^27 and table_stride >= table_width";
     if (k_pages == 0 || v_pages == 0 || query_start == 0 || kv_len == 0 || block_table == 0)
         return "requires non-null device pointers";
     if (k_pages % 16 != 0 || v_pages % 16 != 0) return "the pages must be 16-byte aligned";
@@ -1805,7 +1805,7 @@ int64_t kudacuda_sm100_paged_attention_workspace_bytes(int64_t batch, int64_t ro
                                                        int64_t max_kv) {
     if (batch < 0 || batch > kc::kMaxGqaBatch || rows < 0 || rows > (int64_t{1} << 24) || max_query < 0 ||
         kv_heads < 1 || q_heads < kv_heads || q_heads > kc::kMaxGqaHeads || q_heads % kv_heads != 0 ||
-        (head_dim != 64 && head_dim != 128) || max_kv < 0 || max_kv > (int64_t{1} << 30))
+        (head_dim != 64 && head_dim != 128) || max_kv < 0 || max_kv > (int64_t{1} << 27))
         return -1;
     return kc::paged_attention_workspace_bytes(batch, rows, max_query, q_heads, kv_heads, head_dim, max_kv);
 }
