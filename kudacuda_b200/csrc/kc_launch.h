@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace kc {
@@ -39,6 +40,17 @@ size_t device_smem_per_sm();
 size_t device_smem_per_block_optin();
 size_t device_smem_reserved_per_block();
 int current_device_index();
+
+// Allow `kernel` up to `bytes` of dynamic shared memory, once per device
+// (`done`: one bit per device, zero at first, one word per kernel).
+inline cudaError_t opt_in_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    const int dev = current_device_index();
+    const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t{1} << dev : 0;
+    if (bit != 0 && (done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+    const cudaError_t st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (st == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return st;
+}
 
 // ---- NF4 GEMV family -------------------------------------------------------
 // dtype codes: 0 = f32, 1 = f16, 2 = bf16

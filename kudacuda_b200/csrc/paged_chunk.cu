@@ -512,13 +512,9 @@ cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t s) {
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     if (st != cudaSuccess) return st;
     auto kernel = paged_chunk_kernel<DT, D>;
-    static bool opted[64] = {};
-    const int dev = current_device_index();
-    if (dev < 0 || dev >= 64 || !opted[dev]) {
-        st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem<D>::kBytes);
-        if (st != cudaSuccess) return st;
-        if (dev >= 0 && dev < 64) opted[dev] = true;
-    }
+    static std::atomic<uint64_t> opted{0};
+    st = opt_in_smem(reinterpret_cast<const void*>(kernel), ChunkSmem<D>::kBytes, opted);
+    if (st != cudaSuccess) return st;
     const int workers = device_sm_count() < kMaxWorkers ? device_sm_count() : kMaxWorkers;
     st = launch_pdl(kernel, dim3(workers), dim3(kThreads), ChunkSmem<D>::kBytes, s, mk, mv, a);
     if (st != cudaSuccess) return st;

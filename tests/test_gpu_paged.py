@@ -400,6 +400,16 @@ def test_sample_against_the_definition(bridge, dtype, vocab):
     check_rows(bridge, x, u, *cols)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 450001), (BF16, 900003), (F16, 151937)])
+def test_sample_long_rows(bridge, dtype, vocab):
+    """Rows longer than a cluster's shared memory among them."""
+
+    g = torch.Generator().manual_seed(vocab)
+    x = (3.0 * torch.randn((4, vocab), generator=g)).to(dtype).to(DEV)
+    u = torch.rand((4,), generator=g).tolist()
+    check_rows(bridge, x, u, [0.0, 0.7, 1.0, 0.9], [0, 50, 0, 7], [1.0, 0.9, 0.99, 1.0], [0.0, 0.01, 0.0, 0.1])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
 def test_sample_ties_infinities_and_nan(bridge, dtype):
     inf, nan = math.inf, math.nan
