@@ -199,15 +199,17 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
 // The logits become ordered keys (whole numbers in the order of the values,
 // 16 bits wide for the 16-bit types), read from memory once.  What remains is
 // to find the key at which the kept prefix ends: seven keys that split the
-// range still possible are tried at once - each thread counts, or sums the
-// masses of, the entries at or above each of them in registers - and the
-// cluster exchanges the sums through distributed shared memory with one
-// barrier.  The first seven lie at fixed distances below the maximum (in units
-// of the temperature), which leaves few entries; then each try takes three bits
-// off the range.  No sort, no atomics.
+// range still possible are tried at once - each thread counts the entries at or
+// above each of them, and sums their masses, in registers - and the cluster
+// exchanges the sums through distributed shared memory with one barrier.  The
+// first seven lie at fixed distances below the maximum (in units of the
+// temperature), which leaves few entries; when at most kList are left, every
+// block gets all of their keys and finishes alone, without the cluster's
+// barriers.  No sort, no atomics on memory.
 constexpr int kPivots = 7;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;  // more than 8 need the kernel's consent (launch_cluster)
 constexpr int kMaxSampleThreads = 1024;
+constexpr int kList = 1024;
 
 template <int DT>
 struct Keys {
@@ -222,6 +224,12 @@ struct Keys {
     static __device__ __forceinline__ float value(uint32_t k) {
         const uint16_t b = static_cast<uint16_t>((k & 0x8000u) ? (k & 0x7fffu) : ~k);
         return DT == kBF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+    }
+    // the largest of a word's eight
+    static __device__ __forceinline__ uint32_t largest(const Key* k) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(k);
+        const uint32_t m = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+        return max(m & 0xffffu, m >> 16);
     }
     static __device__ __forceinline__ uint32_t near(float x) {
         return key(DT == kBF16 ? f32_to_bf16_bits(x) : f32_to_f16_bits(x));
@@ -239,6 +247,7 @@ struct Keys<kF32> {
     static __device__ __forceinline__ float value(uint32_t k) {
         return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
     }
+    static __device__ __forceinline__ uint32_t largest(const Key* k) { return max(max(k[0], k[1]), max(k[2], k[3])); }
     static __device__ __forceinline__ uint32_t near(float x) { return key(__float_as_uint(x)); }
 };
 
@@ -261,48 +270,88 @@ __device__ __forceinline__ void store_remote(const int64_t* p, uint32_t rank, in
     asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 
+__device__ __forceinline__ void store_remote32(const uint32_t* p, uint32_t rank, uint32_t v) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
+constexpr int kSums = 2 * kPivots + 1;  // masses, their total, numbers
 struct SampleShared {
-    int64_t warp[32][kPivots + 1];
-    int64_t from[2][kMaxCluster][kPivots + 1];  // what each block of the cluster sent, alternating halves
-    int64_t scan[32];
+    int64_t warp[kSums][32];
+    int64_t from[2][kSums][kMaxCluster];  // what each block of the cluster sent, alternating halves
+    // the search, kept by warp 0
+    uint32_t pv[kPivots], lo, hi;
+    int64_t above, target;
+    int listed;          // entries in `list`, or -1
+    int gather, start;   // 1: the list is made next; where this block's entries go in it
+    int own_count;
+    uint32_t own[kList], list[kList];
 };
 
-// Sum (or maximum) over the block and the cluster of n values a thread; in
-// `each`, the blocks' own contributions stay readable until the call after next.
-template <int N, bool MAX>
-__device__ __forceinline__ void cluster_reduce(SampleShared& sh, int& turn, int64_t (&v)[N]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+__device__ __forceinline__ int64_t warp_sum64(int64_t x) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+// inclusive prefix over the lanes
+__device__ __forceinline__ int64_t warp_scan64(int64_t x) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const int64_t x = __shfl_xor_sync(0xffffffffu, v[i], o);
-            v[i] = MAX ? (x > v[i] ? x : v[i]) : v[i] + x;
-        }
-        if (lane == 0) sh.warp[warp][i] = v[i];
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (static_cast<int>(threadIdx.x & 31) >= o) x += y;
     }
-    __syncthreads();
+    return x;
+}
+// the warp's sum of a value in [0, 2^48), as two sums of 24-bit halves
+__device__ __forceinline__ int64_t warp_sum48(int64_t x) {
+    const uint32_t lo = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(x) & 0xffffffu);
+    const uint32_t hi = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(x >> 24));
+    return (static_cast<int64_t>(hi) << 24) + lo;
+}
+// Lane i of warp 0 gets the block's sum of sh.warp[i], i < n.
+__device__ __forceinline__ int64_t block_sums(const SampleShared& sh, int n) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    int64_t x = 0;
+    if (lane < n)
+        for (int w = 0; w < warps; ++w) x += sh.warp[lane][w];
+    return x;
+}
+// Lane i of warp 0, i < n, sends its value to every block of the cluster.
+__device__ __forceinline__ void cluster_send(SampleShared& sh, int turn, int n, int64_t x) {
+    const int lane = threadIdx.x & 31;
     const uint32_t ranks = cluster_size(), me = cluster_rank();
+    if (lane < n)
+        for (uint32_t r = 0; r < ranks; ++r) store_remote(&sh.from[turn][lane][me], r, x);
+}
+// The largest of a value per thread, over the cluster.
+__device__ __forceinline__ uint32_t cluster_max(SampleShared& sh, int& turn, uint32_t v) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (lane == 0) sh.warp[0][warp] = v;
+    __syncthreads();
     turn ^= 1;
-    if (threadIdx.x < N) {
-        int64_t s = sh.warp[0][threadIdx.x];
-        for (int w = 1; w < warps; ++w) {
-            const int64_t x = sh.warp[w][threadIdx.x];
-            s = MAX ? (x > s ? x : s) : s + x;
-        }
-        for (uint32_t r = 0; r < ranks; ++r) store_remote(&sh.from[turn][me][threadIdx.x], r, s);
+    const uint32_t ranks = cluster_size();
+    if (warp == 0) {
+        v = __reduce_max_sync(0xffffffffu, lane < warps ? static_cast<uint32_t>(sh.warp[0][lane]) : 0u);
+        if (lane < static_cast<int>(ranks)) store_remote(&sh.from[turn][0][cluster_rank()], lane, v);
     }
     cluster_barrier();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        int64_t s = sh.from[turn][0][i];
-        for (uint32_t r = 1; r < ranks; ++r) {
-            const int64_t x = sh.from[turn][r][i];
-            s = MAX ? (x > s ? x : s) : s + x;
-        }
-        v[i] = s;
-    }
+    return __reduce_max_sync(0xffffffffu, lane < static_cast<int>(ranks) ? static_cast<uint32_t>(sh.from[turn][0][lane]) : 0u);
 }
+
+// rint(2^38 w) of a w in [0, 1] as 2^19 hi + lo: adding 2^23 (1.5 2^23) leaves a
+// number below 2^22 rounded to a whole one in the low mantissa bits, and both
+// differences and scalings are exact, so this is the one rounding of 2^38 w.
+// Two 32-bit sums cost what a 64-bit one does, and no conversion instruction.
+__device__ __forceinline__ void split_mass(float w, int& hi, int& lo) {
+    const float x = __fmul_rn(w, 524288.F);
+    const float y = __fadd_rn(x, 8388608.F);
+    hi = __float_as_int(y) - 0x4B000000;
+    const float r = __fsub_rn(x, __fsub_rn(y, 8388608.F));
+    lo = __float_as_int(__fmaf_rn(r, 524288.F, 12582912.F)) - 0x4B400000;
+}
+__device__ __forceinline__ int64_t join_mass(int hi, int lo) { return (static_cast<int64_t>(hi) << 19) + lo; }
 
 template <int DT>
 __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const SampleArgs a) {
@@ -327,26 +376,34 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
     const int mine = static_cast<int>(static_cast<int64_t>(words) * (rank + 1) / ranks) - word0;
     const int first = word0 * VE - shift;
     uint32_t best = 0;
-    for (int w = tid; w < mine; w += threads) {
-        const int i = first + w * VE;
-        typename K::Raw raw[VE];
-        Key out[VE];
-        const bool all = i >= 0 && i + VE <= n;
-        if (all) *reinterpret_cast<uint4*>(raw) = __ldcs(reinterpret_cast<const uint4*>(src + i));
+    constexpr int kAhead = 4;  // words in flight a thread
+    for (int w0 = tid; w0 < mine; w0 += kAhead * threads) {
+        uint4 in[kAhead];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            uint32_t k = 0;  // below every entry's key: slots outside the row
-            if (all) k = K::key(raw[e]);
-            else if (i + e >= 0 && i + e < n) k = K::key(src[i + e]);
-            best = max(best, k);
-            out[e] = static_cast<Key>(k);
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = first + (w0 + u * threads) * VE;
+            if (w0 + u * threads < mine && i >= 0 && i + VE <= n) in[u] = __ldcs(reinterpret_cast<const uint4*>(src + i));
         }
-        *reinterpret_cast<uint4*>(keys + w * VE) = *reinterpret_cast<const uint4*>(out);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int w = w0 + u * threads, i = first + w * VE;
+            if (w >= mine) break;
+            const auto* raw = reinterpret_cast<const typename K::Raw*>(&in[u]);
+            Key out[VE];
+            const bool all = i >= 0 && i + VE <= n;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                uint32_t k = 0;  // below every entry's key: slots outside the row
+                if (all) k = K::key(raw[e]);
+                else if (i + e >= 0 && i + e < n) k = K::key(src[i + e]);
+                best = max(best, k);
+                out[e] = static_cast<Key>(k);
+            }
+            *reinterpret_cast<uint4*>(keys + w * VE) = *reinterpret_cast<const uint4*>(out);
+        }
     }
     asm volatile("barrier.cluster.wait;" ::: "memory");
-    int64_t red[1] = {static_cast<int64_t>(best)};
-    cluster_reduce<1, true>(sh, turn, red);  // its barriers also publish `keys` to the block
-    const uint32_t top = static_cast<uint32_t>(red[0]);
+    const uint32_t top = cluster_max(sh, turn, best);  // its barriers also publish `keys` to the block
     const float m = K::value(top);
     const bool lead = rank == 0 && tid == 0;
     if (m == -INFINITY) {
@@ -358,15 +415,18 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
         return;
     }
     const float t = a.temperature != nullptr ? a.temperature[row] : 1.F;
-    const int slots = mine * VE;
     if (!(t > 0.F)) {
-        int at = 0x7fffffff;
-        for (int s = tid; s < slots; s += threads)
-            if (keys[s] == top) at = min(at, first + s);
-        red[0] = -static_cast<int64_t>(at);
-        cluster_reduce<1, true>(sh, turn, red);
+        uint32_t after = 0;  // entries from the earliest maximum on
+        for (int w = tid; w < mine && after == 0; w += threads) {
+            Key k[VE];
+            *reinterpret_cast<uint4*>(k) = *reinterpret_cast<const uint4*>(keys + w * VE);
+#pragma unroll
+            for (int e = VE - 1; e >= 0; --e)
+                if (k[e] == top) after = static_cast<uint32_t>(n - (first + w * VE + e));
+        }
+        after = cluster_max(sh, turn, after);
         if (lead) {
-            a.tokens[row] = static_cast<int32_t>(-red[0]);
+            a.tokens[row] = n - static_cast<int32_t>(after);
             if (a.logprobs != nullptr) a.logprobs[row] = 0.F;
         }
         cluster_barrier();
@@ -374,67 +434,167 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
     }
     const float inv = 1.F / t;
     auto weight = [&](uint32_t k) { return k == top ? 1.F : expf((K::value(k) - m) * inv); };
-    auto mass = [&](uint32_t k) { return __float2ll_rn(weight(k) * kMassOne); };
-    // f(key) for every entry at or above `floor_key`, in any order
-    auto sweep = [&](uint32_t floor_key, auto f) {
+    auto mass = [&](uint32_t k) {
+        int hi, lo;
+        split_mass(weight(k), hi, lo);
+        return join_mass(hi, lo);
+    };
+    // f(key) for every entry with key >= from, in any order, and for some below; a
+    // word whose entries all lie below is skipped as a whole, the rest goes
+    // without branches (per-entry ones cost more than they save)
+    auto sweep = [&](uint32_t from, auto f) {
         for (int w = tid; w < mine; w += threads) {
             Key k[VE];
             *reinterpret_cast<uint4*>(k) = *reinterpret_cast<const uint4*>(keys + w * VE);
+            if (K::largest(k) < from) continue;
 #pragma unroll
-            for (int e = 0; e < VE; ++e)
-                if (k[e] >= floor_key) f(static_cast<uint32_t>(k[e]));
+            for (int e = 0; e < VE; ++e) f(static_cast<uint32_t>(k[e]));
         }
     };
-    // The largest key whose entries at or above it reach `target` (in number, or
-    // in mass): lo reaches it, hi does not.  above: what lies above lo.
-    auto locate = [&](auto by_mass, int64_t target, uint32_t& lo, int64_t& above) {
-        uint32_t hi = top + 1;  // nothing lies at or above it
-        above = 0;
-        bool started = false;
-        while (hi - lo > 1) {
-            uint32_t pv[kPivots];
-            if (!started) {
-                const float d[kPivots] = {0.7F, 1.6F, 2.8F, 4.2F, 6.F, 8.5F, 12.F};
+    // The largest key whose entries at or above it reach a target (in number, or
+    // in mass): lo reaches it, hi does not.  above: what lies above lo.  The
+    // target may depend on the sum over the entries above the first lo, which
+    // the first try brings along.  The sums of a try meet in warp 0 (lane i: sum
+    // i), which alone decides; the other warps read its decision.
+    auto locate = [&](auto by_mass, auto target_of, uint32_t& lo, int64_t& above, int64_t& target) {
+        constexpr int N = by_mass ? kSums : kPivots, kCounts = by_mass ? kPivots + 1 : 0;
+        if (warp == 0) {
+            const float d[kPivots] = {0.7F, 1.6F, 2.8F, 4.2F, 6.F, 8.5F, 12.F};
+            float mine_d = d[0];
 #pragma unroll
-                for (int i = 0; i < kPivots; ++i) pv[i] = min(max(K::near(m - d[i] * t), lo + 1), hi - 1);
-                started = true;
-            } else {
-                const uint64_t span = hi - lo;
-#pragma unroll
-                for (int i = 0; i < kPivots; ++i)
-                    pv[i] = min(max(hi - static_cast<uint32_t>(span * (i + 1) / (kPivots + 1)), lo + 1), hi - 1);
+            for (int i = 1; i < kPivots; ++i)
+                if (lane == i) mine_d = d[i];
+            // (with lo == top no key lies between: every pivot is top + 1, where nothing is)
+            if (lane < kPivots) sh.pv[lane] = max(min(K::near(m - mine_d * t), top), lo + 1);
+            if (lane == 0) {
+                sh.lo = lo;
+                sh.hi = top + 1;  // nothing lies at or above it
+                sh.above = 0;
+                sh.listed = -1;
+                sh.gather = 0;
             }
-            // pv falls; entries at or above hi count for every one of them and are known
-            int64_t v[kPivots];
+        }
+        __syncthreads();
+        for (int tries = 0;; ++tries) {
+            const uint32_t hi = sh.hi;
+            const int listed = sh.listed;
+            uint32_t pv[kPivots];  // falling
 #pragma unroll
-            for (int i = 0; i < kPivots; ++i) v[i] = 0;
-            sweep(pv[kPivots - 1], [&](uint32_t k) {
-                if (k >= hi) return;
-                const int64_t x = by_mass ? mass(k) : 1;
+            for (int i = 0; i < kPivots; ++i) pv[i] = sh.pv[i];
+            // sums over the entries below hi: at or above each pivot, and above the first lo
+            int vh[kPivots + 1], vl[kPivots + 1], vc[kPivots];
 #pragma unroll
-                for (int i = 0; i < kPivots; ++i)
-                    if (k >= pv[i]) v[i] += x;
-            });
-            cluster_reduce<kPivots, false>(sh, turn, v);
-            // the first pivot that reaches the target is the new lo, the one before it the new hi
-            uint32_t nlo = lo, nhi = hi;
-            int64_t at_hi = above;
-            bool found = false;
+            for (int i = 0; i <= kPivots; ++i) vh[i] = vl[i] = 0;
 #pragma unroll
-            for (int i = 0; i < kPivots; ++i) {
-                if (found) continue;
-                if (above + v[i] >= target) {
-                    nlo = pv[i];
-                    found = true;
+            for (int i = 0; i < kPivots; ++i) vc[i] = 0;
+            const uint32_t from = by_mass && tries == 0 ? lo + 1 : pv[kPivots - 1];
+            auto take = [&](uint32_t k) {
+                k = k < hi ? k : 0;  // (every pivot is above 0)
+                if constexpr (by_mass) {
+                    int h, l;
+                    split_mass(k >= from ? weight(k) : 0.F, h, l);
+                    vh[kPivots] += h;
+                    vl[kPivots] += l;
+#pragma unroll
+                    for (int i = 0; i < kPivots; ++i)
+                        if (k >= pv[i]) {
+                            vh[i] += h;
+                            vl[i] += l;
+                            vc[i] += 1;
+                        }
                 } else {
-                    nhi = pv[i];
-                    at_hi = above + v[i];
+#pragma unroll
+                    for (int i = 0; i < kPivots; ++i) vc[i] += k >= pv[i];
+                }
+            };
+            if (listed >= 0) {
+                for (int i = tid; i < listed; i += threads) take(sh.list[i]);
+            } else {
+                sweep(from, take);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                int64_t x;
+                if constexpr (by_mass)
+                    x = i <= kPivots ? warp_sum48(join_mass(vh[i], vl[i]))
+                                     : __reduce_add_sync(0xffffffffu, static_cast<unsigned>(vc[i > kPivots ? i - kPivots - 1 : 0]));
+                else x = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(vc[i]));
+                if (lane == 0) sh.warp[i][warp] = x;
+            }
+            __syncthreads();
+            int64_t x = 0;
+            if (warp == 0) x = block_sums(sh, N);
+            if (listed < 0) {
+                turn ^= 1;
+                if (warp == 0) cluster_send(sh, turn, N, x);
+                cluster_barrier();
+                if (warp == 0) {
+                    x = 0;
+                    if (lane < N)
+                        for (uint32_t r = 0; r < ranks; ++r) x += sh.from[turn][lane][r];
                 }
             }
-            above = at_hi;
-            lo = nlo;
-            hi = nhi;
+            if (warp == 0) {
+                if (tries == 0) {
+                    const int64_t t0 = target_of(__shfl_sync(0xffffffffu, x, kPivots));
+                    if (lane == 0) sh.target = t0;
+                    __syncwarp();
+                }
+                const uint32_t my_pv = sh.pv[lane < kPivots ? lane : 0];
+                const unsigned reach =
+                    __ballot_sync(0xffffffffu, lane < kPivots && sh.above + x >= sh.target);
+                // the first pivot that reaches the target is the new lo, the one before it the new hi
+                const int at = reach != 0 ? __ffs(reach) - 1 : kPivots;
+                const int i_lo = min(at, kPivots - 1), i_hi = max(at - 1, 0);
+                const uint32_t nlo = __shfl_sync(0xffffffffu, my_pv, i_lo), nhi = __shfl_sync(0xffffffffu, my_pv, i_hi);
+                const int64_t sum_hi = __shfl_sync(0xffffffffu, x, i_hi);
+                const int64_t number_lo = __shfl_sync(0xffffffffu, x, kCounts + i_lo);
+                const int64_t number_hi = __shfl_sync(0xffffffffu, x, kCounts + i_hi);
+                const uint32_t new_lo = at < kPivots ? nlo : sh.lo, new_hi = at > 0 ? nhi : hi;
+                const int64_t number = number_lo - (at > 0 ? number_hi : 0);
+                const bool gather = listed < 0 && new_hi - new_lo > 1 && at < kPivots && number <= kList;
+                int64_t before = 0;  // entries of the blocks before this one
+                if (gather && lane < static_cast<int>(rank))
+                    before = sh.from[turn][kCounts + at][lane] - (at > 0 ? sh.from[turn][kCounts + at - 1][lane] : 0);
+                before = warp_sum64(before);
+                __syncwarp();
+                const uint64_t span = new_hi - new_lo;
+                if (lane < kPivots)
+                    sh.pv[lane] = max(min(new_hi - static_cast<uint32_t>(span * (lane + 1) / (kPivots + 1)), new_hi - 1),
+                                      new_lo + 1);
+                if (lane == 0) {
+                    sh.lo = new_lo;
+                    sh.hi = new_hi;
+                    if (at > 0) sh.above += sum_hi;
+                    sh.gather = gather ? 1 : 0;
+                    sh.start = static_cast<int>(before);
+                    sh.own_count = 0;
+                    if (gather) sh.listed = static_cast<int>(number);
+                }
+            }
+            __syncthreads();
+            if (sh.gather) {
+                // the keys in [lo, hi) of every block to every block
+                const uint32_t g_lo = sh.lo, g_hi = sh.hi;
+                sweep(g_lo, [&](uint32_t k) {
+                    if (k >= g_lo && k < g_hi) sh.own[atomicAdd(&sh.own_count, 1)] = k;
+                });
+                __syncthreads();
+                const int own = sh.own_count, start = sh.start;
+                for (int i = tid; i < own * static_cast<int>(ranks); i += threads) {
+                    const int r = i / own, j = i - r * own;
+                    store_remote32(&sh.list[start + j], r, sh.own[j]);
+                }
+                cluster_barrier();
+            }
+            if (sh.hi - sh.lo <= 1) break;
         }
+        lo = sh.lo;
+        above = sh.above;
+        target = sh.target;
+        const bool listed = sh.listed >= 0;
+        __syncthreads();
+        if (listed) cluster_barrier();  // the list may be written again
     };
     // kept: key > cut, and the first `ties` (by index) of the entries with key == cut
     uint32_t cut = 0;  // below every entry: all are kept
@@ -445,93 +605,118 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
     constexpr std::integral_constant<bool, false> by_number{};
     constexpr std::integral_constant<bool, true> by_mass{};
     if (k_ > 0 && k_ < n) {
-        int64_t above;
-        locate(by_number, k_, cut, above);
+        int64_t above, target;
+        locate(by_number, [&](int64_t) { return static_cast<int64_t>(k_); }, cut, above, target);
         ties = k_ - above;
         some_ties = true;
     }
     if (p < 1.F) {
-        int64_t sum[1] = {0};
-        sweep(cut + 1, [&](uint32_t k) { sum[0] += mass(k); });
-        cluster_reduce<1, false>(sh, turn, sum);
-        const int64_t whole = sum[0] + (some_ties ? ties * mass(cut) : 0);
-        int64_t reach = __double2ll_ru(__dmul_rn(static_cast<double>(p), __ll2double_rn(whole)));
-        reach = reach < 1 ? 1 : reach;
+        // (with the range empty, lo == cut == top, the one try only brings the sum: nothing lies above)
         uint32_t lo = cut;
-        int64_t above;
-        locate(by_mass, reach, lo, above);
+        int64_t above, reach;
+        locate(by_mass, [&](int64_t over) {
+            const int64_t whole = over + (some_ties ? ties * mass(cut) : 0);
+            const int64_t r = __double2ll_ru(__dmul_rn(static_cast<double>(p), __ll2double_rn(whole)));
+            return r < 1 ? 1 : r;
+        }, lo, above, reach);
         const int64_t each = lo > 0 ? mass(lo) : 0;
         const int64_t need = each > 0 ? (reach - above + each - 1) / each : 0;
         if (each > 0 && (lo > cut || need < ties)) ties = need;
         some_ties = some_ties || lo > 0;
         cut = lo;
     }
-    // Index order from here: a thread's entries are a run of slots, the block's follow one another
-    const int per = ((slots + threads - 1) / threads) | 1;
-    const int s0 = min(slots, tid * per), s1 = min(slots, s0 + per);
-    // inclusive prefix of v over the block; total: the block's sum
-    auto block_scan = [&](int64_t v, int64_t& total) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += x;
-        }
-        __syncthreads();
-        if (lane == 31) sh.scan[warp] = v;
-        __syncthreads();
-        total = 0;
-        int64_t before = 0;
-        for (int w = 0; w < (threads >> 5); ++w) {
-            if (w < warp) before += sh.scan[w];
-            total += sh.scan[w];
-        }
-        return v + before;
-    };
-    int64_t quota = 0;  // how many of this run's entries at `cut` are kept
-    if (some_ties) {
-        int64_t c = 0;
-        for (int s = s0; s < s1; ++s) c += keys[s] == cut;
-        int64_t block_total;
-        const int64_t upto = block_scan(c, block_total);
-        int64_t v[1] = {tid == 0 ? block_total : 0};
-        cluster_reduce<1, false>(sh, turn, v);
-        int64_t before = upto - c;
-        for (uint32_t r = 0; r < rank; ++r) before += sh.from[turn][r][0];
-        quota = min(max(ties - before, static_cast<int64_t>(0)), c);
-    }
     float low = a.min_p != nullptr ? a.min_p[row] : 0.F;
     low = low > 1.F ? 1.F : low;
-    int64_t sum = 0;
-    {
-        int64_t left = quota;
-        for (int s = s0; s < s1; ++s) {
-            const uint32_t k = keys[s];
-            const bool in = k > cut || (k == cut && left-- > 0);
-            if (in && !(weight(k) < low)) sum += mass(k);
+    // Index order from here.  A warp's entries are a run of words; it sums what it
+    // keeps above `cut` and counts its entries at `cut`.
+    const int run = (mine + (threads >> 5) - 1) / (threads >> 5);
+    const int w0 = min(mine, warp * run), w1 = min(mine, w0 + run);
+    int sum_h = 0, sum_l = 0, at_cut = 0;
+    for (int w = w0 + lane; w < w1; w += 32) {
+        Key k[VE];
+        *reinterpret_cast<uint4*>(k) = *reinterpret_cast<const uint4*>(keys + w * VE);
+        if (K::largest(k) < cut) continue;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const float x = weight(k[e]);
+            int h, l;
+            split_mass(k[e] > cut && !(x < low) ? x : 0.F, h, l);
+            sum_h += h;
+            sum_l += l;
+            at_cut += k[e] == cut;
         }
     }
-    int64_t block_total;
-    const int64_t upto = block_scan(sum, block_total);
-    int64_t v[1] = {tid == 0 ? block_total : 0};
-    cluster_reduce<1, false>(sh, turn, v);
-    const int64_t whole = v[0];
-    int64_t before = 0;
-    for (uint32_t r = 0; r < rank; ++r) before += sh.from[turn][r][0];
-    int64_t aim = __double2ll_rd(__dmul_rn(static_cast<double>(a.uniform[row]), __ll2double_rn(whole)));
-    aim = (aim < 0 ? 0 : aim >= whole ? whole - 1 : aim) - before;
-    if (upto - sum <= aim && aim < upto) {
-        int64_t c = upto - sum, left = quota;
-        for (int s = s0; s < s1; ++s) {
-            const uint32_t k = keys[s];
-            const bool in = k > cut || (k == cut && left-- > 0);
-            if (!in || weight(k) < low) continue;
-            const int64_t w = mass(k);
-            c += w;
-            if (c > aim) {
-                a.tokens[row] = first + s;
-                if (a.logprobs != nullptr)
-                    a.logprobs[row] = static_cast<float>(log(__ll2double_rn(w) / __ll2double_rn(whole)));
-                break;
+    if (!some_ties) at_cut = 0;
+    const int64_t warp_mass = warp_sum48(join_mass(sum_h, sum_l));
+    const int64_t warp_ties = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(at_cut));
+    if (lane == 0) {
+        sh.warp[0][warp] = warp_mass;
+        sh.warp[1][warp] = warp_ties;
+    }
+    __syncthreads();
+    turn ^= 1;
+    if (warp == 0) cluster_send(sh, turn, 2, block_sums(sh, 2));
+    cluster_barrier();
+    if (warp == 0) {
+        // the blocks' shares (lane = block), then this block's warps' (lane = warp)
+        const int64_t each = some_ties && !(weight(cut) < low) ? mass(cut) : 0;
+        const bool real = lane < static_cast<int>(ranks);
+        const int64_t block_ties = real ? sh.from[turn][1][lane] : 0;
+        const int64_t block_ties_before = warp_scan64(block_ties) - block_ties;
+        const int64_t block_quota = min(max(ties - block_ties_before, static_cast<int64_t>(0)), block_ties);
+        const int64_t block_mass = (real ? sh.from[turn][0][lane] : 0) + block_quota * each;
+        const int64_t block_upto = warp_scan64(block_mass);
+        const int64_t whole = __shfl_sync(0xffffffffu, block_upto, 31);
+        const int64_t before = __shfl_sync(0xffffffffu, block_upto - block_mass, rank);
+        const int64_t ties_before = __shfl_sync(0xffffffffu, block_ties_before, rank);
+        int64_t aim = __double2ll_rd(__dmul_rn(static_cast<double>(a.uniform[row]), __ll2double_rn(whole)));
+        aim = (aim < 0 ? 0 : aim >= whole ? whole - 1 : aim) - before;
+        if (aim >= 0 && aim < __shfl_sync(0xffffffffu, block_mass, rank)) {
+            const bool real_warp = lane < (threads >> 5);
+            const int64_t ties_of = real_warp ? sh.warp[1][lane] : 0;
+            const int64_t ties_at_warp = ties_before + warp_scan64(ties_of) - ties_of;
+            const int64_t quota_of = min(max(ties - ties_at_warp, static_cast<int64_t>(0)), ties_of);
+            const int64_t all_of = (real_warp ? sh.warp[0][lane] : 0) + quota_of * each;
+            const int64_t upto_of = warp_scan64(all_of);
+            const int hit = __ffs(__ballot_sync(0xffffffffu, upto_of > aim)) - 1;
+            // that warp's run holds the token: 32 words at a time, a lane's entries in order
+            int64_t at = __shfl_sync(0xffffffffu, upto_of - all_of, hit), left = __shfl_sync(0xffffffffu, quota_of, hit);
+            const int h0 = min(mine, hit * run), h1 = min(mine, h0 + run);
+            for (int w = h0; w < h1; w += 32) {
+                Key k[VE];
+                *reinterpret_cast<uint4*>(k) =
+                    w + lane < h1 ? *reinterpret_cast<const uint4*>(keys + (w + lane) * VE) : make_uint4(0, 0, 0, 0);
+                int64_t x[VE], sum = 0;
+                int c = 0;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) c += some_ties && k[e] == cut;
+                const int64_t ties_at = warp_scan64(c);
+                int64_t mine_left = left - (ties_at - c);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    const bool in = k[e] > cut || (some_ties && k[e] == cut && mine_left-- > 0);
+                    x[e] = in && !(weight(k[e]) < low) ? mass(k[e]) : 0;
+                    sum += x[e];
+                }
+                const int64_t upto = warp_scan64(sum);
+                if (at + upto - sum <= aim && aim < at + upto) {
+                    int64_t c2 = at + upto - sum, drawn = 0;
+                    int place = -1;
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        c2 += x[e];
+                        if (place < 0 && c2 > aim) {
+                            place = e;
+                            drawn = x[e];
+                        }
+                    }
+                    a.tokens[row] = first + (w + lane) * VE + place;
+                    if (a.logprobs != nullptr)
+                        a.logprobs[row] = static_cast<float>(log(__ll2double_rn(drawn) / __ll2double_rn(whole)));
+                }
+                at += __shfl_sync(0xffffffffu, upto, 31);
+                left -= __shfl_sync(0xffffffffu, ties_at, 31);
+                if (at > aim) break;
             }
         }
     }
@@ -540,21 +725,23 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
 
 constexpr int kSampleSmem = 200 * 1024;  // the largest slice of a row
 
-// One row to `cluster` blocks of `threads`.  The slice should leave room for
-// two blocks an SM (their barriers overlap), and all rows together should fill
-// the SMs' threads once.
+// One row to `cluster` blocks of `threads`: the kernel's 64 registers leave 1024
+// threads an SM, which the blocks that are resident together share.
 template <int DT>
 cudaError_t launch_cluster(const SampleArgs& a, int cluster, cudaStream_t s) {
     using K = Keys<DT>;
     auto kernel = sample_cluster_kernel<DT>;
     const int words = (a.vocab + 2 * K::kVec - 2) / K::kVec;
     const int slice = (words + cluster - 1) / cluster * 16;
-    const int fit = static_cast<int>(220 * 1024 / (slice + 8 * 1024));
-    int threads = fit >= 8 ? 256 : fit >= 4 ? 512 : 1024;
-    if (static_cast<int64_t>(a.rows) * cluster <= 2 * device_sm_count()) threads = 1024;
-    while (threads > 128 && threads > 2 * (slice / 16)) threads >>= 1;
+    const int fit = 228 * 1024 / (slice + static_cast<int>(sizeof(SampleShared)) + 1024);
+    const int64_t blocks = static_cast<int64_t>(a.rows) * cluster;
+    const int64_t per_sm = (blocks + device_sm_count() - 1) / device_sm_count();
+    int threads = 512;
+    while (threads > 128 && (threads * (per_sm < fit ? per_sm : fit) > 1024 || threads > 2 * (slice / 16))) threads >>= 1;
     static std::atomic<uint64_t> opted{0};
-    const cudaError_t st = opt_in_smem(reinterpret_cast<const void*>(kernel), kSampleSmem, opted);
+    cudaError_t st = opt_in_smem(reinterpret_cast<const void*>(kernel), kSampleSmem, opted);
+    if (st == cudaSuccess && cluster > 8)
+        st = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (st != cudaSuccess) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.rows * cluster));
@@ -577,10 +764,10 @@ cudaError_t launch_cluster(const SampleArgs& a, int cluster, cudaStream_t s) {
 cudaError_t sample_rows(const SampleArgs& a, int dt, cudaStream_t s) {
     if (a.rows == 0) return cudaSuccess;
     const int64_t bytes = static_cast<int64_t>(a.vocab) * (dt == kF32 ? 4 : 2) + 16;
-    int cluster = kMaxCluster;
-    // fewer blocks a row once the rows fill the SMs by themselves, but no slice over 100 KB
+    int cluster = static_cast<int64_t>(a.rows) * kMaxCluster <= device_sm_count() ? kMaxCluster : 8;
+    // fewer blocks a row once the rows fill the SMs by themselves, but no slice over 56 KB (three blocks an SM)
     while (cluster > 1 && static_cast<int64_t>(a.rows) * cluster > 4 * device_sm_count() &&
-           bytes / (cluster / 2) <= 100 * 1024)
+           bytes / (cluster / 2) <= 56 * 1024)
         cluster >>= 1;
     // and none so small that its barrier costs more than its share of the row
     while (cluster > 1 && bytes / cluster < 4096) cluster >>= 1;
