@@ -23,6 +23,7 @@
 #include "kc_launch.h"
 #include "kc_tcgen05.cuh"
 #include "kc_tma.h"
+#include "paged_combine.cuh"
 #include "paged_plan.cuh"
 
 namespace kc {
@@ -31,8 +32,6 @@ namespace {
 constexpr int kRows = 256;   // query rows of an item
 constexpr int kKeys = 128;   // keys of a block
 constexpr int kThreads = 384;
-constexpr float kLn2 = 0.6931471805599453F;
-constexpr float kLog2E = 1.4426950408889634F;
 constexpr float kLazy = 8.F;  // how far the true maximum may exceed m
 
 template <int D>
@@ -69,19 +68,6 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t r;
-    if constexpr (DT == kBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 
 // the item's last block has rows without a key
 __device__ __forceinline__ bool has_tail(int limit) { return limit % kKeys != 0 || limit == 0; }
@@ -136,8 +122,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     pdl_wait_on_producer();
     const int group = p.q_heads / p.kv_heads;
-    const int worker = blockIdx.x, workers = gridDim.x;
-    const int64_t total = paged_places<kRows, kKeys, kThreads>(p, group, worker, 1, workers, sums, &place_seq, &place_at);
+    const int worker = blockIdx.x;
+    int workers = gridDim.x;
+    const int64_t total =
+        paged_places<kRows, kKeys, kThreads>(p, group, worker, 1, 1, workers, sums, &place_seq, &place_at);
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = tmem_slot;
@@ -391,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (live && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
             } else {
-                float* part = Part::slot(a.workspace, workers, worker, w.t0 > 0 ? 0 : 1);
+                float* part = Part::slot(a.workspace, gridDim.x, worker, w.t0 > 0 ? 0 : 1);
                 *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, l);
                 float4* acc = reinterpret_cast<float4*>(part + 2 * kRows);
 #pragma unroll 1
@@ -436,64 +424,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 }  // namespace
-
-// ---------------------------------------------------------------------------
-// The join of cut items: with M the largest of the pieces' maxima,
-// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the pieces
-// (the same bits on every run).  One block per worker that began a cut item
-// and 32 of the item's rows: lane = row, warp = a share of the dims.
-template <int DT, int D, int ROWS>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedAttentionArgs a, int workers) {
-    using Part = PagedPartial<ROWS, D>;
-    pdl_launch_dependents();
-    pdl_wait_on_producer();
-    const int owner = blockIdx.x;
-    const PagedCut* cuts = Part::cuts(a.workspace);
-    const PagedCut cut = cuts[owner];
-    constexpr int kLanes = ROWS < 32 ? ROWS : 32, kShares = 256 / kLanes;
-    const int lane = threadIdx.x % kLanes, share = threadIdx.x / kLanes;
-    const int r = blockIdx.y * kLanes + lane;
-    if (!cut.valid || r >= cut.rows) return;
-    constexpr int kVecs = (D / 4 + kShares - 1) / kShares;  // float4 of a thread
-    float m = -INFINITY, l = 0.F;
-    float4 acc[kVecs];
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) acc[i] = make_float4(0.F, 0.F, 0.F, 0.F);
-    for (int c = owner; c <= cut.last && c < workers; ++c) {
-        if (c > owner && !cuts[c].tail) continue;
-        const float* part = Part::slot(a.workspace, workers, c, c == owner ? 1 : 0);
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part) + r);
-        const float mn = fmaxf(m, ml.x);
-        const float f = m == -INFINITY ? 0.F : exp2f(m - mn), g = ml.x == -INFINITY ? 0.F : exp2f(ml.x - mn);
-        l = l * f + ml.y * g;
-        const float4* o = reinterpret_cast<const float4*>(part + 2 * ROWS);
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int v = share + i * kShares;
-            if (v >= D / 4) break;
-            const float4 x = __ldcg(o + v * ROWS + r);
-            acc[i].x = acc[i].x * f + x.x * g;
-            acc[i].y = acc[i].y * f + x.y * g;
-            acc[i].z = acc[i].z * f + x.z * g;
-            acc[i].w = acc[i].w * f + x.w * g;
-        }
-        m = mn;
-    }
-    const PagedBatch& p = a.p;
-    const int group = p.q_heads / p.kv_heads;
-    const int64_t row = cut.row0 + (cut.r0 + r) / group;
-    const int head = cut.kvh * group + (cut.r0 + r) % group;
-    const float inv = l > 0.F ? 1.F / l : 0.F;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const int v = share + i * kShares;
-        if (v >= D / 4) break;
-        *reinterpret_cast<uint2*>(out + 4 * v) = make_uint2(pack2<DT>(acc[i].x * inv, acc[i].y * inv),
-                                                            pack2<DT>(acc[i].z * inv, acc[i].w * inv));
-    }
-    if (share == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
-}
 
 namespace {
 constexpr int kMaxWorkers = 148;

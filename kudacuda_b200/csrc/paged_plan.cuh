@@ -34,7 +34,13 @@ struct PagedCut {
 };
 
 __device__ __forceinline__ int64_t paged_bound(int64_t total, int worker, int workers) {
-    return total * worker / workers;
+    return worker >= workers ? total : total * worker / workers;
+}
+// No more workers than blocks of keys: every worker that has work has a block
+// or two, and an item has no more pieces than blocks.
+__device__ __forceinline__ int paged_workers(int64_t total, int group, int block, int workers) {
+    return static_cast<int>(min(max(total / (static_cast<int64_t>(group) * block), static_cast<int64_t>(1)),
+                                static_cast<int64_t>(workers)));
 }
 
 struct PagedSeq {
@@ -141,12 +147,13 @@ struct PagedWalk {
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
 
-// Block-wide: the total cost, and for `count` workers first .. first + count - 1
-// of `workers` the sequence in which each one's stretch begins (seq) and that
-// sequence's place (at).  `sums` has one word per warp.  Ends with a barrier.
+// Block-wide: the total cost, the number of workers that share it (at most
+// `workers`), and for the `count` workers first + i * step the sequence in which
+// each one's stretch begins (seq) and that sequence's place (at).  `sums` has
+// one word per warp.  Ends with a barrier.
 template <int ROWS, int KT, int THREADS>
-__device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, int first, int count, int workers,
-                                                int64_t* sums, int* seq, int64_t* at) {
+__device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, int first, int step, int count,
+                                                int& workers, int64_t* sums, int* seq, int64_t* at) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b0 = static_cast<int>(static_cast<int64_t>(p.batch) * tid / THREADS);
     const int b1 = static_cast<int>(static_cast<int64_t>(p.batch) * (tid + 1) / THREADS);
@@ -174,8 +181,10 @@ __device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, 
         total += sums[i];
     }
     int64_t from = before + upto - mine;
+    workers = paged_workers(total, group, KT, workers);
     for (int i = 0; i < count; ++i) {
-        const int64_t x = paged_bound(total, first + i, workers);
+        if (first + i * step >= workers) break;
+        const int64_t x = paged_bound(total, first + i * step, workers);
         if (mine == 0 || x < from || x >= from + mine) continue;
         int64_t c = from;
         for (w.b = b0; w.b < b1; ++w.b) {

@@ -32,10 +32,6 @@ from . import native as _native
 DEFAULT_MANIFEST = Path(__file__).resolve().parent / "manifests" / "b200-sm100.json"
 
 
-# the C ABI's type codes (DType in csrc/kc_launch.h)
-_DTYPE_CODES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-
-
 class NativeCudaError(RuntimeError):
     """The native library rejected a request or a launch failed."""
 
@@ -1443,44 +1439,49 @@ class KudaCudaBridge:
                    int(kv_heads), int(head_dim), sc, 1 if shared_cache else 0, _normalize_cuda_handle(stream_ptr))
 
     # ---------------------------------------------------------------- paged KV cache and sampling
-    @staticmethod
-    def _dtype_code(tensor: Any, label: str, allowed: tuple = (1, 2)) -> int:
-        """The C ABI's code of a tensor's type: 0 float32, 1 float16, 2 bfloat16."""
+    # These run once per layer of a step, so their checks stay on plain attribute
+    # reads (a dtype is one object, so `is` compares it) and one native call.
+    def _torch_types(self) -> tuple:
+        """(codes of the C ABI by dtype, int32, float32), looked up once."""
 
-        code = _DTYPE_CODES.get(str(tensor.dtype), -1)
-        if code not in allowed:
-            raise ValueError(f"{label} has an unsupported dtype {tensor.dtype}")
-        return code
+        types = self.__dict__.get("_types")
+        if types is None:
+            import torch
 
-    def _int32_array(self, tensor: Any, count: int, label: str) -> int:
-        """Pointer of a contiguous int32 vector of at least ``count`` elements."""
+            codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # DType in csrc/kc_launch.h
+            types = self._types = (codes, torch.int32, torch.float32)
+        return types
 
-        if str(tensor.dtype) != "torch.int32" or tensor.dim() != 1 or tensor.shape[0] < count or (
-                count > 1 and tensor.stride(0) != 1):
-            raise ValueError(f"{label} must be a contiguous int32 vector of {count} elements")
-        return self._tensor_pointer(tensor, label)
+    def _paged_batch(self, rows_dtype: Any, k_pages: Any, v_pages: Any, query_start: Any, kv_len: Any,
+                     block_table: Any) -> tuple[int, Any, tuple]:
+        """Checks what the paged entries share: the dtype's code, the pages' shape, and the
+        arguments from query_start to batch."""
 
-    def _paged_batch(self, k_pages: Any, v_pages: Any, query_start: Any, kv_len: Any, block_table: Any,
-                     code: int) -> tuple[list, tuple[int, int, int, int, int]]:
-        """Checks what the paged entries share; the arguments from query_start to batch, and
-        (batch, num_pages, kv_heads, page_size, head_dim)."""
-
-        shape = tuple(k_pages.shape)
-        if len(shape) != 4 or tuple(v_pages.shape) != shape:
+        codes, int32, _ = self._torch_types()
+        code = codes.get(rows_dtype, 0)
+        if code == 0:
+            raise ValueError(f"unsupported dtype {rows_dtype}: float16 or bfloat16")
+        shape = k_pages.shape
+        if len(shape) != 4 or v_pages.shape != shape:
             raise ValueError("k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
-        if self._dtype_code(k_pages, "k_pages") != code or self._dtype_code(v_pages, "v_pages") != code:
+        if k_pages.dtype is not rows_dtype or v_pages.dtype is not rows_dtype:
             raise ValueError("the rows and the pages must have one dtype")
         if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
             raise ValueError("k_pages and v_pages must be contiguous")
-        if str(block_table.dtype) != "torch.int32" or block_table.dim() != 2:
+        if block_table.dtype is not int32 or block_table.dim() != 2:
             raise ValueError("block_table must be int32 [batch, pages]")
         batch, width = block_table.shape
-        if width > 1 and block_table.stride(1) != 1:
+        stride, inner = block_table.stride()
+        if inner != 1 and width > 1:
             raise ValueError("block_table rows must be contiguous")
-        args = [self._int32_array(query_start, batch + 1, "query_start"), self._int32_array(kv_len, batch, "kv_len"),
-                self._tensor_pointer(block_table, "block_table"),
-                block_table.stride(0) if batch > 1 else width, width, batch]
-        return args, (batch, *shape)
+        if (query_start.dtype is not int32 or query_start.dim() != 1 or query_start.shape[0] <= batch
+                or not query_start.is_contiguous()):
+            raise ValueError("query_start must be a contiguous int32 vector of batch + 1 elements")
+        if (kv_len.dtype is not int32 or kv_len.dim() != 1 or kv_len.shape[0] < batch
+                or not kv_len.is_contiguous()):
+            raise ValueError("kv_len must be a contiguous int32 vector of batch elements")
+        return code, shape, (query_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(),
+                             stride if batch > 1 else width, width, batch)
 
     @staticmethod
     def _head_rows(tensor: Any, head_dim: int, label: str) -> tuple[int, int, int]:
@@ -1489,16 +1490,17 @@ class KudaCudaBridge:
 
         shape, stride = tensor.shape, tensor.stride()
         if len(shape) == 3:
-            cols = shape[1] * shape[2]
-            dense = shape[2] == head_dim and stride[2] == 1 and (shape[1] == 1 or stride[1] == head_dim)
+            rows, heads, d = shape
+            cols = heads * d
+            dense = d == head_dim and stride[2] == 1 and (heads == 1 or stride[1] == head_dim)
         elif len(shape) == 2:
-            cols = shape[1]
+            rows, cols = shape
             dense = stride[1] == 1
         else:
             raise ValueError(f"{label} must be [rows, heads, head_dim] or [rows, heads * head_dim]")
         if not dense or cols % head_dim:
             raise ValueError(f"{label} must have contiguous heads of head_dim elements")
-        return shape[0], cols, (stride[0] if shape[0] > 1 else cols)
+        return rows, cols, (stride[0] if rows > 1 else cols)
 
     def dispatch_rope_append_paged(self, qkv: Any, q_out: Any, k_pages: Any, v_pages: Any, rope_cos: Any,
                                    rope_sin: Any, query_start: Any, kv_len: Any, block_table: Any, *,
@@ -1509,29 +1511,31 @@ class KudaCudaBridge:
         ``rope_cos`` / ``rope_sin`` float32 [max_pos, rotary_dim / 2] (None: no rotation); see
         kudacuda_sm100_rope_append_paged in include/kudacuda.h."""
 
-        code = self._dtype_code(qkv, "qkv")
-        batch_args, (_, num_pages, kv_heads, page_size, head_dim) = self._paged_batch(
-            k_pages, v_pages, query_start, kv_len, block_table, code)
+        dtype = qkv.dtype
+        code, (num_pages, kv_heads, page_size, head_dim), batch = self._paged_batch(
+            dtype, k_pages, v_pages, query_start, kv_len, block_table)
         rows, cols, stride = self._head_rows(qkv, head_dim, "qkv")
         out_rows, out_cols, out_stride = self._head_rows(q_out, head_dim, "q_out")
-        if out_rows != rows or cols != out_cols + 2 * kv_heads * head_dim or self._dtype_code(q_out, "q_out") != code:
+        if out_rows != rows or cols != out_cols + 2 * kv_heads * head_dim or q_out.dtype is not dtype:
             raise ValueError("q_out must hold the query heads of qkv's rows in its dtype")
         max_pos = rotary = cos = sin = 0
         if rope_cos is not None:
-            if (str(rope_cos.dtype) != "torch.float32" or str(rope_sin.dtype) != "torch.float32"
-                    or rope_cos.dim() != 2 or tuple(rope_sin.shape) != tuple(rope_cos.shape)
+            f32 = self._types[2]
+            if (rope_cos.dtype is not f32 or rope_sin.dtype is not f32 or rope_cos.dim() != 2
+                    or rope_sin.shape != rope_cos.shape
                     or not (rope_cos.is_contiguous() and rope_sin.is_contiguous())):
                 raise ValueError("rope_cos and rope_sin must be contiguous float32 [max_pos, rotary_dim / 2]")
-            max_pos, rotary = rope_cos.shape[0], 2 * rope_cos.shape[1]
-            cos, sin = self._tensor_pointer(rope_cos, "rope_cos"), self._tensor_pointer(rope_sin, "rope_sin")
-        if bias is not None and (bias.dim() != 1 or bias.shape[0] != cols or bias.stride(0) != 1
-                                 or self._dtype_code(bias, "bias") != code):
+            max_pos, rotary = rope_cos.shape
+            rotary *= 2
+            cos, sin = rope_cos.data_ptr(), rope_sin.data_ptr()
+        if bias is not None and (bias.dim() != 1 or bias.shape[0] != cols or bias.dtype is not dtype
+                                 or not bias.is_contiguous()):
             raise ValueError("bias must have one element per column of qkv, in its dtype")
-        self._call("kudacuda_sm100_rope_append_paged", code, int(qkv.data_ptr()), stride,
-                   0 if bias is None else int(bias.data_ptr()), int(q_out.data_ptr()), out_stride,
-                   self._tensor_pointer(k_pages, "k_pages"), self._tensor_pointer(v_pages, "v_pages"), cos, sin,
-                   max_pos, rotary, 1 if interleaved else 0, *batch_args, rows, out_cols // head_dim, kv_heads,
-                   head_dim, num_pages, page_size, _normalize_cuda_handle(stream_ptr))
+        self._call("kudacuda_sm100_rope_append_paged", code, qkv.data_ptr(), stride,
+                   0 if bias is None else bias.data_ptr(), q_out.data_ptr(), out_stride, k_pages.data_ptr(),
+                   v_pages.data_ptr(), cos, sin, max_pos, rotary, 1 if interleaved else 0, *batch, rows,
+                   out_cols // head_dim, kv_heads, head_dim, num_pages, page_size,
+                   stream_ptr & 0xFFFFFFFFFFFFFFFF)
 
     def paged_attention_workspace(self, query: Any, k_pages: Any, block_table: Any, *, max_query: int) -> Any:
         """The workspace of dispatch_paged_attention for these shapes (uint8, on the query's device)."""
@@ -1555,23 +1559,22 @@ class KudaCudaBridge:
         ``query`` / ``output`` [rows, q_heads, head_dim] (rows may be strided), ``lse`` float32
         [rows, q_heads] or None; see kudacuda_sm100_paged_attention in include/kudacuda.h."""
 
-        code = self._dtype_code(query, "query")
-        batch_args, (_, num_pages, kv_heads, page_size, head_dim) = self._paged_batch(
-            k_pages, v_pages, query_start, kv_len, block_table, code)
+        dtype = query.dtype
+        code, (num_pages, kv_heads, page_size, head_dim), batch = self._paged_batch(
+            dtype, k_pages, v_pages, query_start, kv_len, block_table)
         rows, cols, stride = self._head_rows(query, head_dim, "query")
         out_rows, out_cols, out_stride = self._head_rows(output, head_dim, "output")
-        if out_rows != rows or out_cols != cols or self._dtype_code(output, "output") != code:
+        if out_rows != rows or out_cols != cols or output.dtype is not dtype:
             raise ValueError("output must have the query's shape and dtype")
-        if lse is not None and (str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (rows, cols // head_dim)
+        heads = cols // head_dim
+        if lse is not None and (lse.dtype is not self._types[2] or lse.shape != (rows, heads)
                                 or not lse.is_contiguous()):
             raise ValueError("lse must be contiguous float32 [rows, q_heads]")
-        self._call("kudacuda_sm100_paged_attention", code, int(query.data_ptr()), stride,
-                   self._tensor_pointer(k_pages, "k_pages"), self._tensor_pointer(v_pages, "v_pages"),
-                   int(output.data_ptr()), out_stride, 0 if lse is None else int(lse.data_ptr()),
-                   self._tensor_pointer(workspace, "workspace"), workspace.numel() * workspace.element_size(),
-                   *batch_args, rows, int(max_query), cols // head_dim, kv_heads, head_dim, num_pages, page_size,
-                   float(scale) if scale is not None else 1.0 / math.sqrt(head_dim),
-                   _normalize_cuda_handle(stream_ptr))
+        self._call("kudacuda_sm100_paged_attention", code, query.data_ptr(), stride, k_pages.data_ptr(),
+                   v_pages.data_ptr(), output.data_ptr(), out_stride, 0 if lse is None else lse.data_ptr(),
+                   workspace.data_ptr(), workspace.nbytes, *batch, rows, max_query, heads, kv_heads, head_dim,
+                   num_pages, page_size, scale if scale is not None else head_dim ** -0.5,
+                   stream_ptr & 0xFFFFFFFFFFFFFFFF)
 
     def dispatch_kv_pages_copy(self, k_pages: Any, v_pages: Any, pairs: Any, *, block_table: Any = None,
                                page_map: Any = None, stream_ptr: int) -> None:
@@ -1581,27 +1584,33 @@ class KudaCudaBridge:
         ``page_map`` (int32 [num_pages]) every valid table entry e becomes page_map[e].  No page may be
         both a source and a target; see kudacuda_sm100_kv_pages_copy in include/kudacuda.h."""
 
-        shape = tuple(k_pages.shape)
-        if len(shape) < 3 or tuple(v_pages.shape) != shape or k_pages.dtype != v_pages.dtype:
+        int32 = self._torch_types()[1]
+        shape = k_pages.shape
+        if len(shape) < 3 or v_pages.shape != shape or k_pages.dtype is not v_pages.dtype:
             raise ValueError("k_pages and v_pages must be [layers, num_pages, ...] of one dtype")
         if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
             raise ValueError("k_pages and v_pages must be contiguous")
-        if str(pairs.dtype) != "torch.int32" or pairs.dim() != 2 or pairs.shape[1] != 2 or not pairs.is_contiguous():
+        if pairs.dtype is not int32 or pairs.dim() != 2 or pairs.shape[1] != 2 or not pairs.is_contiguous():
             raise ValueError("pairs must be contiguous int32 [n, 2]")
-        layer_bytes = k_pages.stride(0) * k_pages.element_size()
-        table = [0, 0, 0, 0]
+        size, num_pages = k_pages.element_size(), shape[1]
+        layer_bytes = k_pages.stride(0) * size
+        table = (0, 0, 0, 0)
         if (block_table is None) != (page_map is None):
             raise ValueError("a block table and a page map come together")
         if block_table is not None:
+            if block_table.dtype is not int32 or block_table.dim() != 2:
+                raise ValueError("block_table must be int32 [rows, pages]")
             rows, width = block_table.shape
-            if str(block_table.dtype) != "torch.int32" or (width > 1 and block_table.stride(1) != 1):
-                raise ValueError("block_table must be int32 [rows, pages] with contiguous rows")
-            table = [int(block_table.data_ptr()), block_table.stride(0) if rows > 1 else width, rows, width]
-        self._call("kudacuda_sm100_kv_pages_copy", self._tensor_pointer(k_pages, "k_pages"),
-                   self._tensor_pointer(v_pages, "v_pages"), shape[0], layer_bytes, shape[1],
-                   layer_bytes // max(1, shape[1]), int(pairs.data_ptr()), pairs.shape[0], *table,
-                   0 if page_map is None else self._int32_array(page_map, shape[1], "page_map"),
-                   _normalize_cuda_handle(stream_ptr))
+            stride, inner = block_table.stride()
+            if inner != 1 and width > 1:
+                raise ValueError("block_table rows must be contiguous")
+            if (page_map.dtype is not int32 or page_map.dim() != 1 or page_map.shape[0] != num_pages
+                    or not page_map.is_contiguous()):
+                raise ValueError("page_map must be contiguous int32 [num_pages]")
+            table = (block_table.data_ptr(), stride if rows > 1 else width, rows, width)
+        self._call("kudacuda_sm100_kv_pages_copy", k_pages.data_ptr(), v_pages.data_ptr(), shape[0], layer_bytes,
+                   num_pages, layer_bytes // max(1, num_pages), pairs.data_ptr(), pairs.shape[0], *table,
+                   0 if page_map is None else page_map.data_ptr(), stream_ptr & 0xFFFFFFFFFFFFFFFF)
 
     def dispatch_sample(self, logits: Any, tokens: Any, uniform: Any, *, temperature: Any = None, top_k: Any = None,
                         top_p: Any = None, min_p: Any = None, logprobs: Any = None, stream_ptr: int) -> None:
@@ -1612,25 +1621,27 @@ class KudaCudaBridge:
         ``tokens`` int32 [rows], ``logprobs`` float32 [rows] or None; see kudacuda_sm100_sample in
         include/kudacuda.h."""
 
-        if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-            raise ValueError("logits must be [rows, vocab] with contiguous rows")
-        code = self._dtype_code(logits, "logits", (0, 1, 2))
+        codes, i32, f32 = self._torch_types()
+        code = codes.get(logits.dtype, -1)
+        if code < 0 or logits.dim() != 2:
+            raise ValueError("logits must be float32, float16 or bfloat16 [rows, vocab]")
         rows, vocab = logits.shape
-
-        def column(tensor: Any, dtype: str, label: str, required: bool = False) -> int:
-            if tensor is None and not required:
-                return 0
-            if (str(tensor.dtype) != dtype or tensor.dim() != 1 or tensor.shape[0] != rows
-                    or (rows > 1 and tensor.stride(0) != 1)):
-                raise ValueError(f"{label} must be a contiguous {dtype} vector of {rows} elements")
-            return int(tensor.data_ptr())
-
-        f32, i32 = "torch.float32", "torch.int32"
-        self._call("kudacuda_sm100_sample", code, int(logits.data_ptr()), logits.stride(0) if rows > 1 else vocab,
-                   rows, vocab, column(temperature, f32, "temperature"), column(top_k, i32, "top_k"),
-                   column(top_p, f32, "top_p"), column(min_p, f32, "min_p"), column(uniform, f32, "uniform", True),
-                   column(tokens, i32, "tokens", True), column(logprobs, f32, "logprobs"),
-                   _normalize_cuda_handle(stream_ptr))
+        stride, inner = logits.stride()
+        if inner != 1 and vocab > 1:
+            raise ValueError("logits must have contiguous rows")
+        pointers = []
+        for tensor, dtype in ((temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (uniform, f32),
+                              (tokens, i32), (logprobs, f32)):
+            if tensor is None:
+                pointers.append(0)
+                continue
+            if (tensor.dtype is not dtype or tensor.dim() != 1 or tensor.shape[0] != rows
+                    or not tensor.is_contiguous()):
+                raise ValueError("temperature, top_k, top_p, min_p, uniform, tokens and logprobs must be contiguous "
+                                 f"[rows] vectors (top_k and tokens int32, the others float32) of {rows} elements")
+            pointers.append(tensor.data_ptr())
+        self._call("kudacuda_sm100_sample", code, logits.data_ptr(), stride if rows > 1 else vocab, rows, vocab,
+                   *pointers, stream_ptr & 0xFFFFFFFFFFFFFFFF)
 
     def error_word(self, *, clear: bool = True) -> int:
         word = ctypes.c_int(0)
