@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const PagedAttentionArgs a) {
     using M = ChunkSmem<D>;
-    using W = PagedWalk<kRows, kKeys>;
+    using W = PagedWalk<kRows, kKeys, kKeys>;
     using Part = PagedPartial<kRows, D>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) ChunkBars bars;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int worker = blockIdx.x;
     int workers = gridDim.x;
     const int64_t total =
-        paged_places<kRows, kKeys, kThreads>(p, group, worker, 1, 1, workers, sums, &place_seq, &place_at);
+        paged_place<W, kKeys, kThreads>(p, group, worker, workers, sums, &place_seq, &place_at);
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = tmem_slot;

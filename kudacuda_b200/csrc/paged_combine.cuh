@@ -34,12 +34,12 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedAttention
     const int owner = blockIdx.x;
     const PagedCut* cuts = Part::cuts(a.workspace);
     const PagedCut cut = cuts[owner];
-    constexpr int kLanes = ROWS < 32 ? ROWS : 32, kShares = 256 / kLanes;
+    constexpr int kLanes = 32, kShares = 256 / kLanes;
     const int lane = threadIdx.x % kLanes, share = threadIdx.x / kLanes;
     const int r = blockIdx.y * kLanes + lane;
     if (!cut.valid || r >= cut.rows) return;
     constexpr int kVecs = (D / 4 + kShares - 1) / kShares;  // float4 of a thread
-    constexpr int kAhead = 4;  // pieces whose loads are in flight together
+    constexpr int kAhead = 2;  // pieces whose loads are in flight together: an item is rarely cut twice
     float m = -INFINITY, l = 0.F;
     float4 acc[kVecs];
 #pragma unroll

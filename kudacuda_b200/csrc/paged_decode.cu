@@ -1,15 +1,16 @@
 // paged_decode.cu -- paged attention with few query rows a key head (decoding):
 // the cache is read once, at the speed of memory.
 //
-// A warp is a worker (paged_plan.cuh): it takes a stretch of the batch's work,
-// items of 16 query rows (mma.m16n8k16's M; a single token of a group of 8
-// fills half of it, which costs nothing here) against blocks of 32 keys, and
-// needs no other warp: its own ring of K and V blocks in shared memory, fetched
-// by TMA page by page (128-byte swizzle), its own barriers, its own running
-// maximum, sum and 16 x head_dim accumulator in registers.  So nothing in the
-// loop waits for anything but memory, and kStages blocks of a warp are in
-// flight: 4 warps x 3 blocks x 16 KB on every SM, seven times what covers the
-// latency of 6.5 TB/s.
+// A block of eight warps is a worker (paged_plan.cuh): it takes a stretch of the
+// batch's work, items of 16 query rows (mma.m16n8k16's M; a single token of a
+// group of 8 fills half of it, which costs nothing here) against blocks of 16
+// keys, which go round the warps.  In the loop a warp needs no other: its own
+// ring of K and V blocks in shared memory, fetched by TMA page by page (128-byte
+// swizzle), its own barriers, its own running maximum, sum and 16 x head_dim
+// accumulator in registers.  So the loop waits for nothing but memory, and
+// two to three blocks of every warp are in flight: 128-192 KB on every SM, three
+// to four times what covers the latency of 6.5 TB/s.  Only at the end of a piece
+// do the warps meet, in shared memory, in a fixed order.
 //
 // S = Q K^T with exact products and 32-bit sums; softmax in the log2 domain; P
 // is split into two 16-bit halves (P = hi + lo to about twice the type's
@@ -26,9 +27,11 @@ namespace kc {
 namespace {
 
 constexpr int kRows = 16;
-constexpr int kKeys = 32;
-constexpr int kWarps = 4;
+constexpr int kKeys = 16;
+constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kOver = 64;             // an item's start and end cost about as much as these keys
+constexpr int kLeast = kKeys * kWarps;  // a worker has a block for every warp
 
 template <int D>
 struct DecodeSmem {
@@ -36,7 +39,8 @@ struct DecodeSmem {
     static constexpr int kBlock = kHalves * kKeys * 128;  // [D / 64][32][128 B]
     static constexpr int kStages = D == 128 ? 3 : 6;
     static constexpr int kWarpBytes = kStages * 2 * kBlock;
-    static constexpr int kBytes = 1024 + kWarps * kWarpBytes;
+    static constexpr int kMeet = kWarps / 2 * kRows * D * 4;  // accumulators of half of the warps
+    static constexpr int kBytes = 1024 + kWarps * kWarpBytes + kMeet;
 };
 
 template <int DT>
@@ -75,16 +79,18 @@ __global__ void __launch_bounds__(kThreads)
     paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const PagedAttentionArgs a) {
     using M = DecodeSmem<D>;
-    using W = PagedWalk<kRows, kKeys>;
+    using W = PagedWalk<kRows, kKeys, kOver>;
     using Part = PagedPartial<kRows, D>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full[kWarps][M::kStages];
-    __shared__ int64_t sums[kWarps], place_at[kWarps];
-    __shared__ int place_seq[kWarps];
+    __shared__ float2 row_ml[kWarps][kRows];  // a warp's (maximum, sum) of a row
+    __shared__ int64_t sums[kWarps], place_at;
+    __shared__ int place_seq;
     const PagedBatch& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint8_t* const ring =
-        smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw)) + warp * M::kWarpBytes;
+    uint8_t* const smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+    uint8_t* const ring = smem + warp * M::kWarpBytes;
+    float* const meet = reinterpret_cast<float*>(smem + kWarps * M::kWarpBytes);
     if (lane == 0) {
         for (int i = 0; i < M::kStages; ++i) mbar_init(&full[warp][i], 1);
         fence_mbar_init();
@@ -92,46 +98,56 @@ __global__ void __launch_bounds__(kThreads)
     pdl_launch_dependents();
     pdl_wait_on_producer();
     const int group = p.q_heads / p.kv_heads;
-    // (worker = warp-major, so that few workers lie on many SMs)
-    const int slots = gridDim.x * kWarps, worker = warp * gridDim.x + blockIdx.x;
-    int workers = slots;
-    const int64_t total = paged_places<kRows, kKeys, kThreads>(p, group, blockIdx.x, gridDim.x, kWarps, workers, sums,
-                                                               place_seq, place_at);
-    W w, ahead;  // the piece at hand; the piece whose blocks are being fetched
-    w.begin(p, group, paged_bound(total, worker, workers), paged_bound(total, worker + 1, workers), place_seq[warp],
-            place_at[warp]);
+    const int worker = blockIdx.x;
+    int workers = gridDim.x;
+    const int64_t total = paged_place<W, kLeast, kThreads>(p, group, worker, workers, sums, &place_seq, &place_at);
+    // the piece at hand; the piece whose blocks this warp is fetching
+    W w, ahead;
+    w.begin(p, group, paged_bound(total, worker, workers), paged_bound(total, worker + 1, workers), place_seq, place_at);
     ahead = w;
-    bool more = ahead.next(p, group);
-    int ahead_j = more ? ahead.t0 : 0;
+    // the stretch's blocks are numbered through; this warp has those with number % kWarps == warp
+    int ahead_j = 0, turn_ahead = 0;
+    bool more;
+    // the next piece with a block of this warp: its queries come into L1 while the blocks before it are worked on
+    auto step = [&]() {
+        while ((more = ahead.next(p, group))) {
+            ahead_j = ahead.t0 + ((warp - turn_ahead) & (kWarps - 1));
+            turn_ahead += ahead.t1 - ahead.t0;
+            if (ahead_j < ahead.t1) break;
+        }
+        const int r = lane & 15;
+        if (more && r < ahead.item_rows) {
+            const int token = (ahead.q * kRows + r) / group, head = (ahead.q * kRows + r) % group;
+            const uint16_t* q = static_cast<const uint16_t*>(a.q) + (ahead.piece_start + token) * a.q_stride +
+                                static_cast<int64_t>(ahead.kvh * group + head) * D + (lane >> 4) * (D / 2);
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
+        }
+    };
+    step();
     uint32_t fetched = 0, used = 0;
 
     // fetch the next block, K and V, into its stage (which its reader has left)
     auto fetch = [&]() {
         if (!more) return;
         const int key0 = ahead_j * kKeys;
-        const int box = min(p.page_size, kKeys);  // keys of a TMA box
-        const int boxes = min(kKeys, ahead.limit - key0 + box - 1) / box;
-        const int part = lane / (2 * M::kHalves), half = (lane >> 1) % M::kHalves, v = lane & 1;
+        const bool some = key0 < ahead.limit;  // (an item without keys has one block without)
         const uint32_t s = fetched % M::kStages;
         uint8_t* const stage = ring + s * 2 * M::kBlock;
-        int row = 0;
-        if (part < boxes) {
-            const int key = key0 + part * box, page = p.table[ahead.piece_b * p.table_stride + key / p.page_size];
-            row = -box;  // a missing page reads as zeros: a box that begins before the tensor
-            if (page >= 0 && page < p.num_pages)
-                row = (page * p.kv_heads + ahead.kvh) * p.page_size + key % p.page_size;
-            else if (p.err != nullptr) atomicOr(p.err, 2);
-        }
-        if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], boxes * box * 128 * M::kHalves * 2);
+        if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], some ? 2 * M::kBlock : 0);
         __syncwarp();
-        if (part < boxes)
-            tma_load_2d(stage + v * M::kBlock + half * (kKeys * 128) + part * box * 128, v ? &map_v : &map_k, half * 64,
-                        row, &full[warp][s]);
-        ++fetched;
-        if (++ahead_j == ahead.t1) {
-            more = ahead.next(p, group);
-            ahead_j = more ? ahead.t0 : 0;
+        if (some && lane < 2 * M::kHalves) {
+            const int half = lane >> 1, v = lane & 1;
+            const int page = p.table[ahead.piece_b * p.table_stride + key0 / p.page_size];
+            int row = -kKeys;  // a missing page reads as zeros: a box that begins before the tensor
+            if (page >= 0 && page < p.num_pages)
+                row = (page * p.kv_heads + ahead.kvh) * p.page_size + key0 % p.page_size;
+            else if (p.err != nullptr) atomicOr(p.err, 2);
+            tma_load_2d(stage + v * M::kBlock + half * (kKeys * 128), v ? &map_v : &map_k, half * 64, row,
+                        &full[warp][s]);
         }
+        ++fetched;
+        ahead_j += kWarps;
+        if (ahead_j >= ahead.t1) step();
     };
     for (int i = 0; i < M::kStages - 1; ++i) fetch();
 
@@ -140,44 +156,49 @@ __global__ void __launch_bounds__(kThreads)
     PagedCut cut;
     cut.valid = cut.tail = cut.row0 = cut.r0 = cut.rows = cut.kvh = cut.last = cut.pad = 0;
     bool ok = true;
+    int turn = 0;
     while (w.next(p, group)) {
-        if (w.piece_len > p.table_width * p.page_size && lane == 0 && p.err != nullptr) atomicOr(p.err, 2);
-        // Q: the A fragments of the item's 16 rows, straight from memory
-        uint32_t qf[D / 16][4];
-        int row_keys[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = g + 8 * h, token = (w.q * kRows + r) / group, head = (w.q * kRows + r) % group;
-            const bool live = r < w.item_rows;
-            const uint16_t* q = static_cast<const uint16_t*>(a.q) +
-                                (live ? (w.piece_start + token) * a.q_stride + static_cast<int64_t>(w.kvh * group + head) * D : 0);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    qf[k][2 * e + h] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 * e + 2 * t4) : 0u;
-            row_keys[h] = live ? min(max(w.piece_len - w.piece_n + token + 1, 0), w.limit) : 0;
-        }
+        if (w.piece_len > p.table_width * p.page_size && tid == 0 && p.err != nullptr) atomicOr(p.err, 2);
+        const int first = w.t0 + ((warp - turn) & (kWarps - 1));
+        turn += w.t1 - w.t0;
         float o[D / 8][4];
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.F;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.F, 0.F};
-        for (int j = w.t0; j < w.t1; ++j) {
+        // Q: the A fragments of the item's 16 rows, straight from memory
+        uint32_t qf[D / 16][4];
+        int row_keys[2] = {0, 0};
+        if (first < w.t1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = g + 8 * h, token = (w.q * kRows + r) / group, head = (w.q * kRows + r) % group;
+                const bool live = r < w.item_rows;
+                const uint16_t* q = static_cast<const uint16_t*>(a.q) +
+                                    (live ? (w.piece_start + token) * a.q_stride + static_cast<int64_t>(w.kvh * group + head) * D : 0);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        qf[k][2 * e + h] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 * e + 2 * t4) : 0u;
+                row_keys[h] = live ? min(max(w.piece_len - w.piece_n + token + 1, 0), w.limit) : 0;
+            }
+        }
+        for (int j = first; j < w.t1; j += kWarps) {
             fetch();
             const uint32_t s = used % M::kStages;
-            if (!mbar_wait_bounded(&full[warp][s], (used / M::kStages) & 1)) ok = false;
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
+            ok = ok && mbar_wait_bounded(&full[warp][s], (used / M::kStages) & 1);
             ++used;
+            if (!__all_sync(0xffffffffu, ok)) {  // the piece stays wrong, the error word says so
+                ok = false;
+                continue;
+            }
             const uint32_t kb = smem_u32(ring + s * 2 * M::kBlock), vb = kb + M::kBlock;
             // S: 16 rows x 32 keys, four tiles of 8 keys
-            float sc[4][4];
+            float sc[kKeys / 8][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.F;
+            for (int n = 0; n < kKeys / 8; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.F;
 #pragma unroll
-            for (int n2 = 0; n2 < 2; ++n2) {
+            for (int n2 = 0; n2 < kKeys / 16; ++n2) {
                 // ldmatrix: keys 16 n2 .. + 15 (two tiles), 16 dims (two 8-dim words)
                 const int key = 16 * n2 + (lane & 7) + ((lane >> 4) << 3);
                 const uint32_t row = kb + key * 128;
@@ -194,7 +215,7 @@ __global__ void __launch_bounds__(kThreads)
             const int valid = w.limit - key0;  // keys of the block that exist
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int key = key0 + 8 * n + 2 * t4 + (e & 1);
@@ -223,9 +244,9 @@ __global__ void __launch_bounds__(kThreads)
             }
             const float sub[2] = {m[0] == -INFINITY ? 0.F : m[0], m[1] == -INFINITY ? 0.F : m[1]};
             // P in A-fragment order, 16 keys a fragment, as hi + lo
-            uint32_t ph[2][4], pl[2][4];
+            uint32_t ph[kKeys / 16][4], pl[kKeys / 16][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float e0 = ex2(sc[n][2 * h] - sub[h]), e1 = ex2(sc[n][2 * h + 1] - sub[h]);
@@ -236,7 +257,7 @@ __global__ void __launch_bounds__(kThreads)
                     pl[n >> 1][2 * (n & 1) + h] = pack2<DT>(e0 - back.x, e1 - back.y);
                 }
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
+            for (int kk = 0; kk < kKeys / 16; ++kk) {
                 const int key = 16 * kk + (lane & 15);
                 const uint32_t row = vb + key * 128;
                 // slots without a key may hold anything, a NaN too: their V must not meet P = 0
@@ -266,60 +287,152 @@ __global__ void __launch_bounds__(kThreads)
             // next fetch() begins with the warp's barrier) before the copy starts
             __syncwarp();
         }
-        if (!ok) break;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            if (t4 == 0) row_ml[warp][g + 8 * h] = make_float2(m[h], l[h]);
         }
-        if (w.whole()) {
+        // The warps meet: every one brings its accumulator to the row's maximum, the
+        // upper four leave theirs, the lower four add one each and leave the sum, and
+        // all threads add those four.  (columns are swizzled by the row)
+        __syncthreads();
+        float f[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = g + 8 * h;
-                if (r >= w.item_rows) continue;
+        for (int h = 0; h < 2; ++h) {
+            float mx = row_ml[0][g + 8 * h].x;
+            for (int i = 1; i < kWarps; ++i) mx = fmaxf(mx, row_ml[i][g + 8 * h].x);
+            f[h] = m[h] == -INFINITY ? 0.F : ex2(m[h] - mx);
+        }
+        float* const spot = meet + (warp & 3) * kRows * D;
+        auto place = [&](int i, int h) {
+            return reinterpret_cast<float2*>(spot + (g + 8 * h) * D + (8 * (i ^ g) + 2 * t4));
+        };
+        if (warp >= 4) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) *place(i, h) = make_float2(o[i][2 * h] * f[h], o[i][2 * h + 1] * f[h]);
+        }
+        __syncthreads();
+        if (warp < 4) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float2 x = *place(i, h);
+                    *place(i, h) = make_float2(o[i][2 * h] * f[h] + x.x, o[i][2 * h + 1] * f[h] + x.y);
+                }
+        }
+        __syncthreads();
+        const bool whole = w.whole();
+        float* const part = Part::slot(a.workspace, gridDim.x, worker, w.t0 > 0 ? 0 : 1);
+        for (int i = tid; i < w.item_rows * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), d = 4 * (i % (D / 4));
+            float mx = -INFINITY, sum = 0.F;
+            for (int v = 0; v < kWarps; ++v) mx = fmaxf(mx, row_ml[v][r].x);
+            for (int v = 0; v < kWarps; ++v) {
+                const float2 x = row_ml[v][r];
+                if (x.x != -INFINITY) sum += x.y * ex2(x.x - mx);
+            }
+            const float* at = meet + r * D + ((((d >> 3) ^ (r & 7)) << 3) | (d & 7));
+            float4 x = *reinterpret_cast<const float4*>(at);
+#pragma unroll
+            for (int v = 1; v < 4; ++v) {
+                const float4 y = *reinterpret_cast<const float4*>(at + v * kRows * D);
+                x.x += y.x;
+                x.y += y.y;
+                x.z += y.z;
+                x.w += y.w;
+            }
+            if (whole) {
                 const int64_t row = w.piece_start + (w.q * kRows + r) / group;
                 const int head = w.kvh * group + (w.q * kRows + r) % group;
-                const float inv = l[h] > 0.F ? 1.F / l[h] : 0.F;
-                uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * t4) = pack2<DT>(o[i][2 * h] * inv, o[i][2 * h + 1] * inv);
-                if (t4 == 0 && a.lse != nullptr)
-                    a.lse[row * p.q_heads + head] = l[h] > 0.F ? m[h] * kLn2 + logf(l[h]) : -INFINITY;
-            }
-        } else {
-            float* part = Part::slot(a.workspace, slots, worker, w.t0 > 0 ? 0 : 1);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = g + 8 * h;
-                if (r >= w.item_rows) continue;
-                if (t4 == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m[h], l[h]);
-                float* acc = part + 2 * kRows;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const int d = 8 * i + 2 * t4;
-                    __stcg(reinterpret_cast<float2*>(acc + ((d >> 2) * kRows + r) * 4 + (d & 3)),
-                           make_float2(o[i][2 * h], o[i][2 * h + 1]));
-                }
-            }
-            if (w.t0 > 0) {
-                cut.tail = 1;
+                const float inv = sum > 0.F ? 1.F / sum : 0.F;
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.out_stride +
+                                          static_cast<int64_t>(head) * D + d) =
+                    make_uint2(pack2<DT>(x.x * inv, x.y * inv), pack2<DT>(x.z * inv, x.w * inv));
+                if (d == 0 && a.lse != nullptr)
+                    a.lse[row * p.q_heads + head] = sum > 0.F ? mx * kLn2 + logf(sum) : -INFINITY;
             } else {
-                cut.valid = 1;
-                cut.row0 = w.piece_start;
-                cut.r0 = w.q * kRows;
-                cut.rows = w.item_rows;
-                cut.kvh = w.kvh;
-                cut.last = static_cast<int>((w.item_end * workers + total - 1) / total - 1);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(part) + r, make_float2(mx, sum));
+                __stcg(reinterpret_cast<float4*>(part + 2 * kRows + r * D + d), x);
             }
         }
+        if (!whole && w.t0 > 0) {
+            cut.tail = 1;
+        } else if (!whole) {
+            cut.valid = 1;
+            cut.row0 = w.piece_start;
+            cut.r0 = w.q * kRows;
+            cut.rows = w.item_rows;
+            cut.kvh = w.kvh;
+            cut.last = static_cast<int>((w.item_end * workers + total - 1) / total - 1);
+        }
+        __syncthreads();  // `meet` and `row_ml` are free again
     }
     if (!ok) {
         if (lane == 0 && p.err != nullptr) atomicOr(p.err, 16);
         // no copy may still be on its way when the block ends
-        for (; used < fetched; ++used) mbar_wait_bounded(&full[warp][used % M::kStages], (used / M::kStages) & 1);
+        for (uint32_t i = fetched > M::kStages ? fetched - M::kStages : 0; i < fetched; ++i)
+            mbar_wait_bounded(&full[warp][i % M::kStages], (i / M::kStages) & 1);
     }
-    if (lane == 0) Part::cuts(a.workspace)[worker] = cut;
+    if (tid == 0) Part::cuts(a.workspace)[worker] = cut;
+}
+
+// The join of cut items (paged_combine.cuh): a thread takes four dims of a row,
+// four pieces in flight.
+constexpr int kJoinThreads = 256;
+template <int DT, int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttentionArgs a) {
+    using Part = PagedPartial<kRows, D>;
+    constexpr int kAhead = 4;
+    pdl_launch_dependents();
+    pdl_wait_on_producer();
+    const int owner = blockIdx.x, workers = gridDim.x;
+    const PagedCut* cuts = Part::cuts(a.workspace);
+    const PagedCut cut = cuts[owner];
+    if (!cut.valid) return;
+    const int last = min(cut.last, workers - 1);
+    const PagedBatch& p = a.p;
+    const int group = p.q_heads / p.kv_heads;
+    for (int i = threadIdx.x; i < cut.rows * (D / 4); i += kJoinThreads) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        float m = -INFINITY, l = 0.F;
+        float4 acc = make_float4(0.F, 0.F, 0.F, 0.F);
+        for (int c0 = owner; c0 <= last; c0 += kAhead) {
+            float2 ml[kAhead];
+            float4 x[kAhead];
+            bool there[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                // (read whether it is there or not: one round trip for everything)
+                const int c = min(c0 + u, last);
+                there[u] = c0 + u <= last && (c == owner || cuts[c].tail);
+                const float* part = Part::slot(a.workspace, workers, c, c == owner ? 1 : 0);
+                ml[u] = __ldcg(reinterpret_cast<const float2*>(part) + r);
+                x[u] = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * D + d));
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (!there[u]) continue;
+                const float mn = fmaxf(m, ml[u].x);
+                const float f = m == -INFINITY ? 0.F : ex2(m - mn), g = ml[u].x == -INFINITY ? 0.F : ex2(ml[u].x - mn);
+                l = l * f + ml[u].y * g;
+                acc.x = acc.x * f + x[u].x * g;
+                acc.y = acc.y * f + x[u].y * g;
+                acc.z = acc.z * f + x[u].z * g;
+                acc.w = acc.w * f + x[u].w * g;
+                m = mn;
+            }
+        }
+        const int64_t row = cut.row0 + (cut.r0 + r) / group;
+        const int head = cut.kvh * group + (cut.r0 + r) % group;
+        const float inv = l > 0.F ? 1.F / l : 0.F;
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D + d) =
+            make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+        if (d == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
+    }
 }
 
 constexpr int kMaxBlocks = 148;
@@ -328,7 +441,7 @@ template <int DT, int D>
 cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     const PagedBatch& p = a.p;
     const uint64_t rows = static_cast<uint64_t>(p.num_pages) * p.kv_heads * p.page_size;
-    const uint32_t box = p.page_size < kKeys ? p.page_size : kKeys;
+    const uint32_t box = kKeys;  // no page is smaller
     CUtensorMap mk, mv;
     const CUtensorMapDataType type =
         DT == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -345,14 +458,14 @@ cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     const int blocks = device_sm_count() < kMaxBlocks ? device_sm_count() : kMaxBlocks;
     st = launch_pdl(kernel, dim3(blocks), dim3(kThreads), DecodeSmem<D>::kBytes, s, mk, mv, a);
     if (st != cudaSuccess) return st;
-    return launch_pdl(paged_combine_kernel<DT, D, kRows>, dim3(blocks * kWarps, 1), dim3(256), 0, s, a, blocks * kWarps);
+    return launch_pdl(paged_join_kernel<DT, D>, dim3(blocks), dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace
 
 int64_t paged_decode_workspace_bytes(int head_dim) {
-    return head_dim == 128 ? PagedPartial<kRows, 128>::bytes(kMaxBlocks * kWarps)
-                           : PagedPartial<kRows, 64>::bytes(kMaxBlocks * kWarps);
+    return head_dim == 128 ? PagedPartial<kRows, 128>::bytes(kMaxBlocks)
+                           : PagedPartial<kRows, 64>::bytes(kMaxBlocks);
 }
 
 cudaError_t paged_decode(const PagedAttentionArgs& a, int dt, cudaStream_t s) {

@@ -4,8 +4,8 @@
 // A sequence with n new tokens and G query heads per key head has n * G query
 // rows per key head (row R: token R / G, head R % G); ROWS of them are a tile,
 // and (sequence, key head, tile) is an item whose keys come in blocks of KT.
-// Every item has a cost (its last row's keys, counted per query row, and one
-// block for its start and end), the items stand in one line, and worker c of N
+// Every item has a cost (its last row's keys, counted per query row, and OVER
+// keys for its start and end), the items stand in one line, and worker c of N
 // takes the stretch [c U / N, (c + 1) U / N) of the total cost U.  A stretch
 // that ends inside an item is rounded down to a block, by the same formula for
 // both neighbours, so lengths of any mix load every worker alike and an item
@@ -36,10 +36,9 @@ struct PagedCut {
 __device__ __forceinline__ int64_t paged_bound(int64_t total, int worker, int workers) {
     return worker >= workers ? total : total * worker / workers;
 }
-// No more workers than blocks of keys: every worker that has work has a block
-// or two, and an item has no more pieces than blocks.
-__device__ __forceinline__ int paged_workers(int64_t total, int group, int block, int workers) {
-    return static_cast<int>(min(max(total / (static_cast<int64_t>(group) * block), static_cast<int64_t>(1)),
+// No more workers than there is work for: `least` keys a worker.
+__device__ __forceinline__ int paged_workers(int64_t total, int group, int least, int workers) {
+    return static_cast<int>(min(max(total / (static_cast<int64_t>(group) * least), static_cast<int64_t>(1)),
                                 static_cast<int64_t>(workers)));
 }
 
@@ -55,7 +54,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& p, int b) {
     return s;
 }
 
-template <int ROWS, int KT>
+template <int ROWS, int KT, int OVER>
 struct PagedWalk {
     // the line
     int64_t x0, x1;
@@ -70,7 +69,7 @@ struct PagedWalk {
 
     // cost of the first k tiles of a key head
     __device__ __forceinline__ int64_t cost(int group, int k) const {
-        const int64_t base = static_cast<int64_t>(max(len - n, 0) + KT) * group;
+        const int64_t base = static_cast<int64_t>(max(len - n, 0) + OVER) * group;
         if (k >= tiles_q)
             return tiles_q * base + static_cast<int64_t>(ROWS / 2) * (tiles_q - 1) * tiles_q + rows;
         return k * base + static_cast<int64_t>(ROWS / 2) * k * (k + 1);
@@ -148,16 +147,16 @@ struct PagedWalk {
 };
 
 // Block-wide: the total cost, the number of workers that share it (at most
-// `workers`), and for the `count` workers first + i * step the sequence in which
-// each one's stretch begins (seq) and that sequence's place (at).  `sums` has
-// one word per warp.  Ends with a barrier.
-template <int ROWS, int KT, int THREADS>
-__device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, int first, int step, int count,
-                                                int& workers, int64_t* sums, int* seq, int64_t* at) {
+// `workers`, each with LEAST keys or more), and for worker `mine` the sequence in
+// which its stretch begins (seq) and that sequence's place (at).  `sums` has one
+// word per warp.  Ends with a barrier.
+template <class W, int LEAST, int THREADS>
+__device__ __forceinline__ int64_t paged_place(const PagedBatch& p, int group, int worker, int& workers,
+                                               int64_t* sums, int* seq, int64_t* at) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b0 = static_cast<int>(static_cast<int64_t>(p.batch) * tid / THREADS);
     const int b1 = static_cast<int>(static_cast<int64_t>(p.batch) * (tid + 1) / THREADS);
-    PagedWalk<ROWS, KT> w;
+    W w;
     int64_t mine = 0;
     for (w.b = b0; w.b < b1; ++w.b) {
         w.load(p, group);
@@ -170,9 +169,9 @@ __device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, 
         if (lane >= o) upto += v;
     }
     if (lane == 31) sums[warp] = upto;
-    if (tid < count) {
-        seq[tid] = p.batch;
-        at[tid] = 0;
+    if (tid == 0) {
+        *seq = p.batch;
+        *at = 0;
     }
     __syncthreads();
     int64_t total = 0, before = 0;
@@ -181,11 +180,9 @@ __device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, 
         total += sums[i];
     }
     int64_t from = before + upto - mine;
-    workers = paged_workers(total, group, KT, workers);
-    for (int i = 0; i < count; ++i) {
-        if (first + i * step >= workers) break;
-        const int64_t x = paged_bound(total, first + i * step, workers);
-        if (mine == 0 || x < from || x >= from + mine) continue;
+    workers = paged_workers(total, group, LEAST, workers);
+    const int64_t x = paged_bound(total, worker, workers);
+    if (worker < workers && mine > 0 && x >= from && x < from + mine) {
         int64_t c = from;
         for (w.b = b0; w.b < b1; ++w.b) {
             w.load(p, group);
@@ -193,8 +190,8 @@ __device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, 
             if (x < e) break;
             c = e;
         }
-        seq[i] = w.b;
-        at[i] = c;
+        *seq = w.b;
+        *at = c;
     }
     __syncthreads();
     return total;
@@ -202,7 +199,7 @@ __device__ __forceinline__ int64_t paged_places(const PagedBatch& p, int group, 
 
 // Where a worker's partial results lie: slot 0 the end of an item begun by an
 // earlier worker, slot 1 the beginning of an item that later ones end.  A slot
-// is ROWS (maximum, sum) pairs and the accumulator as float4 [D / 4][ROWS].
+// is ROWS (maximum, sum) pairs and the accumulator, as its writer finds it best.
 template <int ROWS, int D>
 struct PagedPartial {
     static constexpr int64_t kFloats = static_cast<int64_t>(ROWS) * (D + 2);
