@@ -40,4 +40,19 @@ cudaError_t encode_tmap_2d(CUtensorMap* out, CUtensorMapDataType dtype, const vo
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t encode_tmap_3d(CUtensorMap* out, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                           uint64_t rows, uint64_t planes, uint64_t row_stride, uint64_t plane_stride,
+                           uint32_t box_inner, uint32_t box_rows, uint32_t box_planes, CUtensorMapSwizzle swizzle,
+                           CUtensorMapL2promotion promotion) {
+    EncodeTiledFn f = encode_fn();
+    if (f == nullptr) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {inner, rows, planes};
+    const cuuint64_t strides[2] = {row_stride, plane_stride};
+    const cuuint32_t box[3] = {box_inner, box_rows, box_planes};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = f(out, dtype, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 }  // namespace kc

@@ -22,4 +22,11 @@ cudaError_t encode_tmap_2d(CUtensorMap* out, CUtensorMapDataType dtype, const vo
                            uint64_t rows, uint64_t row_stride, uint32_t box_inner, uint32_t box_rows,
                            CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion);
 
+// 3D tensor [planes][rows][inner], rows row_stride and planes plane_stride bytes
+// apart; box = box_planes x box_rows x box_inner.
+cudaError_t encode_tmap_3d(CUtensorMap* out, CUtensorMapDataType dtype, const void* base, uint64_t inner,
+                           uint64_t rows, uint64_t planes, uint64_t row_stride, uint64_t plane_stride,
+                           uint32_t box_inner, uint32_t box_rows, uint32_t box_planes, CUtensorMapSwizzle swizzle,
+                           CUtensorMapL2promotion promotion);
+
 }  // namespace kc

@@ -14,7 +14,7 @@
 // The final O / l does not depend on m.
 //
 // Warps: 0-3 and 4-7 softmax, tile 0 and 1; 8 K/V producer (TMA, one box per
-// page and 64 dims, 128-byte swizzle); 9 MMA issuer; 10 loads Q and clears the
+// page and 64 dims, 128-byte swizzle); 9 MMA issuer; 10 fetches Q and clears the
 // rows of the last V block past the item's last key (their P is 0, but 0 times
 // a NaN in an unused slot is not); 11 idle.
 #include <cuda_bf16.h>
@@ -69,6 +69,56 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {  // NaN if one is
+    float m;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
+// two 32-bit numbers in a register pair
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float low(uint64_t v) {
+    float x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+    return x;
+}
+__device__ __forceinline__ float high(uint64_t v) {
+    float x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+    return y;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+// 2^x of a pair on the fma pipes, for some of the keys: 2^x instructions of 16 a
+// clock would need as long for a block as its matrix products.  x = n + f with n
+// whole (adding 1.5 2^23 rounds it into the low mantissa bits) and |f| <= 1/2; 2^f by a
+// polynomial of degree 4, fitted to the least relative error (2.7e-6); n is added
+// to the exponent.  x is at most a few; below -126 it counts as -126.
+__device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
+    const uint64_t magic = pair(12582912.F, 12582912.F), minus = pair(-12582912.F, -12582912.F);
+    x = pair(fmaxf(low(x), -126.F), fmaxf(high(x), -126.F));
+    const uint64_t n = add2(x, magic);
+    const uint64_t f = fma2(add2(n, minus), pair(-1.F, -1.F), x);
+    uint64_t p = fma2(f, pair(0.009570102207362652F, 0.009570102207362652F), pair(0.05591785907745361F, 0.05591785907745361F));
+    p = fma2(p, f, pair(0.240247443318367F, 0.240247443318367F));
+    p = fma2(p, f, pair(0.6931217908859253F, 0.6931217908859253F));
+    p = fma2(p, f, pair(0.9999992847442627F, 0.9999992847442627F));
+    return pair(__int_as_float(__float_as_int(low(p)) + (__float_as_int(low(n)) << 23)),
+                __int_as_float(__float_as_int(high(p)) + (__float_as_int(high(n)) << 23)));
+}
+constexpr uint32_t kByPoly = 0x52;  // which of eight pairs go by the polynomial (three)
+
 // the item's last block has rows without a key
 __device__ __forceinline__ bool has_tail(int limit) { return limit % kKeys != 0 || limit == 0; }
 
@@ -76,13 +126,13 @@ struct ChunkBars {
     uint64_t kv_full[8], kv_empty[8];
     uint64_t v_tail[8];  // the last V block of an item has landed, rows past its last key not cleared yet
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_ready[2], o_done[2];
+    uint64_t s_full[2], p_half[2], p_ready[2], o_done[2];
 };
 
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                       const PagedAttentionArgs a) {
+                       const __grid_constant__ CUtensorMap map_q, const PagedAttentionArgs a, int q_by_tma) {
     using M = ChunkSmem<D>;
     using W = PagedWalk<kRows, kKeys, kKeys>;
     using Part = PagedPartial<kRows, D>;
@@ -113,6 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bars.q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_half[i], 128);
             mbar_init(&bars.p_ready[i], 128);
             mbar_init(&bars.o_done[i], 1);
         }
@@ -123,15 +174,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_wait_on_producer();
     const int group = p.q_heads / p.kv_heads;
     const int worker = blockIdx.x;
-    int workers = gridDim.x;
-    const int64_t total =
-        paged_place<W, kKeys, kThreads>(p, group, worker, workers, sums, &place_seq, &place_at);
+    const PagedShares shares =
+        paged_place<W, kKeys, kThreads>(p, group, worker, gridDim.x, sums, &place_seq, &place_at);
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = tmem_slot;
     volatile int* const abort_p = &abort_flag;
     W w;
-    w.begin(p, group, paged_bound(total, worker, workers), paged_bound(total, worker + 1, workers), place_seq, place_at);
+    w.begin(p, group, shares, worker, place_seq, place_at);
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -200,13 +250,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint32_t ka = r_addr + (sk % M::kStages) * M::kTile;
                         for (int t = 0; t < active; ++t) {
                             if (j > 0) {
-                                bar_wait(&bars.p_ready[t], np[t]++ & 1, abort_p);
-                                tc_fence_after();
+                                // (the first half of P multiplies while the second is still being made)
 #pragma unroll
-                                for (int k = 0; k < kKeys / 16; ++k)
-                                    umma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
-                                                 umma_desc_sw128_mn(va + 2048 * k, 128 * 128), kIdescO,
-                                                 (j > 1 || k > 0) ? 1u : 0u);
+                                for (int h = 0; h < 2; ++h) {
+                                    bar_wait(h ? &bars.p_ready[t] : &bars.p_half[t], np[t] & 1, abort_p);
+                                    tc_fence_after();
+#pragma unroll
+                                    for (int k = h * (kKeys / 32); k < (h + 1) * (kKeys / 32); ++k)
+                                        umma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
+                                                     umma_desc_sw128_mn(va + 2048 * k, 128 * 128), kIdescO,
+                                                     (j > 1 || k > 0) ? 1u : 0u);
+                                }
+                                ++np[t];
                             }
                             if (j < n) {
 #pragma unroll
@@ -234,34 +289,38 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- Q: row R of the item is token R / group, head R % group; rows past the item are zero
             uint32_t items = 0, seq = 0, tail_parity = 0;
             const uint16_t* q = static_cast<const uint16_t*>(a.q);
-            constexpr int kChunks = D / 8, kAbreast = 32 / kChunks;  // 16-byte chunks of a row, rows a pass
-            const int c = lane % kChunks, sub = lane / kChunks;
             while (w.next(p, group)) {
                 // (a long wait: the whole of the piece before)
                 if (items > 0 && !bar_wait(&bars.q_empty, (items - 1) & 1, abort_p, true, 1u << 22)) break;
                 const int r_all = w.item_rows > 128 ? 256 : 128;
-                int token = (w.q * kRows + sub) / group, head = (w.q * kRows + sub) % group;
-                for (int r = sub; r < r_all; r += kAbreast) {
-                    const uint32_t dst = smem_u32(qs) + (r >> 7) * M::kTile + (c >> 3) * (128 * 128) + (r & 127) * 128 +
-                                         (((c & 7) ^ (r & 7)) << 4);
-                    const bool live = r < w.item_rows;
-                    const uint16_t* src =
-                        q + (live ? (w.piece_start + token) * a.q_stride +
-                                        static_cast<int64_t>(w.kvh * group + head) * D + c * 8
-                                  : 0);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                                 "r"(live ? 16 : 0)
-                                 : "memory");
-                    head += kAbreast;
-                    while (head >= group) {
-                        head -= group;
-                        ++token;
+                if (q_by_tma) {  // 128 / group whole tokens a tile (rows past the item are other tokens': not stored)
+                    if (lane == 0) mbar_arrive_expect_tx(&bars.q_full, r_all * D * 2);
+                    __syncwarp();
+                    const int t = lane / M::kHalves, half = lane % M::kHalves;
+                    if (t * 128 < r_all)
+                        tma_load_3d(qs + t * M::kTile + half * (128 * 128), &map_q, half * 64, w.kvh * group,
+                                    w.piece_start + (w.q * kRows + t * 128) / group, &bars.q_full);
+                } else {
+                    for (int r = lane; r < r_all; r += 32) {  // a lane a row
+                        const bool live = r < w.item_rows;
+                        const int token = (w.q * kRows + r) / group, head = (w.q * kRows + r) - token * group;
+                        const uint16_t* src =
+                            q + (live ? (w.piece_start + token) * a.q_stride +
+                                            static_cast<int64_t>(w.kvh * group + head) * D
+                                      : 0);
+                        const uint32_t dst = smem_u32(qs) + (r >> 7) * M::kTile + (r & 127) * 128;
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                             dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)),
+                                         "l"(src + 8 * c), "r"(live ? 16 : 0)
+                                         : "memory");
                     }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&bars.q_full);
                 }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.q_full);
                 ++items;
                 seq += 2 * (w.t1 - w.t0);
                 if (w.t1 == w.tiles && has_tail(w.limit)) {
@@ -279,6 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) bar_arrive(&bars.kv_full[sv]);
                 }
             }
+            if (q_by_tma && items > 0) bar_wait(&bars.q_full, (items - 1) & 1, abort_p, false);  // Q has landed
         }
     } else {
         // ---- softmax: thread = row
@@ -304,19 +364,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < kKeys; i += 32) tmem_ld32(ts + i, s + i);
                 tmem_wait_ld();
                 const int keys = row_keys - j * kKeys;
-                if (__any_sync(0xffffffffu, keys < kKeys)) {
+                const bool masked = __any_sync(0xffffffffu, keys < kKeys);
+                if (masked) {
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i) s[i] = i < keys ? s[i] : -INFINITY;
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
+                float mx[2] = {s[0], s[1]};
 #pragma unroll
-                for (int i = 4; i < kKeys; i += 4) {
-                    mx[0] = fmaxf(mx[0], s[i]);
-                    mx[1] = fmaxf(mx[1], s[i + 1]);
-                    mx[2] = fmaxf(mx[2], s[i + 2]);
-                    mx[3] = fmaxf(mx[3], s[i + 3]);
+                for (int i = 2; i < kKeys - 2; i += 4) {
+                    mx[0] = max3(mx[0], s[i], s[i + 1]);
+                    mx[1] = max3(mx[1], s[i + 2], s[i + 3]);
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                const float top = max3(max3(mx[0], s[kKeys - 2], s[kKeys - 1]), mx[1], mx[1]) * c;
+                if (top != top) l = top;  // a NaN score makes the row NaN
                 const bool grow = top > m + kLazy;  // from -inf: any finite maximum
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mn = grow ? top : m;
@@ -337,30 +397,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 const float sub = m == -INFINITY ? 0.F : m;
-                float sum[4] = {0.F, 0.F, 0.F, 0.F};
+                const uint64_t c2 = pair(c, c), sub2 = pair(-sub, -sub);
+                uint64_t sum2[2] = {0, 0};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t pk[32];
+                    if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float e0 = ex2(fmaf(s[64 * h + 2 * i], c, -sub));
-                        const float e1 = ex2(fmaf(s[64 * h + 2 * i + 1], c, -sub));
-                        sum[(2 * i) & 3] += e0;
-                        sum[(2 * i + 1) & 3] += e1;
-                        pk[i] = pack2<DT>(e0, e1);
+                        for (int i = 0; i < 32; ++i) {
+                            const uint64_t x = fma2(pair(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), c2, sub2);
+                            const uint64_t e = pair(ex2(low(x)), ex2(high(x)));
+                            sum2[i & 1] = add2(sum2[i & 1], e);
+                            pk[i] = pack2<DT>(low(e), high(e));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const uint64_t x = fma2(pair(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), c2, sub2);
+                            const uint64_t e = kByPoly >> (i & 7) & 1 ? ex2_poly(x) : pair(ex2(low(x)), ex2(high(x)));
+                            sum2[i & 1] = add2(sum2[i & 1], e);
+                            pk[i] = pack2<DT>(low(e), high(e));
+                        }
                     }
                     tmem_st32(ts + 32 * h, pk);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    bar_arrive(h ? &bars.p_ready[t] : &bars.p_half[t]);
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                bar_arrive(&bars.p_ready[t]);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                sum2[0] = add2(sum2[0], sum2[1]);
+                l += low(sum2[0]) + high(sum2[0]);
             }
             // ---- the piece's end
             bar_wait(&bars.o_done[t], no++ & 1, abort_p);
             tc_fence_after();
             if (w.whole()) {
-                const float inv = l > 0.F ? 1.F / l : 0.F;
+                const float inv = l == 0.F ? 0.F : 1.F / l;
                 const int64_t row = w.piece_start + token;
                 const int head = w.kvh * group + (w.q * kRows + r) % group;
                 uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
@@ -377,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                            pack2<DT>(o[k + 4] * inv, o[k + 5] * inv), pack2<DT>(o[k + 6] * inv, o[k + 7] * inv));
                     }
                 }
-                if (live && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
+                if (live && a.lse != nullptr) a.lse[row * p.q_heads + head] = l == 0.F ? -INFINITY : m * kLn2 + logf(l);
             } else {
                 float* part = Part::slot(a.workspace, gridDim.x, worker, w.t0 > 0 ? 0 : 1);
                 *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, l);
@@ -398,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // what the combine kernel needs to know of this worker's cut items
     if (tid == 352) {
         W v;
-        v.begin(p, group, paged_bound(total, worker, workers), paged_bound(total, worker + 1, workers), place_seq, place_at);
+        v.begin(p, group, shares, worker, place_seq, place_at);
         PagedCut cut;
         cut.valid = cut.tail = cut.row0 = cut.r0 = cut.rows = cut.kvh = cut.last = cut.pad = 0;
         while (v.next(p, group)) {
@@ -409,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 cut.r0 = v.q * kRows;
                 cut.rows = v.item_rows;
                 cut.kvh = v.kvh;
-                cut.last = static_cast<int>((v.item_end * workers + total - 1) / total - 1);
+                cut.last = shares.of(v.item_end - 1);
             }
         }
         Part::cuts(a.workspace)[worker] = cut;
@@ -432,7 +503,7 @@ template <int DT, int D>
 cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t s) {
     const PagedBatch& p = a.p;
     const uint64_t rows = static_cast<uint64_t>(p.num_pages) * p.kv_heads * p.page_size;
-    CUtensorMap mk, mv;
+    CUtensorMap mk, mv, mq;
     const CUtensorMapDataType type =
         DT == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     cudaError_t st = encode_tmap_2d(&mk, type, a.k_pages, D, rows, D * 2, 64, p.page_size, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -441,12 +512,22 @@ cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t s) {
         st = encode_tmap_2d(&mv, type, a.v_pages, D, rows, D * 2, 64, p.page_size, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     if (st != cudaSuccess) return st;
+    // a tile of 128 rows is whole tokens when the group divides it: then Q comes by TMA too
+    const int group = p.q_heads / p.kv_heads;
+    const int by_tma = group <= 128 && 128 % group == 0 ? 1 : 0;
+    if (by_tma) {
+        st = encode_tmap_3d(&mq, type, a.q, D, p.q_heads, p.rows, D * 2, a.q_stride * 2, 64, group, 128 / group,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+        if (st != cudaSuccess) return st;
+    } else {
+        mq = mk;
+    }
     auto kernel = paged_chunk_kernel<DT, D>;
     static std::atomic<uint64_t> opted{0};
     st = opt_in_smem(reinterpret_cast<const void*>(kernel), ChunkSmem<D>::kBytes, opted);
     if (st != cudaSuccess) return st;
     const int workers = device_sm_count() < kMaxWorkers ? device_sm_count() : kMaxWorkers;
-    st = launch_pdl(kernel, dim3(workers), dim3(kThreads), ChunkSmem<D>::kBytes, s, mk, mv, a);
+    st = launch_pdl(kernel, dim3(workers), dim3(kThreads), ChunkSmem<D>::kBytes, s, mk, mv, mq, a, by_tma);
     if (st != cudaSuccess) return st;
     return launch_pdl(paged_combine_kernel<DT, D, kRows>, dim3(workers, kRows / 32), dim3(256), 0, s, a, workers);
 }

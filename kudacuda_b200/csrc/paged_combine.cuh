@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedAttention
     const int group = p.q_heads / p.kv_heads;
     const int64_t row = cut.row0 + (cut.r0 + r) / group;
     const int head = cut.kvh * group + (cut.r0 + r) % group;
-    const float inv = l > 0.F ? 1.F / l : 0.F;
+    const float inv = l == 0.F ? 0.F : 1.F / l;
     uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedAttention
         *reinterpret_cast<uint2*>(out + 4 * v) = make_uint2(pack2<DT>(acc[i].x * inv, acc[i].y * inv),
                                                             pack2<DT>(acc[i].z * inv, acc[i].w * inv));
     }
-    if (share == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
+    if (share == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l == 0.F ? -INFINITY : m * kLn2 + logf(l);
 }
 
 }  // namespace kc

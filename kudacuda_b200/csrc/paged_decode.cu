@@ -14,8 +14,10 @@
 //
 // S = Q K^T with exact products and 32-bit sums; softmax in the log2 domain; P
 // is split into two 16-bit halves (P = hi + lo to about twice the type's
-// precision), so P V is as good as with 32-bit probabilities: the tensor cores
-// have time to spare while the cache arrives.
+// precision), so P V is as good as with 32-bit probabilities.  Items of at most
+// 8 rows put lo into the fragment's other 8 rows, whose sum with the first 8 is
+// taken at the end: half of the products, and the tensor cores keep time to
+// spare while the cache arrives.
 #include "kc_common.cuh"
 #include "kc_launch.h"
 #include "kc_tcgen05.cuh"
@@ -30,8 +32,8 @@ constexpr int kRows = 16;
 constexpr int kKeys = 16;
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kOver = 64;             // an item's start and end cost about as much as these keys
-constexpr int kLeast = kKeys * kWarps;  // a worker has a block for every warp
+constexpr int kOver = 384;            // an item's start and end cost about as much as these keys
+constexpr int kLeast = 192;           // a worker has a block or so for every warp
 
 template <int D>
 struct DecodeSmem {
@@ -74,6 +76,13 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+// What the warps need of a piece; thread 0 lists them, kList at a time.
+struct Piece {
+    int b, start, n, len, kvh, r0, rows, limit, t0, t1;
+    int whole;
+};
+constexpr int kList = 12;
+
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads)
     paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -85,7 +94,8 @@ __global__ void __launch_bounds__(kThreads)
     __shared__ __align__(8) uint64_t full[kWarps][M::kStages];
     __shared__ float2 row_ml[kWarps][kRows];  // a warp's (maximum, sum) of a row
     __shared__ int64_t sums[kWarps], place_at;
-    __shared__ int place_seq;
+    __shared__ int place_seq, listed;
+    __shared__ Piece list[kList];
     const PagedBatch& p = a.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* const smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
@@ -99,68 +109,103 @@ __global__ void __launch_bounds__(kThreads)
     pdl_wait_on_producer();
     const int group = p.q_heads / p.kv_heads;
     const int worker = blockIdx.x;
-    int workers = gridDim.x;
-    const int64_t total = paged_place<W, kLeast, kThreads>(p, group, worker, workers, sums, &place_seq, &place_at);
-    // the piece at hand; the piece whose blocks this warp is fetching
-    W w, ahead;
-    w.begin(p, group, paged_bound(total, worker, workers), paged_bound(total, worker + 1, workers), place_seq, place_at);
-    ahead = w;
-    // the stretch's blocks are numbered through; this warp has those with number % kWarps == warp
-    int ahead_j = 0, turn_ahead = 0;
-    bool more;
+    const PagedShares shares =
+        paged_place<W, kLeast, kThreads>(p, group, worker, gridDim.x, sums, &place_seq, &place_at);
+    PagedCut cut;  // (thread 0's)
+    cut.valid = cut.tail = cut.row0 = cut.r0 = cut.rows = cut.kvh = cut.last = cut.pad = 0;
+    W w;  // (thread 0's)
+    if (tid == 0) w.begin(p, group, shares, worker, place_seq, place_at);
+    bool ok = true;
+    uint32_t fetched = 0, used = 0;
+    for (;;) {
+    // ---- the next pieces of the stretch
+    if (tid == 0) {
+        int n = 0;
+        while (n < kList && w.next(p, group)) {
+            Piece& e = list[n++];
+            e.b = w.piece_b;
+            e.start = w.piece_start;
+            e.n = w.piece_n;
+            e.len = w.piece_len;
+            e.kvh = w.kvh;
+            e.r0 = w.q * kRows;
+            e.rows = w.item_rows;
+            e.limit = w.limit;
+            e.t0 = w.t0;
+            e.t1 = w.t1;
+            e.whole = w.whole() ? 1 : 0;
+            if (w.t0 > 0) {
+                cut.tail = 1;
+            } else if (!w.whole()) {
+                cut.valid = 1;
+                cut.row0 = w.piece_start;
+                cut.r0 = w.q * kRows;
+                cut.rows = w.item_rows;
+                cut.kvh = w.kvh;
+                cut.last = shares.of(w.item_end - 1);
+            }
+            if (w.piece_len > p.table_width * p.page_size && p.err != nullptr) atomicOr(p.err, 2);
+        }
+        listed = n;
+    }
+    __syncthreads();
+    const int pieces = listed;
+    if (pieces == 0) break;
+    // the pieces' blocks are numbered through; this warp has those with number % kWarps == warp
+    int ahead = -1, ahead_j = 0, ahead_t1 = 0, turn_ahead = 0;  // the block to be fetched next
     // the next piece with a block of this warp: its queries come into L1 while the blocks before it are worked on
     auto step = [&]() {
-        while ((more = ahead.next(p, group))) {
-            ahead_j = ahead.t0 + ((warp - turn_ahead) & (kWarps - 1));
-            turn_ahead += ahead.t1 - ahead.t0;
-            if (ahead_j < ahead.t1) break;
+        while (++ahead < pieces) {
+            const int t0 = list[ahead].t0;
+            ahead_t1 = list[ahead].t1;
+            ahead_j = t0 + ((warp - turn_ahead) & (kWarps - 1));
+            turn_ahead += ahead_t1 - t0;
+            if (ahead_j < ahead_t1) break;
         }
+        if (ahead >= pieces) return;
+        const Piece& e = list[ahead];
         const int r = lane & 15;
-        if (more && r < ahead.item_rows) {
-            const int token = (ahead.q * kRows + r) / group, head = (ahead.q * kRows + r) % group;
-            const uint16_t* q = static_cast<const uint16_t*>(a.q) + (ahead.piece_start + token) * a.q_stride +
-                                static_cast<int64_t>(ahead.kvh * group + head) * D + (lane >> 4) * (D / 2);
+        if (r < e.rows) {
+            const int token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
+            const uint16_t* q = static_cast<const uint16_t*>(a.q) + (e.start + token) * a.q_stride +
+                                static_cast<int64_t>(e.kvh * group + head) * D + (lane >> 4) * (D / 2);
             asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
         }
     };
-    step();
-    uint32_t fetched = 0, used = 0;
-
     // fetch the next block, K and V, into its stage (which its reader has left)
     auto fetch = [&]() {
-        if (!more) return;
+        if (ahead < 0 || ahead_j >= ahead_t1) step();
+        if (ahead >= pieces) return;
+        const Piece& e = list[ahead];
         const int key0 = ahead_j * kKeys;
-        const bool some = key0 < ahead.limit;  // (an item without keys has one block without)
+        const bool some = key0 < e.limit;  // (an item without keys has one block without)
         const uint32_t s = fetched % M::kStages;
         uint8_t* const stage = ring + s * 2 * M::kBlock;
         if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], some ? 2 * M::kBlock : 0);
         __syncwarp();
         if (some && lane < 2 * M::kHalves) {
             const int half = lane >> 1, v = lane & 1;
-            const int page = p.table[ahead.piece_b * p.table_stride + key0 / p.page_size];
+            const int page = p.table[e.b * p.table_stride + key0 / p.page_size];
             int row = -kKeys;  // a missing page reads as zeros: a box that begins before the tensor
             if (page >= 0 && page < p.num_pages)
-                row = (page * p.kv_heads + ahead.kvh) * p.page_size + key0 % p.page_size;
+                row = (page * p.kv_heads + e.kvh) * p.page_size + (key0 & (p.page_size - 1));
             else if (p.err != nullptr) atomicOr(p.err, 2);
             tma_load_2d(stage + v * M::kBlock + half * (kKeys * 128), v ? &map_v : &map_k, half * 64, row,
                         &full[warp][s]);
         }
         ++fetched;
         ahead_j += kWarps;
-        if (ahead_j >= ahead.t1) step();
     };
-    for (int i = 0; i < M::kStages - 1; ++i) fetch();
 
     const float c = a.scale * kLog2E;
     const int g = lane >> 2, t4 = lane & 3;  // an accumulator's rows g and g + 8, columns 2 t4 and 2 t4 + 1
-    PagedCut cut;
-    cut.valid = cut.tail = cut.row0 = cut.r0 = cut.rows = cut.kvh = cut.last = cut.pad = 0;
-    bool ok = true;
     int turn = 0;
-    while (w.next(p, group)) {
-        if (w.piece_len > p.table_width * p.page_size && tid == 0 && p.err != nullptr) atomicOr(p.err, 2);
-        const int first = w.t0 + ((warp - turn) & (kWarps - 1));
-        turn += w.t1 - w.t0;
+#pragma unroll 1
+    for (int piece = 0; piece < pieces; ++piece) {
+        const Piece e = list[piece];
+        const bool narrow = e.rows <= 8;
+        const int first = e.t0 + ((warp - turn) & (kWarps - 1));
+        turn += e.t1 - e.t0;
         float o[D / 8][4];
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.F;
@@ -168,22 +213,25 @@ __global__ void __launch_bounds__(kThreads)
         // Q: the A fragments of the item's 16 rows, straight from memory
         uint32_t qf[D / 16][4];
         int row_keys[2] = {0, 0};
-        if (first < w.t1) {
+        if (first < e.t1) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int r = g + 8 * h, token = (w.q * kRows + r) / group, head = (w.q * kRows + r) % group;
-                const bool live = r < w.item_rows;
+                const int r = g + 8 * h, token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
+                const bool live = r < e.rows;
                 const uint16_t* q = static_cast<const uint16_t*>(a.q) +
-                                    (live ? (w.piece_start + token) * a.q_stride + static_cast<int64_t>(w.kvh * group + head) * D : 0);
+                                    (live ? (e.start + token) * a.q_stride + static_cast<int64_t>(e.kvh * group + head) * D : 0);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        qf[k][2 * e + h] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 * e + 2 * t4) : 0u;
-                row_keys[h] = live ? min(max(w.piece_len - w.piece_n + token + 1, 0), w.limit) : 0;
+                    for (int x = 0; x < 2; ++x)
+                        qf[k][2 * x + h] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 * x + 2 * t4) : 0u;
+                row_keys[h] = live ? min(max(e.len - e.n + token + 1, 0), e.limit) : 0;
             }
         }
-        for (int j = first; j < w.t1; j += kWarps) {
+        // (the first blocks are on their way while the queries come)
+        for (; piece == 0 && fetched - used < M::kStages - 1 && ahead < pieces;) fetch();
+#pragma unroll 1
+        for (int j = first; j < e.t1; j += kWarps) {
             fetch();
             const uint32_t s = used % M::kStages;
             ok = ok && mbar_wait_bounded(&full[warp][s], (used / M::kStages) & 1);
@@ -194,9 +242,11 @@ __global__ void __launch_bounds__(kThreads)
             }
             const uint32_t kb = smem_u32(ring + s * 2 * M::kBlock), vb = kb + M::kBlock;
             // S: 16 rows x 32 keys, four tiles of 8 keys
-            float sc[kKeys / 8][4];
+            float sc[kKeys / 8][4], sc2[kKeys / 8][4];  // even and odd steps of 16 dims: two chains
 #pragma unroll
-            for (int n = 0; n < kKeys / 8; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.F;
+            for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[n][i] = sc2[n][i] = 0.F;
 #pragma unroll
             for (int n2 = 0; n2 < kKeys / 16; ++n2) {
                 // ldmatrix: keys 16 n2 .. + 15 (two tiles), 16 dims (two 8-dim words)
@@ -207,21 +257,21 @@ __global__ void __launch_bounds__(kThreads)
                     const int word = 2 * (k & 3) + ((lane >> 3) & 1);
                     uint32_t b[4];
                     ldsm4(b, row + (k >> 2) * (kKeys * 128) + ((word ^ (key & 7)) << 4));
-                    mma16816<DT>(sc[2 * n2], qf[k], b[0], b[1]);
-                    mma16816<DT>(sc[2 * n2 + 1], qf[k], b[2], b[3]);
+                    mma16816<DT>(k & 1 ? sc2[2 * n2] : sc[2 * n2], qf[k], b[0], b[1]);
+                    mma16816<DT>(k & 1 ? sc2[2 * n2 + 1] : sc[2 * n2 + 1], qf[k], b[2], b[3]);
                 }
             }
             const int key0 = j * kKeys;
-            const int valid = w.limit - key0;  // keys of the block that exist
+            const int valid = e.limit - key0;  // keys of the block that exist
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = key0 + 8 * n + 2 * t4 + (e & 1);
-                    const float x = key < row_keys[e >> 1] ? sc[n][e] * c : -INFINITY;
-                    sc[n][e] = x;
-                    top[e >> 1] = fmaxf(top[e >> 1], x);
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 8 * n + 2 * t4 + (i & 1);
+                    const float x = key < row_keys[i >> 1] ? (sc[n][i] + sc2[n][i]) * c : -INFINITY;
+                    sc[n][i] = x;
+                    top[i >> 1] = fmaxf(top[i >> 1], x);
                 }
             float f[2];
 #pragma unroll
@@ -233,6 +283,7 @@ __global__ void __launch_bounds__(kThreads)
                 m[h] = mn;
                 l[h] *= f[h];
             }
+            if (narrow) f[1] = f[0];
             if (__any_sync(0xffffffffu, f[0] != 1.F || f[1] != 1.F)) {
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
@@ -242,9 +293,13 @@ __global__ void __launch_bounds__(kThreads)
                     o[i][3] *= f[1];
                 }
             }
+            if (narrow) {
+                m[1] = -INFINITY;  // (rows 8 .. 15 hold the low halves of rows 0 .. 7)
+                l[1] = 0.F;
+            }
             const float sub[2] = {m[0] == -INFINITY ? 0.F : m[0], m[1] == -INFINITY ? 0.F : m[1]};
             // P in A-fragment order, 16 keys a fragment, as hi + lo
-            uint32_t ph[kKeys / 16][4], pl[kKeys / 16][4];
+            uint32_t ph[kKeys / 16][4], pl[kKeys / 16][4];  // (narrow: one fragment of both)
 #pragma unroll
             for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
@@ -253,8 +308,10 @@ __global__ void __launch_bounds__(kThreads)
                     l[h] += e0 + e1;
                     const uint32_t hi = pack2<DT>(e0, e1);
                     const float2 back = unpack2<DT>(hi);
-                    ph[n >> 1][2 * (n & 1) + h] = hi;
-                    pl[n >> 1][2 * (n & 1) + h] = pack2<DT>(e0 - back.x, e1 - back.y);
+                    const uint32_t lo = pack2<DT>(e0 - back.x, e1 - back.y);
+                    if (!narrow || h == 0) ph[n >> 1][2 * (n & 1) + h] = hi;
+                    if (narrow && h == 0) ph[n >> 1][2 * (n & 1) + 1] = lo;
+                    pl[n >> 1][2 * (n & 1) + h] = lo;
                 }
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; ++kk) {
@@ -278,9 +335,11 @@ __global__ void __launch_bounds__(kThreads)
                     b[2] &= keep0;
                     b[3] &= keep1;
                     mma16816<DT>(o[2 * d], ph[kk], b[0], b[1]);
-                    mma16816<DT>(o[2 * d], pl[kk], b[0], b[1]);
                     mma16816<DT>(o[2 * d + 1], ph[kk], b[2], b[3]);
-                    mma16816<DT>(o[2 * d + 1], pl[kk], b[2], b[3]);
+                    if (!narrow) {
+                        mma16816<DT>(o[2 * d], pl[kk], b[0], b[1]);
+                        mma16816<DT>(o[2 * d + 1], pl[kk], b[2], b[3]);
+                    }
                 }
             }
             // this stage is refilled one block from now: every lane has read it (the
@@ -292,6 +351,13 @@ __global__ void __launch_bounds__(kThreads)
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
             if (t4 == 0) row_ml[warp][g + 8 * h] = make_float2(m[h], l[h]);
+        }
+        if (narrow) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] += o[i][2];
+                o[i][1] += o[i][3];
+            }
         }
         // The warps meet: every one brings its accumulator to the row's maximum, the
         // upper four leave theirs, the lower four add one each and leave the sum, and
@@ -325,15 +391,14 @@ __global__ void __launch_bounds__(kThreads)
                 }
         }
         __syncthreads();
-        const bool whole = w.whole();
-        float* const part = Part::slot(a.workspace, gridDim.x, worker, w.t0 > 0 ? 0 : 1);
-        for (int i = tid; i < w.item_rows * (D / 4); i += kThreads) {
+        float* const part = Part::slot(a.workspace, gridDim.x, worker, e.t0 > 0 ? 0 : 1);
+        for (int i = tid; i < e.rows * (D / 4); i += kThreads) {
             const int r = i / (D / 4), d = 4 * (i % (D / 4));
             float mx = -INFINITY, sum = 0.F;
             for (int v = 0; v < kWarps; ++v) mx = fmaxf(mx, row_ml[v][r].x);
             for (int v = 0; v < kWarps; ++v) {
                 const float2 x = row_ml[v][r];
-                if (x.x != -INFINITY) sum += x.y * ex2(x.x - mx);
+                sum += x.y * (x.x == -INFINITY ? 0.F : ex2(x.x - mx));
             }
             const float* at = meet + r * D + ((((d >> 3) ^ (r & 7)) << 3) | (d & 7));
             float4 x = *reinterpret_cast<const float4*>(at);
@@ -345,31 +410,24 @@ __global__ void __launch_bounds__(kThreads)
                 x.z += y.z;
                 x.w += y.w;
             }
-            if (whole) {
-                const int64_t row = w.piece_start + (w.q * kRows + r) / group;
-                const int head = w.kvh * group + (w.q * kRows + r) % group;
-                const float inv = sum > 0.F ? 1.F / sum : 0.F;
+            if (e.whole) {
+                const int token = (e.r0 + r) / group;
+                const int64_t row = e.start + token;
+                const int head = e.kvh * group + (e.r0 + r) - token * group;
+                const float inv = sum == 0.F ? 0.F : 1.F / sum;
                 *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.out_stride +
                                           static_cast<int64_t>(head) * D + d) =
                     make_uint2(pack2<DT>(x.x * inv, x.y * inv), pack2<DT>(x.z * inv, x.w * inv));
                 if (d == 0 && a.lse != nullptr)
-                    a.lse[row * p.q_heads + head] = sum > 0.F ? mx * kLn2 + logf(sum) : -INFINITY;
+                    a.lse[row * p.q_heads + head] = sum == 0.F ? -INFINITY : mx * kLn2 + logf(sum);
             } else {
                 if (d == 0) __stcg(reinterpret_cast<float2*>(part) + r, make_float2(mx, sum));
                 __stcg(reinterpret_cast<float4*>(part + 2 * kRows + r * D + d), x);
             }
         }
-        if (!whole && w.t0 > 0) {
-            cut.tail = 1;
-        } else if (!whole) {
-            cut.valid = 1;
-            cut.row0 = w.piece_start;
-            cut.r0 = w.q * kRows;
-            cut.rows = w.item_rows;
-            cut.kvh = w.kvh;
-            cut.last = static_cast<int>((w.item_end * workers + total - 1) / total - 1);
-        }
-        __syncthreads();  // `meet` and `row_ml` are free again
+        __syncthreads();  // `meet`, `row_ml` and in the end the list are free again
+    }
+    if (pieces < kList) break;
     }
     if (!ok) {
         if (lane == 0 && p.err != nullptr) atomicOr(p.err, 16);
@@ -428,10 +486,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
         }
         const int64_t row = cut.row0 + (cut.r0 + r) / group;
         const int head = cut.kvh * group + (cut.r0 + r) % group;
-        const float inv = l > 0.F ? 1.F / l : 0.F;
+        const float inv = l == 0.F ? 0.F : 1.F / l;
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D + d) =
             make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
-        if (d == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l > 0.F ? m * kLn2 + logf(l) : -INFINITY;
+        if (d == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l == 0.F ? -INFINITY : m * kLn2 + logf(l);
     }
 }
 

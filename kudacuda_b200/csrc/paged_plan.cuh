@@ -33,14 +33,31 @@ struct PagedCut {
     int pad;
 };
 
-__device__ __forceinline__ int64_t paged_bound(int64_t total, int worker, int workers) {
-    return worker >= workers ? total : total * worker / workers;
+// (almost always both fit 32 bits, whose division is several times as fast)
+__device__ __forceinline__ int64_t paged_div(int64_t x, int64_t y) {
+    if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+    return x / y;
 }
-// No more workers than there is work for: `least` keys a worker.
-__device__ __forceinline__ int paged_workers(int64_t total, int group, int least, int workers) {
-    return static_cast<int>(min(max(total / (static_cast<int64_t>(group) * least), static_cast<int64_t>(1)),
-                                static_cast<int64_t>(workers)));
-}
+// How the line is cut: the first `rest` workers take size + 1, the others size.
+struct PagedShares {
+    int64_t size, rest;
+    int workers;
+    // No more workers than there is work for: about `least` keys a worker.
+    __device__ __forceinline__ void set(int64_t total, int group, int least, int most) {
+        const float w = static_cast<float>(total) / (static_cast<float>(group) * static_cast<float>(least));
+        workers = w < static_cast<float>(most) ? max(static_cast<int>(w), 1) : most;
+        size = paged_div(total, workers);
+        rest = total - size * workers;
+    }
+    __device__ __forceinline__ int64_t from(int worker) const {
+        return size * worker + (worker < rest ? worker : rest);
+    }
+    // the worker whose stretch holds x
+    __device__ __forceinline__ int of(int64_t x) const {
+        const int64_t high = (size + 1) * rest;
+        return static_cast<int>(x < high ? paged_div(x, size + 1) : rest + paged_div(x - high, max(size, int64_t{1})));
+    }
+};
 
 struct PagedSeq {
     int start, n, len;
@@ -90,19 +107,18 @@ struct PagedWalk {
             ++b;
         }
     }
-    // the stretch [from, to), which begins in or after sequence `seq`, whose cost begins at `at`
-    __device__ __forceinline__ void begin(const PagedBatch& p, int group, int64_t from, int64_t to, int seq,
+    // a worker's stretch, which begins in or after sequence `seq`, whose cost begins at `at`
+    __device__ __forceinline__ void begin(const PagedBatch& p, int group, const PagedShares& shares, int worker, int seq,
                                           int64_t at) {
-        x0 = from;
-        x1 = to;
+        x0 = shares.from(worker);
+        x1 = shares.from(worker + 1);
         b = seq;
         head_at = at;
         next_kvh = next_q = 0;
         tiles_q = 0;
         skip_empty(p, group);
         if (b >= p.batch || x0 <= at) return;
-        const int64_t rem = x0 - at;
-        next_kvh = static_cast<int>(min(rem / head_cost, static_cast<int64_t>(p.kv_heads - 1)));
+        next_kvh = static_cast<int>(min(paged_div(x0 - at, head_cost), static_cast<int64_t>(p.kv_heads - 1)));
         head_at = at + next_kvh * head_cost;
         int lo = 0, hi = tiles_q - 1;  // the last tile that begins at or before x0
         while (lo < hi) {
@@ -124,8 +140,10 @@ struct PagedWalk {
             const int last_token = (q * ROWS + item_rows - 1) / group;
             limit = min(max(len - n + last_token + 1, 0), p.table_width * p.page_size);
             tiles = max((limit + KT - 1) / KT, 1);
-            t0 = x0 <= lo ? 0 : static_cast<int>((x0 - lo) * tiles / (hi - lo));
-            t1 = x1 >= hi ? tiles : static_cast<int>((x1 - lo) * tiles / (hi - lo));
+            // (the same expression on both sides of a cut, so the two agree)
+            const float each = static_cast<float>(tiles) / static_cast<float>(hi - lo);
+            t0 = x0 <= lo ? 0 : min(tiles, static_cast<int>(static_cast<float>(x0 - lo) * each));
+            t1 = x1 >= hi ? tiles : min(tiles, static_cast<int>(static_cast<float>(x1 - lo) * each));
             piece_b = b;
             piece_start = start;
             piece_n = n;
@@ -146,13 +164,12 @@ struct PagedWalk {
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
 
-// Block-wide: the total cost, the number of workers that share it (at most
-// `workers`, each with LEAST keys or more), and for worker `mine` the sequence in
-// which its stretch begins (seq) and that sequence's place (at).  `sums` has one
-// word per warp.  Ends with a barrier.
+// Block-wide: how the work is shared (at most `most` workers, each with LEAST keys
+// or more), and for `worker` the sequence in which its stretch begins (seq) and
+// that sequence's place (at).  `sums` has one word per warp.  Ends with a barrier.
 template <class W, int LEAST, int THREADS>
-__device__ __forceinline__ int64_t paged_place(const PagedBatch& p, int group, int worker, int& workers,
-                                               int64_t* sums, int* seq, int64_t* at) {
+__device__ __forceinline__ PagedShares paged_place(const PagedBatch& p, int group, int worker, int most,
+                                                   int64_t* sums, int* seq, int64_t* at) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b0 = static_cast<int>(static_cast<int64_t>(p.batch) * tid / THREADS);
     const int b1 = static_cast<int>(static_cast<int64_t>(p.batch) * (tid + 1) / THREADS);
@@ -180,9 +197,10 @@ __device__ __forceinline__ int64_t paged_place(const PagedBatch& p, int group, i
         total += sums[i];
     }
     int64_t from = before + upto - mine;
-    workers = paged_workers(total, group, LEAST, workers);
-    const int64_t x = paged_bound(total, worker, workers);
-    if (worker < workers && mine > 0 && x >= from && x < from + mine) {
+    PagedShares shares;
+    shares.set(total, group, LEAST, most);
+    const int64_t x = shares.from(worker);
+    if (worker < shares.workers && mine > 0 && x >= from && x < from + mine) {
         int64_t c = from;
         for (w.b = b0; w.b < b1; ++w.b) {
             w.load(p, group);
@@ -194,7 +212,7 @@ __device__ __forceinline__ int64_t paged_place(const PagedBatch& p, int group, i
         *at = c;
     }
     __syncthreads();
-    return total;
+    return shares;
 }
 
 // Where a worker's partial results lie: slot 0 the end of an item begun by an

@@ -195,6 +195,23 @@ def test_attention_flags_a_missing_page_and_spares_the_others(bridge, new):
     assert bridge.error_word(clear=True) == 2
 
 
+@pytest.mark.parametrize("new", [[1, 1], [70, 3]])
+def test_attention_nan_reaches_the_rows_that_attend_it_alone(bridge, new):
+    lens = [200, 150]
+    k, v, table, keys, vals = R.make_cache(lens, 2, 16, 128, BF16, DEV, 65)
+    q = torch.randn((sum(new), 16, 128), generator=torch.Generator().manual_seed(66)).to(BF16).to(DEV)
+    good, good_lse = attend(bridge, q, k, v, table, new, lens)
+    k = k.clone()
+    pos = 180 if new[0] > 1 else 77
+    k[int(table[0, pos // 16]), 1, pos % 16, 5] = math.nan  # a key of the second key head
+    out, lse = attend(bridge, q, k, v, table, new, lens)
+    assert bridge.error_word(clear=True) == 0
+    first = max(0, pos - (lens[0] - new[0]))  # the first row of sequence 0 that attends it
+    assert out[first:new[0], 8:].isnan().all() and lse[first:new[0], 8:].isnan().all()
+    assert torch.equal(out[:, :8], good[:, :8]) and torch.equal(out[:first], good[:first])
+    assert torch.equal(out[new[0]:], good[new[0]:]) and torch.equal(lse[new[0]:], good_lse[new[0]:])
+
+
 def test_attention_no_rows(bridge):
     k, v, table, _, _ = R.make_cache([5], 2, 16, 128, BF16, DEV, 71)
     q = torch.empty((0, 16, 128), dtype=BF16, device=DEV)
