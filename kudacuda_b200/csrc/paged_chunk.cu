@@ -32,6 +32,8 @@ namespace {
 constexpr int kRows = 256;   // query rows of an item
 constexpr int kKeys = 128;   // keys of a block
 constexpr int kThreads = 384;
+constexpr int kOver = 256;   // an item's start and end cost about as much as these keys
+constexpr int kLeast = 128;
 constexpr float kLazy = 8.F;  // how far the true maximum may exceed m
 
 template <int D>
@@ -100,25 +102,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
 }
-// 2^x of a pair on the fma pipes, for some of the keys: 2^x instructions of 16 a
-// clock would need as long for a block as its matrix products.  x = n + f with n
-// whole (adding 1.5 2^23 rounds it into the low mantissa bits) and |f| <= 1/2; 2^f by a
-// polynomial of degree 4, fitted to the least relative error (2.7e-6); n is added
-// to the exponent.  x is at most a few; below -126 it counts as -126.
-__device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
-    const uint64_t magic = pair(12582912.F, 12582912.F), minus = pair(-12582912.F, -12582912.F);
-    x = pair(fmaxf(low(x), -126.F), fmaxf(high(x), -126.F));
-    const uint64_t n = add2(x, magic);
-    const uint64_t f = fma2(add2(n, minus), pair(-1.F, -1.F), x);
-    uint64_t p = fma2(f, pair(0.009570102207362652F, 0.009570102207362652F), pair(0.05591785907745361F, 0.05591785907745361F));
-    p = fma2(p, f, pair(0.240247443318367F, 0.240247443318367F));
-    p = fma2(p, f, pair(0.6931217908859253F, 0.6931217908859253F));
-    p = fma2(p, f, pair(0.9999992847442627F, 0.9999992847442627F));
-    return pair(__int_as_float(__float_as_int(low(p)) + (__float_as_int(low(n)) << 23)),
-                __int_as_float(__float_as_int(high(p)) + (__float_as_int(high(n)) << 23)));
-}
-constexpr uint32_t kByPoly = 0x52;  // which of eight pairs go by the polynomial (three)
-
 // the item's last block has rows without a key
 __device__ __forceinline__ bool has_tail(int limit) { return limit % kKeys != 0 || limit == 0; }
 
@@ -134,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_q, const PagedAttentionArgs a, int q_by_tma) {
     using M = ChunkSmem<D>;
-    using W = PagedWalk<kRows, kKeys, kKeys>;
+    using W = PagedWalk<kRows, kKeys, kOver>;
     using Part = PagedPartial<kRows, D>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) ChunkBars bars;
@@ -143,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ int64_t sums[kThreads / 32], place_at;
     __shared__ int place_seq;
     const PagedBatch& p = a.p;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     uint8_t* const base = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
     uint8_t* const qs = base;
     uint8_t* const ring = base + 2 * M::kTile;
@@ -175,16 +158,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int group = p.q_heads / p.kv_heads;
     const int worker = blockIdx.x;
     const PagedShares shares =
-        paged_place<W, kKeys, kThreads>(p, group, worker, gridDim.x, sums, &place_seq, &place_at);
+        paged_place<W, kLeast, kThreads>(p, group, worker, gridDim.x, sums, &place_seq, &place_at);
     tc_fence_after();
     pdl_launch_dependents();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     volatile int* const abort_p = &abort_flag;
     W w;
     w.begin(p, group, shares, worker, place_seq, place_at);
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) {
             // ---- K/V producer: K_0, V_0, K_1, V_1, ... of every piece through the ring
             uint32_t seq = 0, tail_use = 0, tail_parity = 0;  // per stage: its last copy was a tail, tails so far
@@ -229,15 +212,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else bar_wait(&bars.kv_full[s], (i / M::kStages) & 1, abort_p, false);
             }
         } else if (warp == 9) {
-            // ---- MMA issuer
-            if (lane == 0) {
+            // ---- MMA issuer: the warp runs converged, lane 0 issues
+            {
+                const uint32_t lead = lane == 0 ? 1u : 0u;
                 constexpr uint32_t kIdescS = umma_idesc(DT == kBF16, 128, 128, false);
                 constexpr uint32_t kIdescO = umma_idesc(DT == kBF16, 128, D, true);
                 uint32_t seq = 0, items = 0, np[2] = {0, 0};
                 const uint32_t q_addr = smem_u32(qs), r_addr = smem_u32(ring);
-                while (w.next(p, group)) {
-                    const int active = w.item_rows > 128 ? 2 : 1;
-                    const int n = w.t1 - w.t0;
+                while (__shfl_sync(0xffffffffu, w.next(p, group) ? 1 : 0, 0)) {
+                    const int active = __shfl_sync(0xffffffffu, w.item_rows > 128 ? 2 : 1, 0);
+                    const int n = __shfl_sync(0xffffffffu, w.t1 - w.t0, 0);
                     bar_wait(&bars.q_full, items & 1, abort_p);
                     for (int j = 0; j <= n; ++j) {
                         // O_t += P_t(j - 1) V(j - 1), then S_t = Q_t K(j)^T over P_t(j - 1)'s
@@ -257,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     tc_fence_after();
 #pragma unroll
                                     for (int k = h * (kKeys / 32); k < (h + 1) * (kKeys / 32); ++k)
-                                        umma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
+                                        umma_bf16_ts_warp(lead, tmem + 256 + t * D, tmem + t * 128 + 8 * k,
                                                      umma_desc_sw128_mn(va + 2048 * k, 128 * 128), kIdescO,
                                                      (j > 1 || k > 0) ? 1u : 0u);
                                 }
@@ -267,17 +251,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                                 for (int k = 0; k < D / 16; ++k) {
                                     const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-                                    umma_bf16(tmem + t * 128, umma_desc_sw128(q_addr + t * M::kTile + off),
+                                    umma_bf16_warp(lead, tmem + t * 128, umma_desc_sw128(q_addr + t * M::kTile + off),
                                               umma_desc_sw128(ka + off), kIdescS, k > 0 ? 1u : 0u);
                                 }
-                                umma_commit(&bars.s_full[t]);
+                                umma_commit_warp(lead, &bars.s_full[t]);
                             } else {
-                                umma_commit(&bars.o_done[t]);
+                                umma_commit_warp(lead, &bars.o_done[t]);
                             }
                             if (t == active - 1) {
-                                if (j > 0) umma_commit(&bars.kv_empty[sv % M::kStages]);
-                                if (j < n) umma_commit(&bars.kv_empty[sk % M::kStages]);
-                                if (j == n - 1) umma_commit(&bars.q_empty);
+                                if (j > 0) umma_commit_warp(lead, &bars.kv_empty[sv % M::kStages]);
+                                if (j < n) umma_commit_warp(lead, &bars.kv_empty[sk % M::kStages]);
+                                if (j == n - 1) umma_commit_warp(lead, &bars.q_empty);
                             }
                         }
                     }
@@ -342,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ---- softmax: thread = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = warp >> 2;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
@@ -364,8 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < kKeys; i += 32) tmem_ld32(ts + i, s + i);
                 tmem_wait_ld();
                 const int keys = row_keys - j * kKeys;
-                const bool masked = __any_sync(0xffffffffu, keys < kKeys);
-                if (masked) {
+                if (__any_sync(0xffffffffu, keys < kKeys)) {
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i) s[i] = i < keys ? s[i] : -INFINITY;
                 }
@@ -402,22 +385,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t pk[32];
-                    if (masked) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const uint64_t x = fma2(pair(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), c2, sub2);
-                            const uint64_t e = pair(ex2(low(x)), ex2(high(x)));
-                            sum2[i & 1] = add2(sum2[i & 1], e);
-                            pk[i] = pack2<DT>(low(e), high(e));
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const uint64_t x = fma2(pair(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), c2, sub2);
-                            const uint64_t e = kByPoly >> (i & 7) & 1 ? ex2_poly(x) : pair(ex2(low(x)), ex2(high(x)));
-                            sum2[i & 1] = add2(sum2[i & 1], e);
-                            pk[i] = pack2<DT>(low(e), high(e));
-                        }
+                    for (int i = 0; i < 32; ++i) {
+                        const uint64_t x = fma2(pair(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), c2, sub2);
+                        const uint64_t e = pair(ex2(low(x)), ex2(high(x)));
+                        sum2[i & 1] = add2(sum2[i & 1], e);
+                        pk[i] = pack2<DT>(low(e), high(e));
                     }
                     tmem_st32(ts + 32 * h, pk);
                     tmem_wait_st();
