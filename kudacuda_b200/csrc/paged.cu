@@ -51,11 +51,13 @@ __device__ __forceinline__ uint4 pack8(const float* x) {
 // A warp owns one token: its lanes split a head into units of 16 elements
 // (two 16-byte words: eight pairs of a rotated unit, or 16 elements that pass
 // through), 32 / (head_dim / 16) heads abreast, and walk `iters` such groups
-// of heads with the unit's eight cos and sin in registers.
+// of heads with the unit's eight cos and sin in registers, all their loads in flight
+// at once.
 constexpr int kRopeThreads = 128;
+constexpr int64_t kRopeWarps = 16384;  // warps that fill the SMs twice over
 
-template <int DT>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeAppendArgs a, int iters, int groups) {
+template <int DT, int ITERS>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeAppendArgs a, int groups) {
     pdl_launch_dependents();
     pdl_wait_on_producer();
     const PagedBatch& p = a.p;
@@ -103,12 +105,20 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeApp
     const int heads = p.q_heads + 2 * p.kv_heads;
     const int64_t slot = static_cast<int64_t>(pos & (p.page_size - 1)) * p.head_dim;
     const int64_t head_elems = static_cast<int64_t>(p.page_size) * p.head_dim;
-    for (int it = 0; it < iters; ++it) {
-        const int h = (group * iters + it) * abreast + hslot;
+    uint4 in0[ITERS], in1[ITERS];
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        const int h = (group * ITERS + it) * abreast + hslot;
+        if (h >= heads) break;
+        in0[it] = __ldcs(reinterpret_cast<const uint4*>(in + h * p.head_dim + o0));
+        in1[it] = __ldcs(reinterpret_cast<const uint4*>(in + h * p.head_dim + o1));
+    }
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        const int h = (group * ITERS + it) * abreast + hslot;
         if (h >= heads) break;
         const int64_t off = static_cast<int64_t>(h) * p.head_dim;
-        uint4 v0 = *reinterpret_cast<const uint4*>(in + off + o0);
-        uint4 v1 = *reinterpret_cast<const uint4*>(in + off + o1);
+        uint4 v0 = in0[it], v1 = in1[it];
         const bool rotate = turned && h < p.q_heads + p.kv_heads;
         if (rotate || a.bias != nullptr) {
             float x[16];
@@ -212,12 +222,16 @@ cudaError_t rope_append_paged(const RopeAppendArgs& a, int dt, cudaStream_t s) {
     if (a.p.rows == 0 || a.p.batch == 0) return cudaSuccess;
     const int abreast = 32 / (a.p.head_dim / 16);
     const int need = (a.p.q_heads + 2 * a.p.kv_heads + abreast - 1) / abreast;
-    const int iters = 1, groups = (need + iters - 1) / iters;
+    // many rows: four groups of heads a warp share the table's row and the lookup;
+    // few: a warp for every group, for the shortest chain
+    const int iters = static_cast<int64_t>(a.p.rows) * need >= kRopeWarps ? 4 : 1;
+    const int groups = (need + iters - 1) / iters;
     const int64_t warps = static_cast<int64_t>(a.p.rows) * groups;
     const int64_t blocks = (warps + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-    return launch_pdl(dt == kBF16 ? rope_append_kernel<kBF16> : rope_append_kernel<kF16>,
-                      dim3(static_cast<unsigned>(blocks)), dim3(kRopeThreads), 0, s, a, iters, groups);
+    auto kernel = dt == kBF16 ? (iters == 4 ? rope_append_kernel<kBF16, 4> : rope_append_kernel<kBF16, 1>)
+                              : (iters == 4 ? rope_append_kernel<kF16, 4> : rope_append_kernel<kF16, 1>);
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRopeThreads), 0, s, a, groups);
 }
 
 cudaError_t kv_pages_copy(const PagesCopyArgs& a, cudaStream_t s) {
