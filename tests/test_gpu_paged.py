@@ -444,6 +444,29 @@ def test_sample_ties_infinities_and_nan(bridge, dtype):
     check_rows(bridge, torch.tensor(rows, dtype=torch.float64).to(dtype).to(DEV), us, *cols)
 
 
+def test_sample_values_of_every_size(bridge):
+    """bf16 values that few entries share, near 0, past 128 and far below, beside ordinary ones."""
+
+    g = torch.Generator().manual_seed(8)
+    rows = []
+    for r in range(24):
+        x = 3.0 * torch.randn((3000,), generator=g)
+        if r % 4 == 1:
+            x[::3] *= 2.0 ** -torch.randint(5, 20, (1000,), generator=g).float()  # near 0, zeros of both signs
+            x[5], x[6] = 0.0, -0.0
+            x = x - 2.0 * (x > 1)
+        if r % 4 == 2:
+            x = x * 40.0
+        if r % 4 == 3:
+            x = x - 140.0
+        rows.append(x)
+    x = torch.stack(rows).to(BF16).to(DEV)
+    u = torch.rand((24,), generator=g).tolist()
+    k = [[0, 7, 0, 2500, 2999, 0][(r // 4) % 6] for r in range(24)]
+    p = [[1.0, 0.9, 0.97, 1.0, 0.99, 0.5][(r // 4) % 6] for r in range(24)]
+    check_rows(bridge, x, u, [[0.8, 30.0][r % 2] for r in range(24)], k, p, [0.0] * 12 + [1e-4] * 12)
+
+
 def test_sample_ends_of_the_uniform_range_and_defaults(bridge):
     x = torch.tensor([[0.0, 1.0, -math.inf, 2.0, -math.inf]] * 4, device=DEV)
     tokens, logp = sample(bridge, x, [0.0, 1.0 - 2.0**-24, 0.5, 5.0])

@@ -1,0 +1,115 @@
+"""GPU tests of serving from the paged cache: steps that mix pieces of prompts and
+single tokens against the batched plan and against themselves cut differently,
+forks, and sampling end to end."""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_decode import norm_close  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def setup():
+    from kudacuda_b200.decode_engine import random_weights, tiny_config
+    from kudacuda_b200.kudacuda_sidecar import KudaCudaBridge
+    from kudacuda_b200.paged_serving import PagedGenerator
+
+    torch.cuda.set_device(0)
+    bridge = KudaCudaBridge(device_id=0)
+    weights = random_weights(bridge, tiny_config(layers=2, vocab=4096), seed=17, device=DEV)
+    gen = PagedGenerator(bridge, weights, num_pages=64, page_size=16, max_position=512, device=DEV)
+    yield bridge, weights, gen
+    bridge.shutdown()
+
+
+def prompt(n, seed):
+    return torch.randint(0, 4096, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def test_a_prompt_in_pieces_gives_what_single_tokens_give(setup):
+    from kudacuda_b200.paged_serving import PagedSequence, Sampling
+
+    _, _, gen = setup
+    ids = prompt(90, 1)
+    greedy = Sampling()
+    finals = []
+    for pieces in ([1] * 90, [64, 26], [7, 40, 1, 42]):
+        seq, at = PagedSequence(), 0
+        for n in pieces:
+            gen.step([(seq, ids[at:at + n])], [greedy], [0.5])
+            at += n
+        finals.append((gen.x[pieces[-1] - 1].float().cpu().numpy(),
+                       gen.cache.k[:, seq.pages[2], :, 3].float().cpu().numpy()))
+        gen.cache.free(seq)
+    for x, k in finals[1:]:
+        norm_close(x, finals[0][0], 2e-2)  # 1e-2 a layer, as everywhere
+        norm_close(k, finals[0][1], 2e-2)
+    assert gen.cache.free_pages == 64
+
+
+def test_paged_steps_agree_with_the_batched_plan(setup):
+    """The same token at the same positions over the same prefix, contiguous and paged caches."""
+
+    from kudacuda_b200.decode_engine import BatchedDecodePlan
+    from kudacuda_b200.paged_serving import PagedSequence, Sampling
+
+    bridge, weights, gen = setup
+    lens = [1, 17, 40]
+    prompts = [prompt(n, 10 + n) for n in lens]
+    seqs = [PagedSequence() for _ in lens]
+    gen.step([(s, p) for s, p in zip(seqs, prompts)], [Sampling()] * 3, [0.0] * 3)
+    ours = [gen.x[sum(lens[:i + 1]) - 1].float().cpu().numpy() for i in range(3)]
+    plan = BatchedDecodePlan(bridge, weights, batch=3, kv_bucket=64, max_tokens=64, device=DEV)
+    stream = torch.cuda.Stream()
+    plan.capture(stream)
+    for t in range(max(lens)):
+        plan.step_tokens([p[min(t, len(p) - 1)] for p in prompts], [min(t, len(p) - 1) for p in prompts], stream)
+    theirs = plan.buffers.x.float().cpu().numpy()
+    bridge.reset_graph()
+    for i in range(3):
+        norm_close(ours[i], theirs[i], 2e-2)
+    for s in seqs:
+        gen.cache.free(s)
+
+
+def test_generate_mixes_prompts_and_forks(setup):
+    from kudacuda_b200.paged_serving import Sampling
+
+    _, _, gen = setup
+    prompts = [prompt(n, 30 + n) for n in (100, 3, 20, 64)]
+    greedy = gen.generate(prompts, 6)
+    assert [len(a) for a in greedy] == [1] * 4 and all(len(a[0]) == 6 for a in greedy)
+    assert gen.cache.free_pages == 64
+    # the same first tokens whatever shares the steps (a near tie may fall either way)
+    alone = [gen.generate([p], 1)[0][0][0] for p in prompts]
+    assert sum(a[0][0] == b for a, b in zip(greedy, alone)) >= 3
+    forked = gen.generate(prompts[2:3], 5, answers=3)[0]
+    assert forked[1] == forked[2] and forked[0][0] == forked[1][0]
+    drawn = gen.generate(prompts[:2], 8, Sampling(temperature=1.5, top_k=200, top_p=0.95, min_p=1e-4), answers=4, seed=3)
+    again = gen.generate(prompts[:2], 8, Sampling(temperature=1.5, top_k=200, top_p=0.95, min_p=1e-4), answers=4, seed=3)
+    assert drawn == again and len({tuple(a) for a in drawn[0]}) == 4
+    assert gen.cache.free_pages == 64
+
+
+def test_step_refuses(setup):
+    from kudacuda_b200.paged_serving import PagedCacheFull, PagedSequence, Sampling
+
+    _, _, gen = setup
+    s = PagedSequence()
+    with pytest.raises(ValueError):
+        gen.step([], [], [])
+    with pytest.raises(ValueError):
+        gen.step([(s, [])], [Sampling()], [0.0])
+    with pytest.raises(ValueError):
+        gen.step([(s, [1] * 65)], [Sampling()], [0.0])
+    with pytest.raises(ValueError):
+        gen.step([(s, [1])], [], [0.0])
+    with pytest.raises(PagedCacheFull):
+        gen.cache.reserve([(s, 64 * 16 + 1)], 0)
+    assert s.length == 0 and gen.cache.free_pages == 64
