@@ -16,7 +16,7 @@
 // Warps: 0-3 and 4-7 softmax, tile 0 and 1; 8 K/V producer (TMA, one box per
 // page and 64 dims, 128-byte swizzle); 9 MMA issuer; 10 fetches Q and clears the
 // rows of the last V block past the item's last key (their P is 0, but 0 times
-// a NaN in an unused slot is not); 11 idle.
+// a NaN in an unused slot is not); 11 only writes the record of this worker's cut items.
 #include <cuda_bf16.h>
 
 #include "kc_common.cuh"
@@ -32,7 +32,7 @@ namespace {
 constexpr int kRows = 256;   // query rows of an item
 constexpr int kKeys = 128;   // keys of a block
 constexpr int kThreads = 384;
-constexpr int kOver = 256;   // an item's start and end cost about as much as these keys
+constexpr int kOver = 384;   // an item's start and end cost about as much as these keys
 constexpr int kLeast = 128;
 constexpr float kLazy = 8.F;  // how far the true maximum may exceed m
 

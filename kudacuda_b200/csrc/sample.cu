@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
 // temperature), which leaves few entries; when at most kList are left, every
 // block gets all of their keys and finishes alone, without the cluster's
 // barriers.  No sort, no atomics on memory.
-constexpr int kPivots = 7;
+constexpr int kPivots = 5;
 constexpr int kMaxCluster = 16;  // more than 8 need the kernel's consent (launch_cluster)
 constexpr int kMaxSampleThreads = 1024;
 constexpr int kList = 1024;
@@ -459,7 +459,11 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
     auto locate = [&](auto by_mass, auto target_of, uint32_t& lo, int64_t& above, int64_t& target) {
         constexpr int N = by_mass ? kSums : kPivots, kCounts = by_mass ? kPivots + 1 : 0;
         if (warp == 0) {
-            const float d[kPivots] = {0.7F, 1.6F, 2.8F, 4.2F, 6.F, 8.5F, 12.F};
+            // Temperatures below the maximum where a nucleus of ordinary logits tends to
+            // end.  Five, spread to 13, over four seeds each (64 rows of 16 bits; 333 of
+            // 32): 81 and 140 us; seven to 12.5: 83 and 144; seven to 12 that start at
+            // 0.7: 84 and 149; three: 81 and 143.
+            const float d[kPivots] = {1.5F, 3.5F, 6.F, 9.F, 13.F};
             float mine_d = d[0];
 #pragma unroll
             for (int i = 1; i < kPivots; ++i)
@@ -558,10 +562,17 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
                     before = sh.from[turn][kCounts + at][lane] - (at > 0 ? sh.from[turn][kCounts + at - 1][lane] : 0);
                 before = warp_sum64(before);
                 __syncwarp();
+                // The next try splits the range evenly: by value while it is wide (by key, a
+                // range about 0 is almost all tiny numbers), by key once it is narrow.
+                const float x_hi = K::value(min(new_hi, top)), x_lo = fmaxf(K::value(new_lo), m - 30.F * t);
+                const float step = (x_hi - x_lo) / (kPivots + 1);
                 const uint64_t span = new_hi - new_lo;
-                if (lane < kPivots)
-                    sh.pv[lane] = max(min(new_hi - static_cast<uint32_t>(span * (lane + 1) / (kPivots + 1)), new_hi - 1),
-                                      new_lo + 1);
+                if (lane < kPivots) {
+                    const uint32_t key = tries < 3 && step > 0.F && step < 1.0e30F
+                                             ? K::near(x_hi - step * (lane + 1))
+                                             : new_hi - static_cast<uint32_t>(span * (lane + 1) / (kPivots + 1));
+                    sh.pv[lane] = max(min(key, new_hi - 1), new_lo + 1);
+                }
                 if (lane == 0) {
                     sh.lo = new_lo;
                     sh.hi = new_hi;
