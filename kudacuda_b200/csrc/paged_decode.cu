@@ -83,8 +83,10 @@ struct Piece {
 };
 constexpr int kList = 12;
 
+// (one block an SM, said aloud, gives the loop 238 registers instead of 175: 64
+// sequences of 500 keys, 4 key heads, take 21.8 us instead of 24.0)
 template <int DT, int D>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                         const PagedAttentionArgs a) {
     using M = DecodeSmem<D>;
@@ -111,385 +113,324 @@ __global__ void __launch_bounds__(kThreads)
     const int worker = blockIdx.x;
     const PagedShares shares =
         paged_place<W, kLeast, kThreads>(p, group, worker, gridDim.x, sums, &place_seq, &place_at);
-    PagedCut cut;  // (thread 0's)
-    cut.valid = cut.tail = cut.row0 = cut.r0 = cut.rows = cut.kvh = cut.last = cut.pad = 0;
     W w;  // (thread 0's)
     if (tid == 0) w.begin(p, group, shares, worker, place_seq, place_at);
+    if (tid == 32) {
+        W v;
+        v.begin(p, group, shares, worker, place_seq, place_at);
+        Part::cuts(a.workspace)[worker] = v.record(p, group, shares, worker);
+    }
     bool ok = true;
     uint32_t fetched = 0, used = 0;
     for (;;) {
-    // ---- the next pieces of the stretch
-    if (tid == 0) {
-        int n = 0;
-        while (n < kList && w.next(p, group)) {
-            Piece& e = list[n++];
-            e.b = w.piece_b;
-            e.start = w.piece_start;
-            e.n = w.piece_n;
-            e.len = w.piece_len;
-            e.kvh = w.kvh;
-            e.r0 = w.q * kRows;
-            e.rows = w.item_rows;
-            e.limit = w.limit;
-            e.t0 = w.t0;
-            e.t1 = w.t1;
-            e.whole = w.whole() ? 1 : 0;
-            if (w.t0 > 0) {
-                cut.tail = 1;
-            } else if (!w.whole()) {
-                cut.valid = 1;
-                cut.row0 = w.piece_start;
-                cut.r0 = w.q * kRows;
-                cut.rows = w.item_rows;
-                cut.kvh = w.kvh;
-                cut.last = shares.of(w.item_end - 1);
+        // ---- the next pieces of the stretch
+        if (tid == 0) {
+            int n = 0;
+            while (n < kList && w.next(p, group)) {
+                Piece& e = list[n++];
+                e.b = w.piece_b;
+                e.start = w.piece_start;
+                e.n = w.piece_n;
+                e.len = w.piece_len;
+                e.kvh = w.kvh;
+                e.r0 = w.q * kRows;
+                e.rows = w.item_rows;
+                e.limit = w.limit;
+                e.t0 = w.t0;
+                e.t1 = w.t1;
+                e.whole = w.whole() ? 1 : 0;
+                if (w.piece_len > p.table_width * p.page_size && p.err != nullptr) atomicOr(p.err, 2);
             }
-            if (w.piece_len > p.table_width * p.page_size && p.err != nullptr) atomicOr(p.err, 2);
+            listed = n;
         }
-        listed = n;
-    }
-    __syncthreads();
-    const int pieces = listed;
-    if (pieces == 0) break;
-    // the pieces' blocks are numbered through; this warp has those with number % kWarps == warp
-    int ahead = -1, ahead_j = 0, ahead_t1 = 0, turn_ahead = 0;  // the block to be fetched next
-    // the next piece with a block of this warp: its queries come into L1 while the blocks before it are worked on
-    auto step = [&]() {
-        while (++ahead < pieces) {
-            const int t0 = list[ahead].t0;
-            ahead_t1 = list[ahead].t1;
-            ahead_j = t0 + ((warp - turn_ahead) & (kWarps - 1));
-            turn_ahead += ahead_t1 - t0;
-            if (ahead_j < ahead_t1) break;
-        }
-        if (ahead >= pieces) return;
-        const Piece& e = list[ahead];
-        const int r = lane & 15;
-        if (r < e.rows) {
-            const int token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
-            const uint16_t* q = static_cast<const uint16_t*>(a.q) + (e.start + token) * a.q_stride +
-                                static_cast<int64_t>(e.kvh * group + head) * D + (lane >> 4) * (D / 2);
-            asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
-        }
-    };
-    // fetch the next block, K and V, into its stage (which its reader has left)
-    auto fetch = [&]() {
-        if (ahead < 0 || ahead_j >= ahead_t1) step();
-        if (ahead >= pieces) return;
-        const Piece& e = list[ahead];
-        const int key0 = ahead_j * kKeys;
-        const bool some = key0 < e.limit;  // (an item without keys has one block without)
-        const uint32_t s = fetched % M::kStages;
-        uint8_t* const stage = ring + s * 2 * M::kBlock;
-        if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], some ? 2 * M::kBlock : 0);
-        __syncwarp();
-        if (some && lane < 2 * M::kHalves) {
-            const int half = lane >> 1, v = lane & 1;
-            const int page = p.table[e.b * p.table_stride + key0 / p.page_size];
-            int row = -kKeys;  // a missing page reads as zeros: a box that begins before the tensor
-            if (page >= 0 && page < p.num_pages)
-                row = (page * p.kv_heads + e.kvh) * p.page_size + (key0 & (p.page_size - 1));
-            else if (p.err != nullptr) atomicOr(p.err, 2);
-            tma_load_2d(stage + v * M::kBlock + half * (kKeys * 128), v ? &map_v : &map_k, half * 64, row,
-                        &full[warp][s]);
-        }
-        ++fetched;
-        ahead_j += kWarps;
-    };
+        __syncthreads();
+        const int pieces = listed;
+        if (pieces == 0) break;
+        // the pieces' blocks are numbered through; this warp has those with number % kWarps == warp
+        int ahead = -1, ahead_j = 0, ahead_t1 = 0, turn_ahead = 0;  // the block to be fetched next
+        // the next piece with a block of this warp: its queries come into L1 while the blocks before it are worked on
+        auto step = [&]() {
+            while (++ahead < pieces) {
+                const int t0 = list[ahead].t0;
+                ahead_t1 = list[ahead].t1;
+                ahead_j = t0 + ((warp - turn_ahead) & (kWarps - 1));
+                turn_ahead += ahead_t1 - t0;
+                if (ahead_j < ahead_t1) break;
+            }
+            if (ahead >= pieces) return;
+            const Piece& e = list[ahead];
+            const int r = lane & 15;
+            if (r < e.rows) {
+                const int token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
+                const uint16_t* q = static_cast<const uint16_t*>(a.q) + (e.start + token) * a.q_stride +
+                                    static_cast<int64_t>(e.kvh * group + head) * D + (lane >> 4) * (D / 2);
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
+            }
+        };
+        // fetch the next block, K and V, into its stage (which its reader has left)
+        auto fetch = [&]() {
+            if (ahead < 0 || ahead_j >= ahead_t1) step();
+            if (ahead >= pieces) return;
+            const Piece& e = list[ahead];
+            const int key0 = ahead_j * kKeys;
+            const bool some = key0 < e.limit;  // (an item without keys has one block without)
+            const uint32_t s = fetched % M::kStages;
+            uint8_t* const stage = ring + s * 2 * M::kBlock;
+            if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], some ? 2 * M::kBlock : 0);
+            __syncwarp();
+            if (some && lane < 2 * M::kHalves) {
+                const int half = lane >> 1, v = lane & 1;
+                const int page = p.table[e.b * p.table_stride + key0 / p.page_size];
+                int row = -kKeys;  // a missing page reads as zeros: a box that begins before the tensor
+                if (page >= 0 && page < p.num_pages)
+                    row = (page * p.kv_heads + e.kvh) * p.page_size + (key0 & (p.page_size - 1));
+                else if (p.err != nullptr) atomicOr(p.err, 2);
+                tma_load_2d(stage + v * M::kBlock + half * (kKeys * 128), v ? &map_v : &map_k, half * 64, row,
+                            &full[warp][s]);
+            }
+            ++fetched;
+            ahead_j += kWarps;
+        };
 
-    const float c = a.scale * kLog2E;
-    const int g = lane >> 2, t4 = lane & 3;  // an accumulator's rows g and g + 8, columns 2 t4 and 2 t4 + 1
-    int turn = 0;
+        const float c = a.scale * kLog2E;
+        const int g = lane >> 2, t4 = lane & 3;  // an accumulator's rows g and g + 8, columns 2 t4 and 2 t4 + 1
+        int turn = 0;
 #pragma unroll 1
-    for (int piece = 0; piece < pieces; ++piece) {
-        const Piece e = list[piece];
-        const bool narrow = e.rows <= 8;
-        const int first = e.t0 + ((warp - turn) & (kWarps - 1));
-        turn += e.t1 - e.t0;
-        float o[D / 8][4];
+        for (int piece = 0; piece < pieces; ++piece) {
+            const Piece e = list[piece];
+            const bool narrow = e.rows <= 8;
+            const int first = e.t0 + ((warp - turn) & (kWarps - 1));
+            turn += e.t1 - e.t0;
+            float o[D / 8][4];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.F;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.F, 0.F};
-        // Q: the A fragments of the item's 16 rows, straight from memory
-        uint32_t qf[D / 16][4];
-        int row_keys[2] = {0, 0};
-        if (first < e.t1) {
+            for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.F;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.F, 0.F};
+            // Q: the A fragments of the item's 16 rows, straight from memory
+            uint32_t qf[D / 16][4];
+            int row_keys[2] = {0, 0};
+            if (first < e.t1) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = g + 8 * h, token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
+                    const bool live = r < e.rows;
+                    const uint16_t* q = static_cast<const uint16_t*>(a.q) +
+                                        (live ? (e.start + token) * a.q_stride +
+                                                    static_cast<int64_t>(e.kvh * group + head) * D
+                                              : 0);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            qf[k][2 * x + h] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 * x + 2 * t4) : 0u;
+                    row_keys[h] = live ? min(max(e.len - e.n + token + 1, 0), e.limit) : 0;
+                }
+            }
+            // (the first blocks are on their way while the queries come)
+            for (; piece == 0 && fetched - used < M::kStages - 1 && ahead < pieces;) fetch();
+#pragma unroll 1
+            for (int j = first; j < e.t1; j += kWarps) {
+                fetch();
+                const uint32_t s = used % M::kStages;
+                ok = ok && mbar_wait_bounded(&full[warp][s], (used / M::kStages) & 1);
+                ++used;
+                if (!__all_sync(0xffffffffu, ok)) {  // the piece stays wrong, the error word says so
+                    ok = false;
+                    continue;
+                }
+                const uint32_t kb = smem_u32(ring + s * 2 * M::kBlock), vb = kb + M::kBlock;
+                // S: 16 rows x 32 keys, four tiles of 8 keys
+                float sc[kKeys / 8][4], sc2[kKeys / 8][4];  // even and odd steps of 16 dims: two chains
+#pragma unroll
+                for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[n][i] = sc2[n][i] = 0.F;
+#pragma unroll
+                for (int n2 = 0; n2 < kKeys / 16; ++n2) {
+                    // ldmatrix: keys 16 n2 .. + 15 (two tiles), 16 dims (two 8-dim words)
+                    const int key = 16 * n2 + (lane & 7) + ((lane >> 4) << 3);
+                    const uint32_t row = kb + key * 128;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const int word = 2 * (k & 3) + ((lane >> 3) & 1);
+                        uint32_t b[4];
+                        ldsm4(b, row + (k >> 2) * (kKeys * 128) + ((word ^ (key & 7)) << 4));
+                        mma16816<DT>(k & 1 ? sc2[2 * n2] : sc[2 * n2], qf[k], b[0], b[1]);
+                        mma16816<DT>(k & 1 ? sc2[2 * n2 + 1] : sc[2 * n2 + 1], qf[k], b[2], b[3]);
+                    }
+                }
+                const int key0 = j * kKeys;
+                const int valid = e.limit - key0;  // keys of the block that exist
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + 8 * n + 2 * t4 + (i & 1);
+                        const float x = key < row_keys[i >> 1] ? (sc[n][i] + sc2[n][i]) * c : -INFINITY;
+                        sc[n][i] = x;
+                        top[i >> 1] = fmaxf(top[i >> 1], x);
+                    }
+                float f[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                    const float mn = fmaxf(m[h], top[h]);
+                    f[h] = mn == -INFINITY ? 1.F : ex2(m[h] - mn);
+                    m[h] = mn;
+                    l[h] *= f[h];
+                }
+                if (narrow) f[1] = f[0];
+                if (__any_sync(0xffffffffu, f[0] != 1.F || f[1] != 1.F)) {
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        o[i][0] *= f[0];
+                        o[i][1] *= f[0];
+                        o[i][2] *= f[1];
+                        o[i][3] *= f[1];
+                    }
+                }
+                if (narrow) {
+                    m[1] = -INFINITY;  // (rows 8 .. 15 hold the low halves of rows 0 .. 7)
+                    l[1] = 0.F;
+                }
+                const float sub[2] = {m[0] == -INFINITY ? 0.F : m[0], m[1] == -INFINITY ? 0.F : m[1]};
+                // P in A-fragment order, 16 keys a fragment, as hi + lo
+                uint32_t ph[kKeys / 16][4], pl[kKeys / 16][4];  // (narrow: one fragment of both)
+#pragma unroll
+                for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float e0 = ex2(sc[n][2 * h] - sub[h]), e1 = ex2(sc[n][2 * h + 1] - sub[h]);
+                        l[h] += e0 + e1;
+                        const uint32_t hi = pack2<DT>(e0, e1);
+                        const float2 back = unpack2<DT>(hi);
+                        const uint32_t lo = pack2<DT>(e0 - back.x, e1 - back.y);
+                        if (!narrow || h == 0) ph[n >> 1][2 * (n & 1) + h] = hi;
+                        if (narrow && h == 0) ph[n >> 1][2 * (n & 1) + 1] = lo;
+                        pl[n >> 1][2 * (n & 1) + h] = lo;
+                    }
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk) {
+                    const int key = 16 * kk + (lane & 15);
+                    const uint32_t row = vb + key * 128;
+                    // slots without a key may hold anything, a NaN too: their V must not meet P = 0
+                    const int left = valid - 16 * kk;
+                    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+                    if (left < 16) {
+                        const int k0 = 2 * t4, k1 = 2 * t4 + 8;
+                        keep0 = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
+                        keep1 = (k1 < left ? 0xffffu : 0u) | (k1 + 1 < left ? 0xffff0000u : 0u);
+                    }
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        const int word = 2 * (d & 3) + (lane >> 4);
+                        uint32_t b[4];
+                        ldsm4t(b, row + (d >> 2) * (kKeys * 128) + ((word ^ (key & 7)) << 4));
+                        b[0] &= keep0;
+                        b[1] &= keep1;
+                        b[2] &= keep0;
+                        b[3] &= keep1;
+                        mma16816<DT>(o[2 * d], ph[kk], b[0], b[1]);
+                        mma16816<DT>(o[2 * d + 1], ph[kk], b[2], b[3]);
+                        if (!narrow) {
+                            mma16816<DT>(o[2 * d], pl[kk], b[0], b[1]);
+                            mma16816<DT>(o[2 * d + 1], pl[kk], b[2], b[3]);
+                        }
+                    }
+                }
+                // this stage is refilled one block from now: every lane has read it (the
+                // next fetch() begins with the warp's barrier) before the copy starts
+                __syncwarp();
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int r = g + 8 * h, token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
-                const bool live = r < e.rows;
-                const uint16_t* q = static_cast<const uint16_t*>(a.q) +
-                                    (live ? (e.start + token) * a.q_stride + static_cast<int64_t>(e.kvh * group + head) * D : 0);
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        qf[k][2 * x + h] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 * x + 2 * t4) : 0u;
-                row_keys[h] = live ? min(max(e.len - e.n + token + 1, 0), e.limit) : 0;
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                if (t4 == 0) row_ml[warp][g + 8 * h] = make_float2(m[h], l[h]);
             }
-        }
-        // (the first blocks are on their way while the queries come)
-        for (; piece == 0 && fetched - used < M::kStages - 1 && ahead < pieces;) fetch();
-#pragma unroll 1
-        for (int j = first; j < e.t1; j += kWarps) {
-            fetch();
-            const uint32_t s = used % M::kStages;
-            ok = ok && mbar_wait_bounded(&full[warp][s], (used / M::kStages) & 1);
-            ++used;
-            if (!__all_sync(0xffffffffu, ok)) {  // the piece stays wrong, the error word says so
-                ok = false;
-                continue;
-            }
-            const uint32_t kb = smem_u32(ring + s * 2 * M::kBlock), vb = kb + M::kBlock;
-            // S: 16 rows x 32 keys, four tiles of 8 keys
-            float sc[kKeys / 8][4], sc2[kKeys / 8][4];  // even and odd steps of 16 dims: two chains
+            if (narrow) {
 #pragma unroll
-            for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[n][i] = sc2[n][i] = 0.F;
-#pragma unroll
-            for (int n2 = 0; n2 < kKeys / 16; ++n2) {
-                // ldmatrix: keys 16 n2 .. + 15 (two tiles), 16 dims (two 8-dim words)
-                const int key = 16 * n2 + (lane & 7) + ((lane >> 4) << 3);
-                const uint32_t row = kb + key * 128;
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const int word = 2 * (k & 3) + ((lane >> 3) & 1);
-                    uint32_t b[4];
-                    ldsm4(b, row + (k >> 2) * (kKeys * 128) + ((word ^ (key & 7)) << 4));
-                    mma16816<DT>(k & 1 ? sc2[2 * n2] : sc[2 * n2], qf[k], b[0], b[1]);
-                    mma16816<DT>(k & 1 ? sc2[2 * n2 + 1] : sc[2 * n2 + 1], qf[k], b[2], b[3]);
+                for (int i = 0; i < D / 8; ++i) {
+                    o[i][0] += o[i][2];
+                    o[i][1] += o[i][3];
                 }
             }
-            const int key0 = j * kKeys;
-            const int valid = e.limit - key0;  // keys of the block that exist
-            float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + 8 * n + 2 * t4 + (i & 1);
-                    const float x = key < row_keys[i >> 1] ? (sc[n][i] + sc2[n][i]) * c : -INFINITY;
-                    sc[n][i] = x;
-                    top[i >> 1] = fmaxf(top[i >> 1], x);
-                }
+            // The warps meet: every one brings its accumulator to the row's maximum, the
+            // upper four leave theirs, the lower four add one each and leave the sum, and
+            // all threads add those four.  (columns are swizzled by the row)
+            __syncthreads();
             float f[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                const float mn = fmaxf(m[h], top[h]);
-                f[h] = mn == -INFINITY ? 1.F : ex2(m[h] - mn);
-                m[h] = mn;
-                l[h] *= f[h];
+                float mx = row_ml[0][g + 8 * h].x;
+                for (int i = 1; i < kWarps; ++i) mx = fmaxf(mx, row_ml[i][g + 8 * h].x);
+                f[h] = m[h] == -INFINITY ? 0.F : ex2(m[h] - mx);
             }
-            if (narrow) f[1] = f[0];
-            if (__any_sync(0xffffffffu, f[0] != 1.F || f[1] != 1.F)) {
+            float* const spot = meet + (warp & 3) * kRows * D;
+            auto place = [&](int i, int h) {
+                return reinterpret_cast<float2*>(spot + (g + 8 * h) * D + (8 * (i ^ g) + 2 * t4));
+            };
+            if (warp >= 4) {
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    o[i][0] *= f[0];
-                    o[i][1] *= f[0];
-                    o[i][2] *= f[1];
-                    o[i][3] *= f[1];
-                }
+                for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) *place(i, h) = make_float2(o[i][2 * h] * f[h], o[i][2 * h + 1] * f[h]);
             }
-            if (narrow) {
-                m[1] = -INFINITY;  // (rows 8 .. 15 hold the low halves of rows 0 .. 7)
-                l[1] = 0.F;
-            }
-            const float sub[2] = {m[0] == -INFINITY ? 0.F : m[0], m[1] == -INFINITY ? 0.F : m[1]};
-            // P in A-fragment order, 16 keys a fragment, as hi + lo
-            uint32_t ph[kKeys / 16][4], pl[kKeys / 16][4];  // (narrow: one fragment of both)
+            __syncthreads();
+            if (warp < 4) {
 #pragma unroll
-            for (int n = 0; n < kKeys / 8; ++n)
+                for (int i = 0; i < D / 8; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float e0 = ex2(sc[n][2 * h] - sub[h]), e1 = ex2(sc[n][2 * h + 1] - sub[h]);
-                    l[h] += e0 + e1;
-                    const uint32_t hi = pack2<DT>(e0, e1);
-                    const float2 back = unpack2<DT>(hi);
-                    const uint32_t lo = pack2<DT>(e0 - back.x, e1 - back.y);
-                    if (!narrow || h == 0) ph[n >> 1][2 * (n & 1) + h] = hi;
-                    if (narrow && h == 0) ph[n >> 1][2 * (n & 1) + 1] = lo;
-                    pl[n >> 1][2 * (n & 1) + h] = lo;
-                }
-#pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk) {
-                const int key = 16 * kk + (lane & 15);
-                const uint32_t row = vb + key * 128;
-                // slots without a key may hold anything, a NaN too: their V must not meet P = 0
-                const int left = valid - 16 * kk;
-                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                if (left < 16) {
-                    const int k0 = 2 * t4, k1 = 2 * t4 + 8;
-                    keep0 = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
-                    keep1 = (k1 < left ? 0xffffu : 0u) | (k1 + 1 < left ? 0xffff0000u : 0u);
-                }
-#pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                    const int word = 2 * (d & 3) + (lane >> 4);
-                    uint32_t b[4];
-                    ldsm4t(b, row + (d >> 2) * (kKeys * 128) + ((word ^ (key & 7)) << 4));
-                    b[0] &= keep0;
-                    b[1] &= keep1;
-                    b[2] &= keep0;
-                    b[3] &= keep1;
-                    mma16816<DT>(o[2 * d], ph[kk], b[0], b[1]);
-                    mma16816<DT>(o[2 * d + 1], ph[kk], b[2], b[3]);
-                    if (!narrow) {
-                        mma16816<DT>(o[2 * d], pl[kk], b[0], b[1]);
-                        mma16816<DT>(o[2 * d + 1], pl[kk], b[2], b[3]);
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 x = *place(i, h);
+                        *place(i, h) = make_float2(o[i][2 * h] * f[h] + x.x, o[i][2 * h + 1] * f[h] + x.y);
                     }
+            }
+            __syncthreads();
+            float* const part = Part::slot(a.workspace, gridDim.x, worker, e.t0 > 0 ? 0 : 1);
+            for (int i = tid; i < e.rows * (D / 4); i += kThreads) {
+                const int r = i / (D / 4), d = 4 * (i % (D / 4));
+                float mx = -INFINITY, sum = 0.F;
+                for (int v = 0; v < kWarps; ++v) mx = fmaxf(mx, row_ml[v][r].x);
+                for (int v = 0; v < kWarps; ++v) {
+                    const float2 x = row_ml[v][r];
+                    sum += x.y * (x.x == -INFINITY ? 0.F : ex2(x.x - mx));
+                }
+                const float* at = meet + r * D + ((((d >> 3) ^ (r & 7)) << 3) | (d & 7));
+                float4 x = *reinterpret_cast<const float4*>(at);
+#pragma unroll
+                for (int v = 1; v < 4; ++v) {
+                    const float4 y = *reinterpret_cast<const float4*>(at + v * kRows * D);
+                    x.x += y.x;
+                    x.y += y.y;
+                    x.z += y.z;
+                    x.w += y.w;
+                }
+                if (e.whole) {
+                    const int token = (e.r0 + r) / group;
+                    const int64_t row = e.start + token;
+                    const int head = e.kvh * group + (e.r0 + r) - token * group;
+                    const float inv = sum == 0.F ? 0.F : 1.F / sum;
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.out_stride +
+                                              static_cast<int64_t>(head) * D + d) =
+                        make_uint2(pack2<DT>(x.x * inv, x.y * inv), pack2<DT>(x.z * inv, x.w * inv));
+                    if (d == 0 && a.lse != nullptr)
+                        a.lse[row * p.q_heads + head] = sum == 0.F ? -INFINITY : mx * kLn2 + logf(sum);
+                } else {
+                    if (d == 0) __stcg(reinterpret_cast<float2*>(part) + r, make_float2(mx, sum));
+                    __stcg(reinterpret_cast<float4*>(part + 2 * kRows + r * D + d), x);
                 }
             }
-            // this stage is refilled one block from now: every lane has read it (the
-            // next fetch() begins with the warp's barrier) before the copy starts
-            __syncwarp();
+            __syncthreads();  // `meet`, `row_ml` and in the end the list are free again
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if (t4 == 0) row_ml[warp][g + 8 * h] = make_float2(m[h], l[h]);
-        }
-        if (narrow) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] += o[i][2];
-                o[i][1] += o[i][3];
-            }
-        }
-        // The warps meet: every one brings its accumulator to the row's maximum, the
-        // upper four leave theirs, the lower four add one each and leave the sum, and
-        // all threads add those four.  (columns are swizzled by the row)
-        __syncthreads();
-        float f[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float mx = row_ml[0][g + 8 * h].x;
-            for (int i = 1; i < kWarps; ++i) mx = fmaxf(mx, row_ml[i][g + 8 * h].x);
-            f[h] = m[h] == -INFINITY ? 0.F : ex2(m[h] - mx);
-        }
-        float* const spot = meet + (warp & 3) * kRows * D;
-        auto place = [&](int i, int h) {
-            return reinterpret_cast<float2*>(spot + (g + 8 * h) * D + (8 * (i ^ g) + 2 * t4));
-        };
-        if (warp >= 4) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) *place(i, h) = make_float2(o[i][2 * h] * f[h], o[i][2 * h + 1] * f[h]);
-        }
-        __syncthreads();
-        if (warp < 4) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float2 x = *place(i, h);
-                    *place(i, h) = make_float2(o[i][2 * h] * f[h] + x.x, o[i][2 * h + 1] * f[h] + x.y);
-                }
-        }
-        __syncthreads();
-        float* const part = Part::slot(a.workspace, gridDim.x, worker, e.t0 > 0 ? 0 : 1);
-        for (int i = tid; i < e.rows * (D / 4); i += kThreads) {
-            const int r = i / (D / 4), d = 4 * (i % (D / 4));
-            float mx = -INFINITY, sum = 0.F;
-            for (int v = 0; v < kWarps; ++v) mx = fmaxf(mx, row_ml[v][r].x);
-            for (int v = 0; v < kWarps; ++v) {
-                const float2 x = row_ml[v][r];
-                sum += x.y * (x.x == -INFINITY ? 0.F : ex2(x.x - mx));
-            }
-            const float* at = meet + r * D + ((((d >> 3) ^ (r & 7)) << 3) | (d & 7));
-            float4 x = *reinterpret_cast<const float4*>(at);
-#pragma unroll
-            for (int v = 1; v < 4; ++v) {
-                const float4 y = *reinterpret_cast<const float4*>(at + v * kRows * D);
-                x.x += y.x;
-                x.y += y.y;
-                x.z += y.z;
-                x.w += y.w;
-            }
-            if (e.whole) {
-                const int token = (e.r0 + r) / group;
-                const int64_t row = e.start + token;
-                const int head = e.kvh * group + (e.r0 + r) - token * group;
-                const float inv = sum == 0.F ? 0.F : 1.F / sum;
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.out_stride +
-                                          static_cast<int64_t>(head) * D + d) =
-                    make_uint2(pack2<DT>(x.x * inv, x.y * inv), pack2<DT>(x.z * inv, x.w * inv));
-                if (d == 0 && a.lse != nullptr)
-                    a.lse[row * p.q_heads + head] = sum == 0.F ? -INFINITY : mx * kLn2 + logf(sum);
-            } else {
-                if (d == 0) __stcg(reinterpret_cast<float2*>(part) + r, make_float2(mx, sum));
-                __stcg(reinterpret_cast<float4*>(part + 2 * kRows + r * D + d), x);
-            }
-        }
-        __syncthreads();  // `meet`, `row_ml` and in the end the list are free again
-    }
-    if (pieces < kList) break;
+        if (pieces < kList) break;
     }
     if (!ok) {
         if (lane == 0 && p.err != nullptr) atomicOr(p.err, 16);
         // no copy may still be on its way when the block ends
         for (uint32_t i = fetched > M::kStages ? fetched - M::kStages : 0; i < fetched; ++i)
             mbar_wait_bounded(&full[warp][i % M::kStages], (i / M::kStages) & 1);
-    }
-    if (tid == 0) Part::cuts(a.workspace)[worker] = cut;
-}
-
-// The join of cut items (paged_combine.cuh): a thread takes four dims of a row,
-// four pieces in flight.
-constexpr int kJoinThreads = 256;
-template <int DT, int D>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttentionArgs a) {
-    using Part = PagedPartial<kRows, D>;
-    constexpr int kAhead = 4;
-    pdl_launch_dependents();
-    pdl_wait_on_producer();
-    const int owner = blockIdx.x, workers = gridDim.x;
-    const PagedCut* cuts = Part::cuts(a.workspace);
-    const PagedCut cut = cuts[owner];
-    if (!cut.valid) return;
-    const int last = min(cut.last, workers - 1);
-    const PagedBatch& p = a.p;
-    const int group = p.q_heads / p.kv_heads;
-    for (int i = threadIdx.x; i < cut.rows * (D / 4); i += kJoinThreads) {
-        const int r = i / (D / 4), d = 4 * (i % (D / 4));
-        float m = -INFINITY, l = 0.F;
-        float4 acc = make_float4(0.F, 0.F, 0.F, 0.F);
-        for (int c0 = owner; c0 <= last; c0 += kAhead) {
-            float2 ml[kAhead];
-            float4 x[kAhead];
-            bool there[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                // (read whether it is there or not: one round trip for everything)
-                const int c = min(c0 + u, last);
-                there[u] = c0 + u <= last && (c == owner || cuts[c].tail);
-                const float* part = Part::slot(a.workspace, workers, c, c == owner ? 1 : 0);
-                ml[u] = __ldcg(reinterpret_cast<const float2*>(part) + r);
-                x[u] = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * D + d));
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (!there[u]) continue;
-                const float mn = fmaxf(m, ml[u].x);
-                const float f = m == -INFINITY ? 0.F : ex2(m - mn), g = ml[u].x == -INFINITY ? 0.F : ex2(ml[u].x - mn);
-                l = l * f + ml[u].y * g;
-                acc.x = acc.x * f + x[u].x * g;
-                acc.y = acc.y * f + x[u].y * g;
-                acc.z = acc.z * f + x[u].z * g;
-                acc.w = acc.w * f + x[u].w * g;
-                m = mn;
-            }
-        }
-        const int64_t row = cut.row0 + (cut.r0 + r) / group;
-        const int head = cut.kvh * group + (cut.r0 + r) % group;
-        const float inv = l == 0.F ? 0.F : 1.F / l;
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D + d) =
-            make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
-        if (d == 0 && a.lse != nullptr) a.lse[row * p.q_heads + head] = l == 0.F ? -INFINITY : m * kLn2 + logf(l);
     }
 }
 
@@ -516,7 +457,7 @@ cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     const int blocks = device_sm_count() < kMaxBlocks ? device_sm_count() : kMaxBlocks;
     st = launch_pdl(kernel, dim3(blocks), dim3(kThreads), DecodeSmem<D>::kBytes, s, mk, mv, a);
     if (st != cudaSuccess) return st;
-    return launch_pdl(paged_join_kernel<DT, D>, dim3(blocks), dim3(kJoinThreads), 0, s, a);
+    return launch_pdl(paged_join_kernel<DT, D, kRows, true>, dim3(blocks), dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace

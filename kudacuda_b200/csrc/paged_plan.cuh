@@ -10,7 +10,8 @@
 // that ends inside an item is rounded down to a block, by the same formula for
 // both neighbours, so lengths of any mix load every worker alike and an item
 // is cut only where a stretch ends.  A cut item's pieces are left as partial
-// results (accumulator, maximum, sum) and joined by the combine kernel.
+// results (accumulator, maximum, sum) and joined by a second kernel
+// (paged_combine.cuh).
 //
 // The costs have a closed form per sequence, so a worker finds its place from
 // the lengths alone: no host work and no plan kernel, and the lengths may
@@ -22,14 +23,14 @@
 
 namespace kc {
 
-// one per worker: the cut item that this worker began, for the combine kernel
+// One per worker: the item that goes on from an earlier worker's stretch into this
+// one's, where it is cut (rows 0: there is none).
 struct PagedCut {
-    int valid;      // 1: an item is cut and this worker has its first piece
-    int tail;       // 1: this worker has a piece of an item begun earlier (slot 0)
-    int row0;       // first query row of the item in the batch's rows (token row)
-    int r0, rows;   // first tile row R and the number of rows
+    int first, last;      // the workers that may have a piece of it
+    int piece;            // 1: this worker left one (in its slot 0; the first worker's is in slot 1)
+    int row0;             // first row (token) of the item's sequence in the batch
+    int r0, rows;         // first tile row R and the number of rows
     int kvh;
-    int last;       // last worker that may have a piece of the item
     int pad;
 };
 
@@ -128,22 +129,30 @@ struct PagedWalk {
         }
         next_q = lo;
     }
+    // the item that comes next; its cost begins at the value returned and ends at item_end
+    __device__ __forceinline__ int64_t item(const PagedBatch& p, int group) {
+        const int64_t lo = head_at + cost(group, next_q);
+        item_end = head_at + cost(group, next_q + 1);
+        kvh = next_kvh;
+        q = next_q;
+        item_rows = min(ROWS, rows - q * ROWS);
+        const int last_token = (q * ROWS + item_rows - 1) / group;
+        limit = min(max(len - n + last_token + 1, 0), p.table_width * p.page_size);
+        tiles = max((limit + KT - 1) / KT, 1);
+        return lo;
+    }
+    // the item's block in which x lies (the same expression on both sides of a cut, so the two agree)
+    __device__ __forceinline__ int block_of(int64_t x, int64_t lo) const {
+        const float each = static_cast<float>(tiles) / static_cast<float>(item_end - lo);
+        return x <= lo ? 0 : x >= item_end ? tiles : min(tiles, static_cast<int>(static_cast<float>(x - lo) * each));
+    }
     // the next piece with a block in it
     __device__ __forceinline__ bool next(const PagedBatch& p, int group) {
         while (b < p.batch) {
-            const int64_t lo = head_at + cost(group, next_q), hi = head_at + cost(group, next_q + 1);
-            if (lo >= x1) return false;
-            kvh = next_kvh;
-            q = next_q;
-            item_end = hi;
-            item_rows = min(ROWS, rows - q * ROWS);
-            const int last_token = (q * ROWS + item_rows - 1) / group;
-            limit = min(max(len - n + last_token + 1, 0), p.table_width * p.page_size);
-            tiles = max((limit + KT - 1) / KT, 1);
-            // (the same expression on both sides of a cut, so the two agree)
-            const float each = static_cast<float>(tiles) / static_cast<float>(hi - lo);
-            t0 = x0 <= lo ? 0 : min(tiles, static_cast<int>(static_cast<float>(x0 - lo) * each));
-            t1 = x1 >= hi ? tiles : min(tiles, static_cast<int>(static_cast<float>(x1 - lo) * each));
+            if (head_at + cost(group, next_q) >= x1) return false;
+            const int64_t lo = item(p, group);
+            t0 = block_of(x0, lo);
+            t1 = block_of(x1, lo);
             piece_b = b;
             piece_start = start;
             piece_n = n;
@@ -160,6 +169,25 @@ struct PagedWalk {
             if (t0 < t1) return true;
         }
         return false;
+    }
+    // after begin(): the item that goes on into this worker's stretch
+    __device__ __forceinline__ PagedCut record(const PagedBatch& p, int group, const PagedShares& shares, int worker) {
+        PagedCut c;
+        c.first = c.last = c.piece = c.row0 = c.r0 = c.rows = c.kvh = c.pad = 0;
+        if (b >= p.batch) return c;
+        const int64_t lo = item(p, group);
+        if (x0 <= lo || x0 >= item_end) return c;
+        int first = shares.of(lo);  // (its share may be less than a block)
+        while (first < worker && block_of(shares.from(first + 1), lo) == 0) ++first;
+        if (first == worker || block_of(shares.from(first + 1), lo) == tiles) return c;  // not cut before here
+        c.first = first;
+        c.last = shares.of(item_end - 1);
+        c.piece = block_of(x0, lo) < block_of(x1, lo) ? 1 : 0;
+        c.row0 = start;
+        c.r0 = q * ROWS;
+        c.rows = item_rows;
+        c.kvh = kvh;
+        return c;
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
