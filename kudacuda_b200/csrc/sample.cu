@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
 // barriers.  No sort, no atomics on memory.
 constexpr int kPivots = 5;
 constexpr int kMaxCluster = 16;  // more than 8 need the kernel's consent (launch_cluster)
-constexpr int kMaxSampleThreads = 1024;
+constexpr int kMaxSampleThreads = 512;
 constexpr int kList = 1024;
 
 template <int DT>
@@ -283,11 +283,16 @@ struct SampleShared {
     // the search, kept by warp 0
     uint32_t pv[kPivots], lo, hi;
     int64_t above, target;
-    int listed;          // entries in `list`, or -1
-    int gather, start;   // 1: the list is made next; where this block's entries go in it
+    int listed, start;   // entries of the list that is made next, or -1; where this block's go in it
     int own_count;
-    uint32_t own[kList], list[kList];
+    uint32_t list[kList];
+    // this block's share of the list, then the list's masses; in the end every thread's mass
+    union {
+        uint32_t own[kList];
+        int64_t mass[kList];
+    };
 };
+static_assert(kMaxSampleThreads <= kList);
 
 __device__ __forceinline__ int64_t warp_sum64(int64_t x) {
 #pragma unroll
@@ -354,7 +359,7 @@ __device__ __forceinline__ void split_mass(float w, int& hi, int& lo) {
 __device__ __forceinline__ int64_t join_mass(int hi, int lo) { return (static_cast<int64_t>(hi) << 19) + lo; }
 
 template <int DT>
-__global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(const SampleArgs a) {
     using K = Keys<DT>;
     using Key = typename K::Key;
     constexpr int VE = K::kVec;
@@ -451,6 +456,19 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
             for (int e = 0; e < VE; ++e) f(static_cast<uint32_t>(k[e]));
         }
     };
+    // No mass lies below: exp(-28) 2^38 rounds to none.
+    const uint32_t none = K::near(m - 28.F * t);
+    // Pivot i of n, falling, for the next try in (lo, hi).  They split the range evenly:
+    // by value while it is wide (by key, a range about 0 is almost all tiny
+    // numbers), by key once it is narrow.
+    auto next_pivot = [&](uint32_t lo, uint32_t hi, int tries, int i, int n) {
+        const float x_hi = K::value(min(hi, top)), x_lo = fmaxf(K::value(lo), m - 30.F * t);
+        const float step = (x_hi - x_lo) / (n + 1);
+        const uint64_t span = hi - lo;
+        const uint32_t key = tries < 3 && step > 0.F && step < 1.0e30F ? K::near(x_hi - step * (i + 1))
+                                                                         : hi - static_cast<uint32_t>(span * (i + 1) / (n + 1));
+        return max(min(key, hi - 1), lo + 1);
+    };
     // The largest key whose entries at or above it reach a target (in number, or
     // in mass): lo reaches it, hi does not.  above: what lies above lo.  The
     // target may depend on the sum over the entries above the first lo, which
@@ -474,14 +492,11 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
                 sh.lo = lo;
                 sh.hi = top + 1;  // nothing lies at or above it
                 sh.above = 0;
-                sh.listed = -1;
-                sh.gather = 0;
             }
         }
         __syncthreads();
         for (int tries = 0;; ++tries) {
             const uint32_t hi = sh.hi;
-            const int listed = sh.listed;
             uint32_t pv[kPivots];  // falling
 #pragma unroll
             for (int i = 0; i < kPivots; ++i) pv[i] = sh.pv[i];
@@ -491,7 +506,7 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
             for (int i = 0; i <= kPivots; ++i) vh[i] = vl[i] = 0;
 #pragma unroll
             for (int i = 0; i < kPivots; ++i) vc[i] = 0;
-            const uint32_t from = by_mass && tries == 0 ? lo + 1 : pv[kPivots - 1];
+            const uint32_t from = by_mass && tries == 0 ? max(lo + 1, none) : pv[kPivots - 1];
             auto take = [&](uint32_t k) {
                 k = k < hi ? k : 0;  // (every pivot is above 0)
                 if constexpr (by_mass) {
@@ -511,11 +526,7 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
                     for (int i = 0; i < kPivots; ++i) vc[i] += k >= pv[i];
                 }
             };
-            if (listed >= 0) {
-                for (int i = tid; i < listed; i += threads) take(sh.list[i]);
-            } else {
-                sweep(from, take);
-            }
+            sweep(from, take);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 int64_t x;
@@ -528,17 +539,13 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
             __syncthreads();
             int64_t x = 0;
             if (warp == 0) x = block_sums(sh, N);
-            if (listed < 0) {
-                turn ^= 1;
-                if (warp == 0) cluster_send(sh, turn, N, x);
-                cluster_barrier();
-                if (warp == 0) {
-                    x = 0;
-                    if (lane < N)
-                        for (uint32_t r = 0; r < ranks; ++r) x += sh.from[turn][lane][r];
-                }
-            }
+            turn ^= 1;
+            if (warp == 0) cluster_send(sh, turn, N, x);
+            cluster_barrier();
             if (warp == 0) {
+                x = 0;
+                if (lane < N)
+                    for (uint32_t r = 0; r < ranks; ++r) x += sh.from[turn][lane][r];
                 if (tries == 0) {
                     const int64_t t0 = target_of(__shfl_sync(0xffffffffu, x, kPivots));
                     if (lane == 0) sh.target = t0;
@@ -556,56 +563,104 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
                 const int64_t number_hi = __shfl_sync(0xffffffffu, x, kCounts + i_hi);
                 const uint32_t new_lo = at < kPivots ? nlo : sh.lo, new_hi = at > 0 ? nhi : hi;
                 const int64_t number = number_lo - (at > 0 ? number_hi : 0);
-                const bool gather = listed < 0 && new_hi - new_lo > 1 && at < kPivots && number <= kList;
+                const bool gather = new_hi - new_lo > 1 && at < kPivots && number <= kList;
                 int64_t before = 0;  // entries of the blocks before this one
                 if (gather && lane < static_cast<int>(rank))
                     before = sh.from[turn][kCounts + at][lane] - (at > 0 ? sh.from[turn][kCounts + at - 1][lane] : 0);
                 before = warp_sum64(before);
                 __syncwarp();
-                // The next try splits the range evenly: by value while it is wide (by key, a
-                // range about 0 is almost all tiny numbers), by key once it is narrow.
-                const float x_hi = K::value(min(new_hi, top)), x_lo = fmaxf(K::value(new_lo), m - 30.F * t);
-                const float step = (x_hi - x_lo) / (kPivots + 1);
-                const uint64_t span = new_hi - new_lo;
-                if (lane < kPivots) {
-                    const uint32_t key = tries < 3 && step > 0.F && step < 1.0e30F
-                                             ? K::near(x_hi - step * (lane + 1))
-                                             : new_hi - static_cast<uint32_t>(span * (lane + 1) / (kPivots + 1));
-                    sh.pv[lane] = max(min(key, new_hi - 1), new_lo + 1);
-                }
+                const uint32_t pivot = next_pivot(new_lo, new_hi, tries, lane, kPivots);
+                if (lane < kPivots) sh.pv[lane] = pivot;
                 if (lane == 0) {
                     sh.lo = new_lo;
                     sh.hi = new_hi;
                     if (at > 0) sh.above += sum_hi;
-                    sh.gather = gather ? 1 : 0;
+                    sh.listed = gather ? static_cast<int>(number) : -1;
                     sh.start = static_cast<int>(before);
                     sh.own_count = 0;
-                    if (gather) sh.listed = static_cast<int>(number);
                 }
             }
             __syncthreads();
-            if (sh.gather) {
-                // the keys in [lo, hi) of every block to every block
-                const uint32_t g_lo = sh.lo, g_hi = sh.hi;
-                sweep(g_lo, [&](uint32_t k) {
-                    if (k >= g_lo && k < g_hi) sh.own[atomicAdd(&sh.own_count, 1)] = k;
-                });
-                __syncthreads();
-                const int own = sh.own_count, start = sh.start;
-                for (int i = tid; i < own * static_cast<int>(ranks); i += threads) {
-                    const int r = i / own, j = i - r * own;
-                    store_remote32(&sh.list[start + j], r, sh.own[j]);
-                }
-                cluster_barrier();
-            }
-            if (sh.hi - sh.lo <= 1) break;
+            if (sh.listed >= 0 || sh.hi - sh.lo <= 1) break;
         }
+        uint32_t hi = sh.hi;
+        const int listed = sh.listed;
         lo = sh.lo;
         above = sh.above;
         target = sh.target;
-        const bool listed = sh.listed >= 0;
+        if (listed >= 0) {
+            // the keys in [lo, hi) of every block to every block
+            sweep(lo, [&](uint32_t k) {
+                if (k >= lo && k < hi) sh.own[atomicAdd(&sh.own_count, 1)] = k;
+            });
+            __syncthreads();
+            const int own = sh.own_count, start = sh.start;
+            for (int i = tid; i < own * static_cast<int>(ranks); i += threads) {
+                const int r = i / own, j = i - r * own;
+                store_remote32(&sh.list[start + j], r, sh.own[j]);
+            }
+            cluster_barrier();
+            if constexpr (by_mass) {
+                for (int i = tid; i < listed; i += threads) sh.mass[i] = mass(sh.list[i]);
+                __syncthreads();
+            }
+            // From here every block finishes alone: a warp tries two keys a round and
+            // all warps read all sums (two halves of sh.warp in turn, so that a
+            // round has one barrier).
+            const int pivots = 2 * (threads >> 5);
+            int inside = listed;  // entries in [lo, hi)
+            for (int tries = 0; hi - lo > 1; ++tries) {
+                const uint32_t p0 = next_pivot(lo, hi, tries, 2 * warp, pivots);
+                const uint32_t p1 = next_pivot(lo, hi, tries, 2 * warp + 1, pivots);
+                int64_t m0 = 0, m1 = 0;
+                int c0 = 0, c1 = 0;
+                for (int i = lane; i < listed; i += 32) {
+                    const uint32_t k = sh.list[i];
+                    const bool in0 = k < hi && k >= p0, in1 = k < hi && k >= p1;
+                    c0 += in0;
+                    c1 += in1;
+                    if constexpr (by_mass) {
+                        const int64_t w = sh.mass[i];
+                        m0 += in0 ? w : 0;
+                        m1 += in1 ? w : 0;
+                    }
+                }
+                c0 = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c0)));
+                c1 = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c1)));
+                if constexpr (by_mass) {
+                    m0 = warp_sum48(m0);
+                    m1 = warp_sum48(m1);
+                }
+                int64_t* const sums = sh.warp[2 * (tries & 1)];
+                int64_t* const counts = sh.warp[2 * (tries & 1) + 1];
+                if (lane == 0) {
+                    counts[2 * warp] = c0;
+                    counts[2 * warp + 1] = c1;
+                    sums[2 * warp] = by_mass ? m0 : c0;
+                    sums[2 * warp + 1] = by_mass ? m1 : c1;
+                }
+                __syncthreads();
+                const int64_t x = lane < pivots ? sums[lane] : 0;
+                const unsigned reach = __ballot_sync(0xffffffffu, lane < pivots && above + x >= target);
+                const int at = reach != 0 ? __ffs(reach) - 1 : pivots;
+                if (at < pivots) inside = static_cast<int>(counts[at]);
+                const uint32_t was_lo = lo, was_hi = hi;
+                if (at < pivots) lo = next_pivot(was_lo, was_hi, tries, at, pivots);
+                if (at > 0) {
+                    hi = next_pivot(was_lo, was_hi, tries, at - 1, pivots);
+                    above += sums[at - 1];
+                    inside -= static_cast<int>(counts[at - 1]);
+                }
+                if (inside == 1) {  // the one entry left is it
+                    uint32_t k = 0;
+                    for (int i = lane; i < listed; i += 32)
+                        if (sh.list[i] < hi) k = max(k, sh.list[i]);
+                    lo = __reduce_max_sync(0xffffffffu, k);
+                    break;
+                }
+            }
+        }
         __syncthreads();
-        if (listed) cluster_barrier();  // the list may be written again
     };
     // kept: key > cut, and the first `ties` (by index) of the entries with key == cut
     uint32_t cut = 0;  // below every entry: all are kept
@@ -638,15 +693,17 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
     }
     float low = a.min_p != nullptr ? a.min_p[row] : 0.F;
     low = low > 1.F ? 1.F : low;
-    // Index order from here.  A warp's entries are a run of words; it sums what it
-    // keeps above `cut` and counts its entries at `cut`.
-    const int run = (mine + (threads >> 5) - 1) / (threads >> 5);
-    const int w0 = min(mine, warp * run), w1 = min(mine, w0 + run);
+    // Index order from here.  A thread's entries are a run of words (an odd number,
+    // so that a warp's reads hit all banks); it sums what it keeps above `cut` and
+    // counts its entries at `cut`.
+    const int run = ((mine + threads - 1) / threads) | 1;
+    const int w0 = min(mine, tid * run), w1 = min(mine, w0 + run);
+    const uint32_t least = max(max(cut, none), low > 0.F ? K::near(m + t * (logf(low) * 1.001F - 0.001F)) : 0u);
     int sum_h = 0, sum_l = 0, at_cut = 0;
-    for (int w = w0 + lane; w < w1; w += 32) {
+    for (int w = w0; w < w1; ++w) {
         Key k[VE];
         *reinterpret_cast<uint4*>(k) = *reinterpret_cast<const uint4*>(keys + w * VE);
-        if (K::largest(k) < cut) continue;
+        if (K::largest(k) < least) continue;
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
             const float x = weight(k[e]);
@@ -658,7 +715,10 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
         }
     }
     if (!some_ties) at_cut = 0;
-    const int64_t warp_mass = warp_sum48(join_mass(sum_h, sum_l));
+    const int64_t thread_mass = join_mass(sum_h, sum_l);
+    sh.mass[tid] = thread_mass;  // (the list is done with)
+    sh.list[tid] = at_cut;
+    const int64_t warp_mass = warp_sum48(thread_mass);
     const int64_t warp_ties = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(at_cut));
     if (lane == 0) {
         sh.warp[0][warp] = warp_mass;
@@ -690,9 +750,18 @@ __global__ void __launch_bounds__(kMaxSampleThreads) sample_cluster_kernel(const
             const int64_t all_of = (real_warp ? sh.warp[0][lane] : 0) + quota_of * each;
             const int64_t upto_of = warp_scan64(all_of);
             const int hit = __ffs(__ballot_sync(0xffffffffu, upto_of > aim)) - 1;
-            // that warp's run holds the token: 32 words at a time, a lane's entries in order
+            // that warp's threads (lane = thread), then the words of the one that holds the
+            // token, 32 at a time, a lane's entries in order
             int64_t at = __shfl_sync(0xffffffffu, upto_of - all_of, hit), left = __shfl_sync(0xffffffffu, quota_of, hit);
-            const int h0 = min(mine, hit * run), h1 = min(mine, h0 + run);
+            const int ties_here = sh.list[32 * hit + lane];
+            const int64_t ties_before_here = warp_scan64(ties_here) - ties_here;
+            const int64_t quota_here = min(max(left - ties_before_here, static_cast<int64_t>(0)), static_cast<int64_t>(ties_here));
+            const int64_t mass_here = sh.mass[32 * hit + lane] + quota_here * each;
+            const int64_t upto_here = warp_scan64(mass_here);
+            const int hit_lane = __ffs(__ballot_sync(0xffffffffu, at + upto_here > aim)) - 1;
+            at += __shfl_sync(0xffffffffu, upto_here - mass_here, hit_lane);
+            left = __shfl_sync(0xffffffffu, quota_here, hit_lane);
+            const int h0 = min(mine, (32 * hit + hit_lane) * run), h1 = min(mine, h0 + run);
             for (int w = h0; w < h1; w += 32) {
                 Key k[VE];
                 *reinterpret_cast<uint4*>(k) =
