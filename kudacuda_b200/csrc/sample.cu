@@ -283,7 +283,9 @@ struct SampleShared {
     // the search, kept by warp 0
     uint32_t pv[kPivots], lo, hi;
     int64_t above, target;
+    int at_hi;           // entries at or above hi
     int listed, start;   // entries of the list that is made next, or -1; where this block's go in it
+    int everything;      // 1: it holds all entries at or above lo, 0: those below hi
     int own_count;
     uint32_t list[kList];
     // this block's share of the list, then the list's masses; in the end every thread's mass
@@ -469,13 +471,94 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                                                                          : hi - static_cast<uint32_t>(span * (i + 1) / (n + 1));
         return max(min(key, hi - 1), lo + 1);
     };
-    // The largest key whose entries at or above it reach a target (in number, or
-    // in mass): lo reaches it, hi does not.  above: what lies above lo.  The
-    // target may depend on the sum over the entries above the first lo, which
-    // the first try brings along.  The sums of a try meet in warp 0 (lane i: sum
-    // i), which alone decides; the other warps read its decision.
-    auto locate = [&](auto by_mass, auto target_of, uint32_t& lo, int64_t& above, int64_t& target) {
+    // The search: the largest key whose entries at or above it reach a target (in
+    // number, or in mass).  lo reaches it (or is where the search began), hi does
+    // not; above: what lies at or above hi, in the end above lo.
+    int listed = -1;          // entries in sh.list, or -1
+    bool everything = false;  // the list holds all entries at or above its lowest
+    // The end of it, on the list, every block by itself: a warp tries two keys a
+    // round and all warps read all sums (two halves of sh.warp in turn, so that a
+    // round has one barrier).  base: what lies above the list; at_lo, at_hi: entries
+    // of the list at or above lo, hi.
+    auto finish = [&](auto by_mass, uint32_t& lo, uint32_t hi, int64_t base, int at_lo, int at_hi, int64_t& above,
+                      int64_t target) {
+        const int pivots = 2 * (threads >> 5);
+        for (int tries = 0; hi - lo > 1 && at_lo - at_hi > 1; ++tries) {
+            const uint32_t p0 = next_pivot(lo, hi, tries, 2 * warp, pivots);
+            const uint32_t p1 = next_pivot(lo, hi, tries, 2 * warp + 1, pivots);
+            int64_t m0 = 0, m1 = 0;
+            int c0 = 0, c1 = 0;
+            for (int i = lane; i < listed; i += 32) {
+                const uint32_t k = sh.list[i];
+                c0 += k >= p0;
+                c1 += k >= p1;
+                if constexpr (by_mass) {
+                    const int64_t w = sh.mass[i];
+                    m0 += k >= p0 ? w : 0;
+                    m1 += k >= p1 ? w : 0;
+                }
+            }
+            c0 = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c0)));
+            c1 = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c1)));
+            if constexpr (by_mass) {
+                m0 = warp_sum48(m0);
+                m1 = warp_sum48(m1);
+            }
+            int64_t* const sums = sh.warp[2 * (tries & 1)];
+            int64_t* const counts = sh.warp[2 * (tries & 1) + 1];
+            if (lane == 0) {
+                counts[2 * warp] = c0;
+                counts[2 * warp + 1] = c1;
+                sums[2 * warp] = by_mass ? m0 : c0;
+                sums[2 * warp + 1] = by_mass ? m1 : c1;
+            }
+            __syncthreads();
+            const int64_t x = lane < pivots ? sums[lane] : 0;
+            const unsigned reach = __ballot_sync(0xffffffffu, lane < pivots && base + x >= target);
+            const int at = reach != 0 ? __ffs(reach) - 1 : pivots;
+            const uint32_t was_lo = lo, was_hi = hi;
+            if (at < pivots) {
+                lo = next_pivot(was_lo, was_hi, tries, at, pivots);
+                at_lo = static_cast<int>(counts[at]);
+            }
+            if (at > 0) {
+                hi = next_pivot(was_lo, was_hi, tries, at - 1, pivots);
+                at_hi = static_cast<int>(counts[at - 1]);
+                above = base + sums[at - 1];
+            }
+        }
+        if (hi - lo > 1 && at_lo - at_hi == 1) {  // one entry is left
+            uint32_t k = 0;
+            for (int i = lane; i < listed; i += 32)
+                if (sh.list[i] < hi) k = max(k, sh.list[i]);
+            k = __reduce_max_sync(0xffffffffu, k);
+            if (above + (by_mass ? mass(k) : 1) >= target) lo = k;
+            else above += by_mass ? mass(k) : 1;
+        }
+        __syncthreads();
+    };
+    // All of it.  The target may depend on the sum over the entries above the first
+    // lo, which the first try brings along.  The sums of a try meet in warp 0
+    // (lane i: sum i), which alone decides; the other warps read its decision.
+    auto locate = [&](auto by_mass, auto target_of, bool want_list, uint32_t& lo, int64_t& above, int64_t& target) {
+        if (by_mass && listed >= 0 && everything) {  // the search by number has left the entries that are kept
+            int64_t over = 0;
+            int count = 0;
+            for (int i = tid; i < listed; i += threads) sh.mass[i] = mass(sh.list[i]);
+            __syncthreads();
+            for (int i = lane; i < listed; i += 32)
+                if (sh.list[i] > lo) {
+                    over += sh.mass[i];
+                    ++count;
+                }
+            count = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(count)));
+            target = target_of(warp_sum48(over));
+            above = 0;
+            finish(by_mass, lo, top + 1, 0, count, 0, above, target);
+            return;
+        }
         constexpr int N = by_mass ? kSums : kPivots, kCounts = by_mass ? kPivots + 1 : 0;
+        int hi_number = 0;  // (warp 0's) entries at or above hi; lane i: of block i
         if (warp == 0) {
             // Temperatures below the maximum where a nucleus of ordinary logits tends to
             // end.  Five, spread to 13, over four seeds each (64 rows of 16 bits; 333 of
@@ -492,23 +575,22 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                 sh.lo = lo;
                 sh.hi = top + 1;  // nothing lies at or above it
                 sh.above = 0;
+                sh.at_hi = 0;
             }
         }
         __syncthreads();
         for (int tries = 0;; ++tries) {
-            const uint32_t hi = sh.hi;
             uint32_t pv[kPivots];  // falling
 #pragma unroll
             for (int i = 0; i < kPivots; ++i) pv[i] = sh.pv[i];
-            // sums over the entries below hi: at or above each pivot, and above the first lo
+            // sums over the entries at or above each pivot, and above the first lo
             int vh[kPivots + 1], vl[kPivots + 1], vc[kPivots];
 #pragma unroll
             for (int i = 0; i <= kPivots; ++i) vh[i] = vl[i] = 0;
 #pragma unroll
             for (int i = 0; i < kPivots; ++i) vc[i] = 0;
             const uint32_t from = by_mass && tries == 0 ? max(lo + 1, none) : pv[kPivots - 1];
-            auto take = [&](uint32_t k) {
-                k = k < hi ? k : 0;  // (every pivot is above 0)
+            sweep(from, [&](uint32_t k) {
                 if constexpr (by_mass) {
                     int h, l;
                     split_mass(k >= from ? weight(k) : 0.F, h, l);
@@ -525,8 +607,7 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
 #pragma unroll
                     for (int i = 0; i < kPivots; ++i) vc[i] += k >= pv[i];
                 }
-            };
-            sweep(from, take);
+            });
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 int64_t x;
@@ -537,13 +618,11 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                 if (lane == 0) sh.warp[i][warp] = x;
             }
             __syncthreads();
-            int64_t x = 0;
-            if (warp == 0) x = block_sums(sh, N);
             turn ^= 1;
-            if (warp == 0) cluster_send(sh, turn, N, x);
+            if (warp == 0) cluster_send(sh, turn, N, block_sums(sh, N));
             cluster_barrier();
             if (warp == 0) {
-                x = 0;
+                int64_t x = 0;
                 if (lane < N)
                     for (uint32_t r = 0; r < ranks; ++r) x += sh.from[turn][lane][r];
                 if (tries == 0) {
@@ -552,46 +631,53 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                     __syncwarp();
                 }
                 const uint32_t my_pv = sh.pv[lane < kPivots ? lane : 0];
-                const unsigned reach =
-                    __ballot_sync(0xffffffffu, lane < kPivots && sh.above + x >= sh.target);
+                const unsigned reach = __ballot_sync(0xffffffffu, lane < kPivots && x >= sh.target);
                 // the first pivot that reaches the target is the new lo, the one before it the new hi
                 const int at = reach != 0 ? __ffs(reach) - 1 : kPivots;
                 const int i_lo = min(at, kPivots - 1), i_hi = max(at - 1, 0);
                 const uint32_t nlo = __shfl_sync(0xffffffffu, my_pv, i_lo), nhi = __shfl_sync(0xffffffffu, my_pv, i_hi);
                 const int64_t sum_hi = __shfl_sync(0xffffffffu, x, i_hi);
-                const int64_t number_lo = __shfl_sync(0xffffffffu, x, kCounts + i_lo);
-                const int64_t number_hi = __shfl_sync(0xffffffffu, x, kCounts + i_hi);
-                const uint32_t new_lo = at < kPivots ? nlo : sh.lo, new_hi = at > 0 ? nhi : hi;
-                const int64_t number = number_lo - (at > 0 ? number_hi : 0);
-                const bool gather = new_hi - new_lo > 1 && at < kPivots && number <= kList;
-                int64_t before = 0;  // entries of the blocks before this one
-                if (gather && lane < static_cast<int>(rank))
-                    before = sh.from[turn][kCounts + at][lane] - (at > 0 ? sh.from[turn][kCounts + at - 1][lane] : 0);
-                before = warp_sum64(before);
-                __syncwarp();
+                const int number_lo = static_cast<int>(__shfl_sync(0xffffffffu, x, kCounts + i_lo));
+                const int number_hi = static_cast<int>(__shfl_sync(0xffffffffu, x, kCounts + i_hi));
+                const uint32_t new_lo = at < kPivots ? nlo : sh.lo, new_hi = at > 0 ? nhi : sh.hi;
+                const int all_hi = at > 0 ? number_hi : sh.at_hi;
+                const bool real = lane < static_cast<int>(ranks);
+                if (at > 0) hi_number = real ? static_cast<int>(sh.from[turn][kCounts + i_hi][lane]) : 0;
+                // A list of all that lies above lo, or of what lies between, if they are few.
+                const bool narrow = new_hi - new_lo <= 1;
+                const bool all = at < kPivots && number_lo <= kList && (!narrow || want_list);
+                const bool some = at < kPivots && number_lo - all_hi <= kList && !narrow;
+                const int own = all || some ? static_cast<int>(real ? sh.from[turn][kCounts + i_lo][lane] : 0) - (all ? 0 : hi_number) : 0;
+                // (entries of the blocks before this one)
+                const int before = static_cast<int>(
+                    __reduce_add_sync(0xffffffffu, static_cast<unsigned>(lane < static_cast<int>(rank) ? own : 0)));
                 const uint32_t pivot = next_pivot(new_lo, new_hi, tries, lane, kPivots);
+                __syncwarp();
                 if (lane < kPivots) sh.pv[lane] = pivot;
                 if (lane == 0) {
                     sh.lo = new_lo;
                     sh.hi = new_hi;
-                    if (at > 0) sh.above += sum_hi;
-                    sh.listed = gather ? static_cast<int>(number) : -1;
-                    sh.start = static_cast<int>(before);
+                    if (at > 0) sh.above = sum_hi;
+                    sh.at_hi = all_hi;
+                    sh.listed = all ? number_lo : some ? number_lo - all_hi : -1;
+                    sh.everything = all ? 1 : 0;
+                    sh.start = before;
                     sh.own_count = 0;
                 }
             }
             __syncthreads();
             if (sh.listed >= 0 || sh.hi - sh.lo <= 1) break;
         }
-        uint32_t hi = sh.hi;
-        const int listed = sh.listed;
+        const uint32_t hi = sh.hi;
+        listed = sh.listed;
+        everything = sh.everything != 0;
         lo = sh.lo;
         above = sh.above;
         target = sh.target;
-        if (listed >= 0) {
-            // the keys in [lo, hi) of every block to every block
+        if (listed >= 0) {  // the keys of every block to every block
+            const uint32_t end = everything ? top + 1 : hi;
             sweep(lo, [&](uint32_t k) {
-                if (k >= lo && k < hi) sh.own[atomicAdd(&sh.own_count, 1)] = k;
+                if (k >= lo && k < end) sh.own[atomicAdd(&sh.own_count, 1)] = k;
             });
             __syncthreads();
             const int own = sh.own_count, start = sh.start;
@@ -604,63 +690,11 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                 for (int i = tid; i < listed; i += threads) sh.mass[i] = mass(sh.list[i]);
                 __syncthreads();
             }
-            // From here every block finishes alone: a warp tries two keys a round and
-            // all warps read all sums (two halves of sh.warp in turn, so that a
-            // round has one barrier).
-            const int pivots = 2 * (threads >> 5);
-            int inside = listed;  // entries in [lo, hi)
-            for (int tries = 0; hi - lo > 1; ++tries) {
-                const uint32_t p0 = next_pivot(lo, hi, tries, 2 * warp, pivots);
-                const uint32_t p1 = next_pivot(lo, hi, tries, 2 * warp + 1, pivots);
-                int64_t m0 = 0, m1 = 0;
-                int c0 = 0, c1 = 0;
-                for (int i = lane; i < listed; i += 32) {
-                    const uint32_t k = sh.list[i];
-                    const bool in0 = k < hi && k >= p0, in1 = k < hi && k >= p1;
-                    c0 += in0;
-                    c1 += in1;
-                    if constexpr (by_mass) {
-                        const int64_t w = sh.mass[i];
-                        m0 += in0 ? w : 0;
-                        m1 += in1 ? w : 0;
-                    }
-                }
-                c0 = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c0)));
-                c1 = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c1)));
-                if constexpr (by_mass) {
-                    m0 = warp_sum48(m0);
-                    m1 = warp_sum48(m1);
-                }
-                int64_t* const sums = sh.warp[2 * (tries & 1)];
-                int64_t* const counts = sh.warp[2 * (tries & 1) + 1];
-                if (lane == 0) {
-                    counts[2 * warp] = c0;
-                    counts[2 * warp + 1] = c1;
-                    sums[2 * warp] = by_mass ? m0 : c0;
-                    sums[2 * warp + 1] = by_mass ? m1 : c1;
-                }
-                __syncthreads();
-                const int64_t x = lane < pivots ? sums[lane] : 0;
-                const unsigned reach = __ballot_sync(0xffffffffu, lane < pivots && above + x >= target);
-                const int at = reach != 0 ? __ffs(reach) - 1 : pivots;
-                if (at < pivots) inside = static_cast<int>(counts[at]);
-                const uint32_t was_lo = lo, was_hi = hi;
-                if (at < pivots) lo = next_pivot(was_lo, was_hi, tries, at, pivots);
-                if (at > 0) {
-                    hi = next_pivot(was_lo, was_hi, tries, at - 1, pivots);
-                    above += sums[at - 1];
-                    inside -= static_cast<int>(counts[at - 1]);
-                }
-                if (inside == 1) {  // the one entry left is it
-                    uint32_t k = 0;
-                    for (int i = lane; i < listed; i += 32)
-                        if (sh.list[i] < hi) k = max(k, sh.list[i]);
-                    lo = __reduce_max_sync(0xffffffffu, k);
-                    break;
-                }
-            }
+            const int at_hi = everything ? sh.at_hi : 0;
+            finish(by_mass, lo, hi, everything ? 0 : above, listed, at_hi, above, target);
+        } else {
+            __syncthreads();
         }
-        __syncthreads();
     };
     // kept: key > cut, and the first `ties` (by index) of the entries with key == cut
     uint32_t cut = 0;  // below every entry: all are kept
@@ -672,7 +706,7 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
     constexpr std::integral_constant<bool, true> by_mass{};
     if (k_ > 0 && k_ < n) {
         int64_t above, target;
-        locate(by_number, [&](int64_t) { return static_cast<int64_t>(k_); }, cut, above, target);
+        locate(by_number, [&](int64_t) { return static_cast<int64_t>(k_); }, p < 1.F, cut, above, target);
         ties = k_ - above;
         some_ties = true;
     }
@@ -684,7 +718,7 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
             const int64_t whole = over + (some_ties ? ties * mass(cut) : 0);
             const int64_t r = __double2ll_ru(__dmul_rn(static_cast<double>(p), __ll2double_rn(whole)));
             return r < 1 ? 1 : r;
-        }, lo, above, reach);
+        }, false, lo, above, reach);
         const int64_t each = lo > 0 ? mass(lo) : 0;
         const int64_t need = each > 0 ? (reach - above + each - 1) / each : 0;
         if (each > 0 && (lo > cut || need < ties)) ties = need;
