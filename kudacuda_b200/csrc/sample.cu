@@ -210,6 +210,8 @@ constexpr int kPivots = 5;
 constexpr int kMaxCluster = 16;  // more than 8 need the kernel's consent (launch_cluster)
 constexpr int kMaxSampleThreads = 512;
 constexpr int kList = 1024;
+constexpr int kBins = 256;
+static_assert(3 * kBins <= kList && kBins % kMaxCluster == 0);
 
 template <int DT>
 struct Keys {
@@ -286,6 +288,7 @@ struct SampleShared {
     int at_hi;           // entries at or above hi
     int listed, start;   // entries of the list that is made next, or -1; where this block's go in it
     int everything;      // 1: it holds all entries at or above lo, 0: those below hi
+    int counted;         // 1: so few keys are left that each is counted
     int own_count;
     uint32_t list[kList];
     // this block's share of the list, then the list's masses; in the end every thread's mass
@@ -661,12 +664,13 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                     sh.at_hi = all_hi;
                     sh.listed = all ? number_lo : some ? number_lo - all_hi : -1;
                     sh.everything = all ? 1 : 0;
+                    sh.counted = at < kPivots && new_hi - new_lo <= kBins ? 1 : 0;
                     sh.start = before;
                     sh.own_count = 0;
                 }
             }
             __syncthreads();
-            if (sh.listed >= 0 || sh.hi - sh.lo <= 1) break;
+            if (sh.listed >= 0 || sh.hi - sh.lo <= 1 || sh.counted != 0) break;
         }
         const uint32_t hi = sh.hi;
         listed = sh.listed;
@@ -692,6 +696,59 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
             }
             const int at_hi = everything ? sh.at_hi : 0;
             finish(by_mass, lo, hi, everything ? 0 : above, listed, at_hi, above, target);
+        } else if (hi - lo > 1) {
+            // Many entries of few keys (16-bit types): counters, one a key, in the place of
+            // the list.  Block i adds up the keys number i, i + ranks, ... of all blocks
+            // and tells them.
+            const uint32_t span = hi - lo;
+            const int per = kBins / static_cast<int>(ranks);
+            uint32_t* const bin = sh.list;
+            uint32_t* const got = sh.list + kBins;
+            uint32_t* const sum = sh.list + 2 * kBins;
+            for (int i = tid; i < kBins; i += threads) bin[i] = 0;
+            __syncthreads();
+            sweep(lo, [&](uint32_t k) {
+                if (k - lo < span) atomicAdd(&bin[k - lo], 1u);
+            });
+            __syncthreads();
+            for (int i = tid; i < kBins; i += threads) {
+                const int owner = i & (static_cast<int>(ranks) - 1);
+                store_remote32(&got[rank * per + i / ranks], owner, bin[i]);
+            }
+            cluster_barrier();
+            for (int i = tid; i < per; i += threads) {
+                uint32_t c = 0;
+                for (uint32_t r = 0; r < ranks; ++r) c += got[r * per + i];
+                for (uint32_t r = 0; r < ranks; ++r) store_remote32(&sum[i * ranks + rank], r, c);
+            }
+            cluster_barrier();
+            // every warp: a lane has kBins / 32 keys in a row, the highest first
+            constexpr int kEach = kBins / 32;
+            int64_t x[kEach], mine_sum = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const uint32_t back = lane * kEach + i;  // keys below hi - 1
+                x[i] = back < span ? static_cast<int64_t>(sum[span - 1 - back]) : 0;
+                if constexpr (by_mass)
+                    if (x[i] != 0) x[i] *= mass(hi - 1 - back);
+                mine_sum += x[i];
+            }
+            const int64_t upto = warp_scan64(mine_sum);
+            const unsigned reach = __ballot_sync(0xffffffffu, above + upto >= target);
+            const int at = reach != 0 ? __ffs(reach) - 1 : 31;  // (lo reaches the target, so some lane does)
+            int64_t c = above + upto - mine_sum;
+            uint32_t found = lo;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const uint32_t back = lane * kEach + i;
+                if (found == lo && back + 1 < span) {
+                    if (c + x[i] >= target) found = hi - 1 - back;
+                    else c += x[i];
+                }
+            }
+            lo = __shfl_sync(0xffffffffu, found, at);
+            above = __shfl_sync(0xffffffffu, c, at);
+            __syncthreads();
         } else {
             __syncthreads();
         }
