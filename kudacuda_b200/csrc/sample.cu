@@ -198,15 +198,25 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
 //
 // The logits become ordered keys (whole numbers in the order of the values,
 // 16 bits wide for the 16-bit types), read from memory once.  What remains is
-// to find the key at which the kept prefix ends: seven keys that split the
+// to find the key at which the kept prefix ends: kPivots keys that split the
 // range still possible are tried at once - each thread counts the entries at or
 // above each of them, and sums their masses, in registers - and the cluster
-// exchanges the sums through distributed shared memory with one barrier.  The
-// first seven lie at fixed distances below the maximum (in units of the
-// temperature), which leaves few entries; when at most kList are left, every
-// block gets all of their keys and finishes alone, without the cluster's
-// barriers.  No sort, no atomics on memory.
+// exchanges the sums through distributed shared memory with one barrier.  When
+// at most kList entries are left, every block gets all of their keys and
+// finishes alone; when at most kBins keys are left (16-bit types), the entries of
+// each are counted.  Both use atomics only where their order does not show: for
+// places in a list that is only summed over, and for whole numbers.
+//
+// The logits are read once, so memory asks 3 us of 64 rows of 151 936 16-bit
+// logits and 10 us of 333 rows of 50 257 32-bit ones.  What they do cost, rows of
+// all kinds mixed, 60 and 103 us, is instructions and waits: every entry takes an
+// exponential, two roundings and three additions a key tried in the first try,
+// and the pass in index order takes the exponential again (64 rows, all of one
+// kind: greedy 16 us, min-p 20, temperature alone 35, top-k 35, both limits 39,
+// top-p 75).  One row costs 17 us in 16 blocks, mostly its cluster's barriers:
+// there are six or so, of 1 to 2 us with what goes on between them.
 constexpr int kPivots = 5;
+constexpr float kFirst = 2.5F;
 constexpr int kMaxCluster = 16;  // more than 8 need the kernel's consent (launch_cluster)
 constexpr int kMaxSampleThreads = 512;
 constexpr int kList = 1024;
@@ -470,8 +480,9 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
         const float x_hi = K::value(min(hi, top)), x_lo = fmaxf(K::value(lo), m - 30.F * t);
         const float step = (x_hi - x_lo) / (n + 1);
         const uint64_t span = hi - lo;
-        const uint32_t key = tries < 3 && step > 0.F && step < 1.0e30F ? K::near(x_hi - step * (i + 1))
-                                                                         : hi - static_cast<uint32_t>(span * (i + 1) / (n + 1));
+        const bool by_value = tries < 3 && step > 0.F && step < 1.0e30F;
+        const uint32_t key =
+            by_value ? K::near(x_hi - step * (i + 1)) : hi - static_cast<uint32_t>(span * (i + 1) / (n + 1));
         return max(min(key, hi - 1), lo + 1);
     };
     // The search: the largest key whose entries at or above it reach a target (in
@@ -563,17 +574,12 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
         constexpr int N = by_mass ? kSums : kPivots, kCounts = by_mass ? kPivots + 1 : 0;
         int hi_number = 0;  // (warp 0's) entries at or above hi; lane i: of block i
         if (warp == 0) {
-            // Temperatures below the maximum where a nucleus of ordinary logits tends to
-            // end.  Five, spread to 13, over four seeds each (64 rows of 16 bits; 333 of
-            // 32): 81 and 140 us; seven to 12.5: 83 and 144; seven to 12 that start at
-            // 0.7: 84 and 149; three: 81 and 143.
-            const float d[kPivots] = {1.5F, 3.5F, 6.F, 9.F, 13.F};
-            float mine_d = d[0];
-#pragma unroll
-            for (int i = 1; i < kPivots; ++i)
-                if (lane == i) mine_d = d[i];
+            // The first try: every kFirst temperatures below the maximum, which is where a
+            // nucleus of ordinary logits tends to end.  Five keys that far apart, means of
+            // four seeds (64 rows of 16 bits, 333 of 32): 60 and 103 us; four, 3 apart: 64
+            // and 108; at 1.5, 3.5, 6, 9, 13: 66 and 110; six, to 14: 65 and 107.
             // (with lo == top no key lies between: every pivot is top + 1, where nothing is)
-            if (lane < kPivots) sh.pv[lane] = max(min(K::near(m - mine_d * t), top), lo + 1);
+            if (lane < kPivots) sh.pv[lane] = max(min(K::near(m - kFirst * (lane + 1) * t), top), lo + 1);
             if (lane == 0) {
                 sh.lo = lo;
                 sh.hi = top + 1;  // nothing lies at or above it
@@ -614,10 +620,8 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 int64_t x;
-                if constexpr (by_mass)
-                    x = i <= kPivots ? warp_sum48(join_mass(vh[i], vl[i]))
-                                     : __reduce_add_sync(0xffffffffu, static_cast<unsigned>(vc[i > kPivots ? i - kPivots - 1 : 0]));
-                else x = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(vc[i]));
+                if (by_mass && i <= kPivots) x = warp_sum48(join_mass(vh[i], vl[i]));
+                else x = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(vc[by_mass ? i - kPivots - 1 : i]));
                 if (lane == 0) sh.warp[i][warp] = x;
             }
             __syncthreads();
@@ -650,7 +654,8 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                 const bool narrow = new_hi - new_lo <= 1;
                 const bool all = at < kPivots && number_lo <= kList && (!narrow || want_list);
                 const bool some = at < kPivots && number_lo - all_hi <= kList && !narrow;
-                const int own = all || some ? static_cast<int>(real ? sh.from[turn][kCounts + i_lo][lane] : 0) - (all ? 0 : hi_number) : 0;
+                const int own_lo = real ? static_cast<int>(sh.from[turn][kCounts + i_lo][lane]) : 0;
+                const int own = all || some ? own_lo - (all ? 0 : hi_number) : 0;
                 // (entries of the blocks before this one)
                 const int before = static_cast<int>(
                     __reduce_add_sync(0xffffffffu, static_cast<unsigned>(lane < static_cast<int>(rank) ? own : 0)));
@@ -846,7 +851,8 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
             int64_t at = __shfl_sync(0xffffffffu, upto_of - all_of, hit), left = __shfl_sync(0xffffffffu, quota_of, hit);
             const int ties_here = sh.list[32 * hit + lane];
             const int64_t ties_before_here = warp_scan64(ties_here) - ties_here;
-            const int64_t quota_here = min(max(left - ties_before_here, static_cast<int64_t>(0)), static_cast<int64_t>(ties_here));
+            const int64_t quota_here =
+                min(max(left - ties_before_here, static_cast<int64_t>(0)), static_cast<int64_t>(ties_here));
             const int64_t mass_here = sh.mass[32 * hit + lane] + quota_here * each;
             const int64_t upto_here = warp_scan64(mass_here);
             const int hit_lane = __ffs(__ballot_sync(0xffffffffu, at + upto_here > aim)) - 1;
