@@ -1483,6 +1483,13 @@ class KudaCudaBridge:
         return code, shape, (query_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(),
                              stride if batch > 1 else width, width, batch)
 
+    def _require_device(self, *tensors: Any) -> None:
+        """Refuses tensors that are not in this bridge's device memory (a kernel would fault on them)."""
+
+        for t in tensors:
+            if t is not None and t.get_device() != self.device_id:
+                raise ValueError(f"every tensor must be on cuda:{self.device_id}, found {t.device}")
+
     @staticmethod
     def _head_rows(tensor: Any, head_dim: int, label: str) -> tuple[int, int, int]:
         """(rows, columns, row stride) of [rows, heads, head_dim] or [rows, heads * head_dim] with
@@ -1531,6 +1538,7 @@ class KudaCudaBridge:
         if bias is not None and (bias.dim() != 1 or bias.shape[0] != cols or bias.dtype is not dtype
                                  or not bias.is_contiguous()):
             raise ValueError("bias must have one element per column of qkv, in its dtype")
+        self._require_device(qkv, q_out, k_pages, v_pages, rope_cos, rope_sin, query_start, kv_len, block_table, bias)
         self._call("kudacuda_sm100_rope_append_paged", code, qkv.data_ptr(), stride,
                    0 if bias is None else bias.data_ptr(), q_out.data_ptr(), out_stride, k_pages.data_ptr(),
                    v_pages.data_ptr(), cos, sin, max_pos, rotary, 1 if interleaved else 0, *batch, rows,
@@ -1570,6 +1578,7 @@ class KudaCudaBridge:
         if lse is not None and (lse.dtype is not self._types[2] or lse.shape != (rows, heads)
                                 or not lse.is_contiguous()):
             raise ValueError("lse must be contiguous float32 [rows, q_heads]")
+        self._require_device(query, k_pages, v_pages, output, query_start, kv_len, block_table, workspace, lse)
         self._call("kudacuda_sm100_paged_attention", code, query.data_ptr(), stride, k_pages.data_ptr(),
                    v_pages.data_ptr(), output.data_ptr(), out_stride, 0 if lse is None else lse.data_ptr(),
                    workspace.data_ptr(), workspace.nbytes, *batch, rows, max_query, heads, kv_heads, head_dim,
@@ -1608,6 +1617,7 @@ class KudaCudaBridge:
                     or not page_map.is_contiguous()):
                 raise ValueError("page_map must be contiguous int32 [num_pages]")
             table = (block_table.data_ptr(), stride if rows > 1 else width, rows, width)
+        self._require_device(k_pages, v_pages, pairs, block_table, page_map)
         self._call("kudacuda_sm100_kv_pages_copy", k_pages.data_ptr(), v_pages.data_ptr(), shape[0], layer_bytes,
                    num_pages, layer_bytes // max(1, num_pages), pairs.data_ptr(), pairs.shape[0], *table,
                    0 if page_map is None else page_map.data_ptr(), stream_ptr & 0xFFFFFFFFFFFFFFFF)
@@ -1640,6 +1650,7 @@ class KudaCudaBridge:
                 raise ValueError("temperature, top_k, top_p, min_p, uniform, tokens and logprobs must be contiguous "
                                  f"[rows] vectors (top_k and tokens int32, the others float32) of {rows} elements")
             pointers.append(tensor.data_ptr())
+        self._require_device(logits, temperature, top_k, top_p, min_p, uniform, tokens, logprobs)
         self._call("kudacuda_sm100_sample", code, logits.data_ptr(), stride if rows > 1 else vocab, rows, vocab,
                    *pointers, stream_ptr & 0xFFFFFFFFFFFFFFFF)
 

@@ -467,6 +467,36 @@ def test_sample_values_of_every_size(bridge):
     check_rows(bridge, x, u, [[0.8, 30.0][r % 2] for r in range(24)], k, p, [0.0] * 12 + [1e-4] * 12)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 3000), (BF16, 3000), (F16, 3000), (BF16, 20000)])
+def test_sample_many_entries_of_few_values(bridge, dtype, vocab):
+    """The kept prefix ends among more entries than fit a list, all of a few values."""
+
+    g = torch.Generator().manual_seed(vocab)
+    rows = 24
+    x = ((4.0 * 1.5 * torch.randn((rows, vocab), generator=g)).round() / 4.0).to(dtype).to(DEV)
+    u = torch.rand((rows,), generator=g).tolist()
+    k = [[0, 0, 1500, 2999][r % 4] for r in range(rows)]
+    p = [[0.5, 0.9, 0.97, 1.0, 0.99, 0.8][r % 6] for r in range(rows)]
+    check_rows(bridge, x, u, [[0.6, 1.0, 3.0][r % 3] for r in range(rows)], k, p, [0.0] * 16 + [1e-3] * 8)
+
+
+def test_tensors_in_other_memory_are_refused(bridge):
+    x = torch.zeros((2, 64), device=DEV)
+    tokens, u = torch.zeros((2,), dtype=torch.int32, device=DEV), torch.zeros((2,), device=DEV)
+    with pytest.raises(ValueError, match="cuda:0"):
+        bridge.dispatch_sample(x, tokens, u.cpu(), stream_ptr=0)
+    k = torch.zeros((2, 4, 1, 16, 64), dtype=F16, device=DEV)
+    with pytest.raises(ValueError, match="cuda:0"):
+        bridge.dispatch_kv_pages_copy(k, k.clone(), torch.zeros((1, 2), dtype=torch.int32), stream_ptr=0)
+    start, n, table = (torch.tensor(v, dtype=torch.int32, device=DEV) for v in ([0, 1], [1], [[0]]))
+    q, qkv = torch.zeros((1, 1, 64), dtype=F16, device=DEV), torch.zeros((1, 192), dtype=F16, device=DEV)
+    ws = bridge.paged_attention_workspace(q, k[0], table, max_query=1)
+    with pytest.raises(ValueError, match="cuda:0"):
+        bridge.dispatch_paged_attention(q, k[0], k[1], q.clone(), start, n.cpu(), table, ws, max_query=1, stream_ptr=0)
+    with pytest.raises(ValueError, match="cuda:0"):
+        bridge.dispatch_rope_append_paged(qkv, q, k[0], k[1], None, None, start, n, table.cpu(), stream_ptr=0)
+
+
 def test_sample_ends_of_the_uniform_range_and_defaults(bridge):
     x = torch.tensor([[0.0, 1.0, -math.inf, 2.0, -math.inf]] * 4, device=DEV)
     tokens, logp = sample(bridge, x, [0.0, 1.0 - 2.0**-24, 0.5, 5.0])

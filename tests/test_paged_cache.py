@@ -208,6 +208,7 @@ class Recorder:
 def bridge():
     lib = Recorder()
     br = KudaCudaBridge(device_id=0, native_lib=lib)
+    br.device_id = -1  # the index that torch gives host memory
     lib.calls.clear()
     yield SimpleNamespace(br=br, lib=lib)
 
