@@ -339,10 +339,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int token = (w.q * kRows + r) / group;
             // this row's keys, relative to the item: never more than the item's
             const int row_keys = live ? min(max(w.piece_len - w.piece_n + token + 1, 0), w.limit) : w.limit;
+            const bool idle = !__any_sync(0xffffffffu, live);  // a warp of rows past the item: it only keeps step
             float m = -INFINITY, l = 0.F;
             for (int j = w.t0; j < w.t1; ++j) {
                 bar_wait(&bars.s_full[t], ns++ & 1, abort_p);
                 tc_fence_after();
+                if (idle) {  // (what its lanes of P hold reaches no row of the item)
+                    tc_fence_before();
+                    bar_arrive(&bars.p_half[t]);
+                    bar_arrive(&bars.p_ready[t]);
+                    continue;
+                }
                 float s[kKeys];
 #pragma unroll
                 for (int i = 0; i < kKeys; i += 32) tmem_ld32(ts + i, s + i);
@@ -403,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- the piece's end
             bar_wait(&bars.o_done[t], no++ & 1, abort_p);
             tc_fence_after();
+            if (idle) continue;
             if (w.whole()) {
                 const float inv = l == 0.F ? 0.F : 1.F / l;
                 const int64_t row = w.piece_start + token;
@@ -415,22 +423,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_wait_ld();
                     if (live) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8)
-                            *reinterpret_cast<uint4*>(out + i + k) =
-                                make_uint4(pack2<DT>(o[k] * inv, o[k + 1] * inv), pack2<DT>(o[k + 2] * inv, o[k + 3] * inv),
-                                           pack2<DT>(o[k + 4] * inv, o[k + 5] * inv), pack2<DT>(o[k + 6] * inv, o[k + 7] * inv));
+                        for (int k = 0; k < 32; k += 8) {
+                            uint32_t x[4];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) x[y] = pack2<DT>(o[k + 2 * y] * inv, o[k + 2 * y + 1] * inv);
+                            *reinterpret_cast<uint4*>(out + i + k) = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
                     }
                 }
                 if (live && a.lse != nullptr) a.lse[row * p.q_heads + head] = l == 0.F ? -INFINITY : m * kLn2 + logf(l);
             } else {
                 float* part = Part::slot(a.workspace, gridDim.x, worker, w.t0 > 0 ? 0 : 1);
-                *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, l);
+                if (live) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, l);
                 float4* acc = reinterpret_cast<float4*>(part + 2 * kRows);
 #pragma unroll 1
                 for (int i = 0; i < D; i += 32) {
                     float o[32];
                     tmem_ld32(to + i, o);
                     tmem_wait_ld();
+                    if (!live) continue;
 #pragma unroll
                     for (int k = 0; k < 32; k += 4)
                         __stcg(acc + ((i + k) >> 2) * kRows + r, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
