@@ -37,31 +37,15 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
                  : "memory");
 }
 
-// The same for a whole warp that runs converged, of which one lane (`lead`) issues:
-// the descriptors of a converged warp stay in uniform registers, where the
-// instructions want them.  Issued by a lone thread, whose values the compiler
-// cannot know to be uniform, each one costs several register moves (measured in
-// the paged attention: about 95 clocks an instruction, half of its time).
-__device__ __forceinline__ void umma_bf16_warp(uint32_t lead, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
-                                               uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(lead));
-}
-__device__ __forceinline__ void umma_bf16_ts_warp(uint32_t lead, uint32_t tmem_d, uint32_t tmem_a, uint64_t db,
-                                                  uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc), "r"(lead));
-}
-__device__ __forceinline__ void umma_commit_warp(uint32_t lead, uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-        "r"(lead)
-        : "memory");
+// True in one lane of a converged warp, the same one each time.  The compiler
+// knows that a branch on it has one thread, so matrix instructions inside it are
+// issued from uniform registers one after the other: 64 clocks for one of 128 x
+// 128 x 16, as fast as they run.  Behind a test of the lane's number, or with it
+// as their predicate, each takes 92, whatever its size.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
 }
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {

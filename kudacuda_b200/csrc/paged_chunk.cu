@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         paged_place<W, kLeast, kThreads>(p, group, worker, gridDim.x, sums, &place_seq, &place_at);
     tc_fence_after();
     pdl_launch_dependents();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+    const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_slot);
     volatile int* const abort_p = &abort_flag;
     W w;
     w.begin(p, group, shares, worker, place_seq, place_at);
@@ -212,62 +212,65 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else bar_wait(&bars.kv_full[s], (i / M::kStages) & 1, abort_p, false);
             }
         } else if (warp == 9) {
-            // ---- MMA issuer: the warp runs converged, lane 0 issues
-            {
-                const uint32_t lead = lane == 0 ? 1u : 0u;
-                constexpr uint32_t kIdescS = umma_idesc(DT == kBF16, 128, 128, false);
-                constexpr uint32_t kIdescO = umma_idesc(DT == kBF16, 128, D, true);
-                uint32_t seq = 0, items = 0, np[2] = {0, 0};
-                const uint32_t q_addr = smem_u32(qs), r_addr = smem_u32(ring);
-                while (__shfl_sync(0xffffffffu, w.next(p, group) ? 1 : 0, 0)) {
-                    const int active = __shfl_sync(0xffffffffu, w.item_rows > 128 ? 2 : 1, 0);
-                    const int n = __shfl_sync(0xffffffffu, w.t1 - w.t0, 0);
-                    bar_wait(&bars.q_full, items & 1, abort_p);
-                    for (int j = 0; j <= n; ++j) {
-                        // O_t += P_t(j - 1) V(j - 1), then S_t = Q_t K(j)^T over P_t(j - 1)'s
-                        // columns: the matrix instructions of one thread run in order
-                        const uint32_t sv = seq + 2 * j - 1, sk = seq + 2 * j;
-                        if (j > 0) bar_wait(&bars.kv_full[sv % M::kStages], (sv / M::kStages) & 1, abort_p);
-                        if (j < n) bar_wait(&bars.kv_full[sk % M::kStages], (sk / M::kStages) & 1, abort_p);
-                        tc_fence_after();
-                        const uint32_t va = r_addr + (sv % M::kStages) * M::kTile;
-                        const uint32_t ka = r_addr + (sk % M::kStages) * M::kTile;
-                        for (int t = 0; t < active; ++t) {
-                            if (j > 0) {
-                                // (the first half of P multiplies while the second is still being made)
+            // ---- MMA issuer: the warp runs converged, one lane issues
+            constexpr uint32_t kIdescS = umma_idesc(DT == kBF16, 128, 128, false);
+            constexpr uint32_t kIdescO = umma_idesc(DT == kBF16, 128, D, true);
+            uint32_t seq = 0, items = 0, np[2] = {0, 0};
+            const uint32_t q_addr = smem_u32(qs), r_addr = smem_u32(ring);
+            while (__any_sync(0xffffffffu, w.next(p, group))) {
+                const int active = __reduce_max_sync(0xffffffffu, w.item_rows > 128 ? 2 : 1);
+                const int n = __reduce_max_sync(0xffffffffu, w.t1 - w.t0);
+                bar_wait(&bars.q_full, items & 1, abort_p);
+                for (int j = 0; j <= n; ++j) {
+                    // O_t += P_t(j - 1) V(j - 1), then S_t = Q_t K(j)^T over P_t(j - 1)'s
+                    // columns: the matrix instructions of one thread run in order
+                    const uint32_t sv = seq + 2 * j - 1, sk = seq + 2 * j;
+                    if (j > 0) bar_wait(&bars.kv_full[sv % M::kStages], (sv / M::kStages) & 1, abort_p);
+                    if (j < n) bar_wait(&bars.kv_full[sk % M::kStages], (sk / M::kStages) & 1, abort_p);
+                    tc_fence_after();
+                    const uint32_t va = r_addr + (sv % M::kStages) * M::kTile;
+                    const uint32_t ka = r_addr + (sk % M::kStages) * M::kTile;
+                    for (int t = 0; t < active; ++t) {
+                        if (j > 0) {
+                            // (the first half of P multiplies while the second is still being made)
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    bar_wait(h ? &bars.p_ready[t] : &bars.p_half[t], np[t] & 1, abort_p);
-                                    tc_fence_after();
+                            for (int h = 0; h < 2; ++h) {
+                                bar_wait(h ? &bars.p_ready[t] : &bars.p_half[t], np[t] & 1, abort_p);
+                                tc_fence_after();
+                                if (elect_one()) {
 #pragma unroll
                                     for (int k = h * (kKeys / 32); k < (h + 1) * (kKeys / 32); ++k)
-                                        umma_bf16_ts_warp(lead, tmem + 256 + t * D, tmem + t * 128 + 8 * k,
+                                        umma_bf16_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * k,
                                                      umma_desc_sw128_mn(va + 2048 * k, 128 * 128), kIdescO,
                                                      (j > 1 || k > 0) ? 1u : 0u);
                                 }
-                                ++np[t];
+                                __syncwarp();
                             }
+                            ++np[t];
+                        }
+                        if (elect_one()) {
                             if (j < n) {
 #pragma unroll
                                 for (int k = 0; k < D / 16; ++k) {
                                     const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-                                    umma_bf16_warp(lead, tmem + t * 128, umma_desc_sw128(q_addr + t * M::kTile + off),
+                                    umma_bf16(tmem + t * 128, umma_desc_sw128(q_addr + t * M::kTile + off),
                                               umma_desc_sw128(ka + off), kIdescS, k > 0 ? 1u : 0u);
                                 }
-                                umma_commit_warp(lead, &bars.s_full[t]);
+                                umma_commit(&bars.s_full[t]);
                             } else {
-                                umma_commit_warp(lead, &bars.o_done[t]);
+                                umma_commit(&bars.o_done[t]);
                             }
                             if (t == active - 1) {
-                                if (j > 0) umma_commit_warp(lead, &bars.kv_empty[sv % M::kStages]);
-                                if (j < n) umma_commit_warp(lead, &bars.kv_empty[sk % M::kStages]);
-                                if (j == n - 1) umma_commit_warp(lead, &bars.q_empty);
+                                if (j > 0) umma_commit(&bars.kv_empty[sv % M::kStages]);
+                                if (j < n) umma_commit(&bars.kv_empty[sk % M::kStages]);
+                                if (j == n - 1) umma_commit(&bars.q_empty);
                             }
                         }
+                        __syncwarp();
                     }
-                    seq += 2 * n;
-                    ++items;
                 }
+                seq += 2 * n;
+                ++items;
             }
         } else if (warp == 10) {
             // ---- Q: row R of the item is token R / group, head R % group; rows past the item are zero
