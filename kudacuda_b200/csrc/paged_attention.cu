@@ -14,11 +14,13 @@
 namespace kc {
 
 // Query rows a key head (of the longest sequence) up to which the decode kernel
-// serves: its tile, for a second one reads the cache again.  Decode and chunk
-// kernel, us, 4 key heads of 128 bf16 dims, 1 token of 8 heads / 2 / 3:
-//   64 sequences of 500 keys    25.7, 31.7 / 28.8, 32.4 / 42.3, 32.3
-//   16 of 2000                  22.8, 27.8 / 24.8, 28.0 / 32.6, 28.1
-//   2 of 100000                 77.1, 88.2 / 77.8, 87.9 / 136, 88.2
+// serves: its tile, for a second one it reads the cache again.  It also keeps the
+// probabilities to twice the type's precision.  Decode and chunk kernel, us, 4
+// key heads of 128 bf16 dims, 1 token of 8 heads / 2 / 3:
+//   64 sequences of 500 keys    25.8, 27.6 / 28.8, 27.9 / 42.4, 28.2
+//   16 of 2000                  22.9, 23.9 / 24.8, 24.1 / 32.7, 24.5
+//   1 of 8000                   15.1, 17.8 / 15.8, 18.0 / 19.7, 18.4
+//   2 of 100000                 74.4, 79.8 / 75.9, 80.5 / 135, 81.1
 constexpr int64_t kDecodeRows = 16;
 
 int64_t paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t max_query, int64_t q_heads,
