@@ -209,12 +209,12 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
 //
 // The logits are read once, so memory asks 3 us of 64 rows of 151 936 16-bit
 // logits and 10 us of 333 rows of 50 257 32-bit ones.  What they do cost, rows of
-// all kinds mixed, 60 and 103 us, is instructions and waits: every entry takes an
-// exponential, two roundings and three additions a key tried in the first try,
-// and the pass in index order takes the exponential again (64 rows, all of one
-// kind: greedy 16 us, min-p 20, temperature alone 35, top-k 35, both limits 39,
-// top-p 75).  One row costs 17 us in 16 blocks, mostly its cluster's barriers:
-// there are six or so, of 1 to 2 us with what goes on between them.
+// all kinds mixed, 47 and 88 us, is instructions in the first try and in the pass
+// in index order (an exponential and two roundings an entry, three additions more
+// for every key tried), and waits: a row goes through six or so barriers of its
+// cluster, 1 to 2 us each with what lies between, and the slowest row holds up the
+// rest (64 rows, all of one kind: greedy 10 us, min-p 13, temperature alone 23,
+// top-k 29, both limits 34, top-p 62).  One row takes 16 us in 16 blocks.
 constexpr int kPivots = 5;
 constexpr float kFirst = 2.5F;
 constexpr int kMaxCluster = 16;  // more than 8 need the kernel's consent (launch_cluster)
@@ -517,13 +517,12 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
     // Pivot i of n, falling, for the next try in (lo, hi).  They split the range evenly:
     // by value while it is wide (by key, a range about 0 is almost all tiny
     // numbers), by key once it is narrow.
-    auto next_pivot = [&](uint32_t lo, uint32_t hi, int tries, int i, int n) {
+    auto next_pivot = [&](uint32_t lo, uint32_t hi, int tries, int i, uint32_t share) {  // share: 2^32 / (n + 1)
         const float x_hi = K::value(min(hi, top)), x_lo = fmaxf(K::value(lo), m - 30.F * t);
-        const float step = (x_hi - x_lo) / (n + 1);
-        const uint64_t span = hi - lo;
-        const bool by_value = tries < 3 && step > 0.F && step < 1.0e30F;
-        const uint32_t key =
-            by_value ? K::near(x_hi - step * (i + 1)) : hi - static_cast<uint32_t>(span * (i + 1) / (n + 1));
+        const uint32_t part = share * static_cast<uint32_t>(i + 1);
+        const float below = (x_hi - x_lo) * (static_cast<float>(part) * 2.3283064e-10F);
+        const bool by_value = tries < 3 && below > 0.F && below < 1.0e30F;
+        const uint32_t key = by_value ? K::near(x_hi - below) : hi - __umulhi(hi - lo, part);
         return max(min(key, hi - 1), lo + 1);
     };
     // The search: the largest key whose entries at or above it reach a target (in
@@ -538,9 +537,10 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
     auto finish = [&](auto by_mass, uint32_t& lo, uint32_t hi, int64_t base, int at_lo, int at_hi, int64_t& above,
                       int64_t target) {
         const int pivots = 2 * (threads >> 5);
+        const uint32_t share = 0xffffffffu / static_cast<uint32_t>(pivots + 1);
         for (int tries = 0; hi - lo > 1 && at_lo - at_hi > 1; ++tries) {
-            const uint32_t p0 = next_pivot(lo, hi, tries, 2 * warp, pivots);
-            const uint32_t p1 = next_pivot(lo, hi, tries, 2 * warp + 1, pivots);
+            const uint32_t p0 = next_pivot(lo, hi, tries, 2 * warp, share);
+            const uint32_t p1 = next_pivot(lo, hi, tries, 2 * warp + 1, share);
             int64_t m0 = 0, m1 = 0;
             int c0 = 0, c1 = 0;
             for (int i = lane; i < listed; i += 32) {
@@ -573,11 +573,11 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
             const int at = reach != 0 ? __ffs(reach) - 1 : pivots;
             const uint32_t was_lo = lo, was_hi = hi;
             if (at < pivots) {
-                lo = next_pivot(was_lo, was_hi, tries, at, pivots);
+                lo = next_pivot(was_lo, was_hi, tries, at, share);
                 at_lo = static_cast<int>(counts[at]);
             }
             if (at > 0) {
-                hi = next_pivot(was_lo, was_hi, tries, at - 1, pivots);
+                hi = next_pivot(was_lo, was_hi, tries, at - 1, share);
                 at_hi = static_cast<int>(counts[at - 1]);
                 above = base + sums[at - 1];
             }
@@ -617,8 +617,9 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
         if (warp == 0) {
             // The first try: every kFirst temperatures below the maximum, which is where a
             // nucleus of ordinary logits tends to end.  Five keys that far apart, means of
-            // four seeds (64 rows of 16 bits, 333 of 32): 60 and 103 us; four, 3 apart: 64
-            // and 108; at 1.5, 3.5, 6, 9, 13: 66 and 110; six, to 14: 65 and 107.
+            // four seeds (64 rows of 16 bits, 333 of 32), when the rest was slower: 60 and
+            // 103 us; four, 3 apart: 64 and 108; at 1.5, 3.5, 6, 9, 13: 66 and 110; six, to
+            // 14: 65 and 107.
             // (with lo == top no key lies between: every pivot is top + 1, where nothing is)
             if (lane < kPivots) sh.pv[lane] = max(min(K::near(m - kFirst * (lane + 1) * t), top), lo + 1);
             if (lane == 0) {
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
                 // (entries of the blocks before this one)
                 const int before = static_cast<int>(
                     __reduce_add_sync(0xffffffffu, static_cast<unsigned>(lane < static_cast<int>(rank) ? own : 0)));
-                const uint32_t pivot = next_pivot(new_lo, new_hi, tries, lane, kPivots);
+                const uint32_t pivot = next_pivot(new_lo, new_hi, tries, lane, 0xffffffffu / (kPivots + 1));
                 __syncwarp();
                 if (lane < kPivots) sh.pv[lane] = pivot;
                 if (lane == 0) {
@@ -941,7 +942,8 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
 constexpr int kSampleSmem = 200 * 1024;  // the largest slice of a row
 
 // One row to `cluster` blocks of `threads`: the kernel's 64 registers leave 1024
-// threads an SM, which the blocks that are resident together share.
+// threads an SM, which the blocks that are resident together share (blocks of up
+// to 2048 threads in all, in two turns: 64 rows 50 us for 47, 333 rows 102 for 88).
 template <int DT>
 cudaError_t launch_cluster(const SampleArgs& a, int cluster, cudaStream_t s) {
     using K = Keys<DT>;
@@ -979,14 +981,18 @@ cudaError_t launch_cluster(const SampleArgs& a, int cluster, cudaStream_t s) {
 cudaError_t sample_rows(const SampleArgs& a, int dt, cudaStream_t s) {
     if (a.rows == 0) return cudaSuccess;
     const int64_t bytes = static_cast<int64_t>(a.vocab) * (dt == kF32 ? 4 : 2) + 16;
+    // 16 blocks a row while that is one an SM: 1 row of 304 KB 26 us for 28 in 8, 9 rows 28 for 35; 64 rows 89 for 87
     int cluster = static_cast<int64_t>(a.rows) * kMaxCluster <= device_sm_count() ? kMaxCluster : 8;
-    // fewer blocks a row once the rows fill the SMs by themselves, but no slice over 56 KB (three blocks an SM)
+    // fewer blocks a row once the rows fill the SMs by themselves, but no slice over 56 KB (three blocks an SM):
+    // 333 rows of 201 KB 88 us in 4 blocks, 90 in 8, 110 in 2
     while (cluster > 1 && static_cast<int64_t>(a.rows) * cluster > 4 * device_sm_count() &&
            bytes / (cluster / 2) <= 56 * 1024)
         cluster >>= 1;
-    // and none so small that its barrier costs more than its share of the row
+    // and none so small that its barrier costs more than its share of the row: 300 rows of 2 KB 23 us in 1 block,
+    // 28 in 4, 49 in 8; of 64 KB 83 in 4, 87 in 8
     while (cluster > 1 && bytes / cluster < 4096) cluster >>= 1;
     if (bytes / cluster + 16 > kSampleSmem) {  // longer than a cluster holds
+        // (this way 152 000 logits take 1.7 ms: a pass over memory for every bit of a key)
         auto kernel = dt == kBF16 ? sample_rows_kernel<kBF16> : dt == kF16 ? sample_rows_kernel<kF16> : sample_rows_kernel<kF32>;
         return launch_pdl(kernel, dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, s, a);
     }
