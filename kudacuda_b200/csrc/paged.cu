@@ -54,7 +54,7 @@ __device__ __forceinline__ uint4 pack8(const float* x) {
 // of heads with the unit's eight cos and sin in registers, all their loads in flight
 // at once.  Bound by memory: 8192 rows of 32 + 16 heads, every element read and
 // written once, 5.6 TB/s; few rows by the chain of loads from the lengths to
-// the page number (64 rows: 3 us).
+// the page number (64 rows of 16 + 4 heads: 3 us).
 constexpr int kRopeThreads = 128;
 // Warps from which four groups of heads share one: 32 + 16 heads of 128 dims, four
 // against one: 16 rows 3.3 and 2.7 us, 256 rows 3.8 and 3.8, 1024 6.2 and 7.2,

@@ -16,7 +16,27 @@
 // Warps: 0-3 and 4-7 softmax, tile 0 and 1; 8 K/V producer (TMA, one box per
 // page and 64 dims, 128-byte swizzle); 9 MMA issuer; 10 fetches Q and clears the
 // rows of the last V block past the item's last key (their P is 0, but 0 times
-// a NaN in an unused slot is not); 11 only writes the record of this worker's cut items.
+// a NaN in an unused slot is not); 11 only writes the record of the item that goes
+// on into this stretch.
+//
+// P is rounded to the cache's type because that is what the matrix instruction
+// takes (its error, half a step of the type, is that of the output's own rounding;
+// sum and maximum are of the unrounded values).  The two tiles take turns: while
+// one's scores are exponentiated the other's products run, and the first half of
+// P multiplies while the second is made.  Two tiles fill the tensor memory (S 2 x
+// 128, O 2 x 128 columns).
+//
+// Measured, 4 prompts of 2048 tokens of 16 heads over 8192 keys (2 key heads of 128
+// bf16 dims; 0.48 Tflop): 374 us on a cool card, 1.29 Pflop/s (the library's
+// largest product: 1.63), and 432 us after a second of it, when the power limit
+// brings the clocks down (1.11, the library's product: 1.36).  A step of both
+// tiles takes 3550 clocks, of which the products could use 2048; the rest is the
+// chain from a score to its product with V (load from tensor memory 60, maximum
+// 300, exponentials and stores 1250) and six barrier waits of about 180.  Without
+// exponentials it takes as long, without any arithmetic on the scores 3300.
+// What did not help: blocks of 64 keys with doubled scores (652 us where this took
+// 432), part of the exponentials by polynomial, exponentials before the maximum
+// is known, one arrival a warp instead of one a thread, waiting by polling.
 #include <cuda_bf16.h>
 
 #include "kc_common.cuh"
@@ -32,7 +52,9 @@ namespace {
 constexpr int kRows = 256;   // query rows of an item
 constexpr int kKeys = 128;   // keys of a block
 constexpr int kThreads = 384;
-constexpr int kOver = 384;   // an item's start and end cost about as much as these keys
+// An item's start and end cost about as much as these keys: eight ragged batches
+// together 443 us, with 256 469, with 512 440.
+constexpr int kOver = 384;
 constexpr int kLeast = 128;
 constexpr float kLazy = 8.F;  // how far the true maximum may exceed m
 

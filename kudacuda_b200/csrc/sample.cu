@@ -382,7 +382,8 @@ __device__ __forceinline__ uint32_t cluster_max(SampleShared& sh, int& turn, uin
         if (lane < static_cast<int>(ranks)) store_remote(&sh.from[turn][0][cluster_rank()], lane, v);
     }
     cluster_barrier();
-    return __reduce_max_sync(0xffffffffu, lane < static_cast<int>(ranks) ? static_cast<uint32_t>(sh.from[turn][0][lane]) : 0u);
+    v = lane < static_cast<int>(ranks) ? static_cast<uint32_t>(sh.from[turn][0][lane]) : 0u;
+    return __reduce_max_sync(0xffffffffu, v);
 }
 
 // rint(2^38 w) of a w in [0, 1] as 2^19 hi + lo: adding 2^23 (1.5 2^23) leaves a
@@ -982,7 +983,9 @@ cudaError_t sample_rows(const SampleArgs& a, int dt, cudaStream_t s) {
     if (a.rows == 0) return cudaSuccess;
     const int64_t bytes = static_cast<int64_t>(a.vocab) * (dt == kF32 ? 4 : 2) + 16;
     // 16 blocks a row while that is one an SM: 1 row of 304 KB 26 us for 28 in 8, 9 rows 28 for 35; 64 rows 89 for 87
-    int cluster = static_cast<int64_t>(a.rows) * kMaxCluster <= device_sm_count() ? kMaxCluster : 8;
+    // (and where 8 cannot hold it)
+    const bool wide = static_cast<int64_t>(a.rows) * kMaxCluster <= device_sm_count() || bytes / 8 + 16 > kSampleSmem;
+    int cluster = wide ? kMaxCluster : 8;
     // fewer blocks a row once the rows fill the SMs by themselves, but no slice over 56 KB (three blocks an SM):
     // 333 rows of 201 KB 88 us in 4 blocks, 90 in 8, 110 in 2
     while (cluster > 1 && static_cast<int64_t>(a.rows) * cluster > 4 * device_sm_count() &&
@@ -993,7 +996,9 @@ cudaError_t sample_rows(const SampleArgs& a, int dt, cudaStream_t s) {
     while (cluster > 1 && bytes / cluster < 4096) cluster >>= 1;
     if (bytes / cluster + 16 > kSampleSmem) {  // longer than a cluster holds
         // (this way 152 000 logits take 1.7 ms: a pass over memory for every bit of a key)
-        auto kernel = dt == kBF16 ? sample_rows_kernel<kBF16> : dt == kF16 ? sample_rows_kernel<kF16> : sample_rows_kernel<kF32>;
+        auto kernel = dt == kBF16  ? sample_rows_kernel<kBF16>
+                      : dt == kF16 ? sample_rows_kernel<kF16>
+                                   : sample_rows_kernel<kF32>;
         return launch_pdl(kernel, dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, s, a);
     }
     return dt == kBF16 ? launch_cluster<kBF16>(a, cluster, s) : dt == kF16 ? launch_cluster<kF16>(a, cluster, s)
