@@ -419,12 +419,20 @@ def test_sample_against_the_definition(bridge, dtype, vocab):
 
 @pytest.mark.parametrize("dtype,vocab", [(torch.float32, 450001), (BF16, 900003), (F16, 151937)])
 def test_sample_long_rows(bridge, dtype, vocab):
-    """Rows longer than a cluster's shared memory among them."""
+    """Rows of several hundred words a thread, odd lengths, every alignment of a row."""
 
     g = torch.Generator().manual_seed(vocab)
     x = (3.0 * torch.randn((4, vocab), generator=g)).to(dtype).to(DEV)
     u = torch.rand((4,), generator=g).tolist()
     check_rows(bridge, x, u, [0.0, 0.7, 1.0, 0.9], [0, 50, 0, 7], [1.0, 0.9, 0.99, 1.0], [0.0, 0.01, 0.0, 0.1])
+
+
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 900001), (BF16, 1700001)])
+def test_sample_rows_longer_than_sixteen_blocks_hold(bridge, dtype, vocab):
+    g = torch.Generator().manual_seed(vocab)
+    x = (3.0 * torch.randn((3, vocab), generator=g)).to(dtype).to(DEV)
+    u = torch.rand((3,), generator=g).tolist()
+    check_rows(bridge, x, u, [0.0, 0.7, 0.25], [0, 50, 0], [1.0, 0.9, 0.9], [0.0, 0.01, 0.0])
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
