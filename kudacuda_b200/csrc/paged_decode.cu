@@ -117,6 +117,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_wait_on_producer();
     const int group = p.q_heads / p.kv_heads;
     const int worker = blockIdx.x;
+    // (an item's rows are few: exact without an integer division)
+    const float per_token = __frcp_rn(static_cast<float>(group));
+    auto token_of = [&](int row) { return static_cast<int>((static_cast<float>(row) + 0.5F) * per_token); };
     const PagedShares shares =
         paged_place<W, kLeast, kThreads>(p, group, worker, gridDim.x, sums, &place_seq, &place_at);
     W w;  // (thread 0's)
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Piece& e = list[ahead];
             const int r = lane & 15;
             if (r < e.rows) {
-                const int token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
+                const int token = token_of(e.r0 + r), head = (e.r0 + r) - token * group;
                 const uint16_t* q = static_cast<const uint16_t*>(a.q) + (e.start + token) * a.q_stride +
                                     static_cast<int64_t>(e.kvh * group + head) * D + (lane >> 4) * (D / 2);
                 asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (first < e.t1) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int r = g + 8 * h, token = (e.r0 + r) / group, head = (e.r0 + r) - token * group;
+                    const int r = g + 8 * h, token = token_of(e.r0 + r), head = (e.r0 + r) - token * group;
                     const bool live = r < e.rows;
                     const uint16_t* q = static_cast<const uint16_t*>(a.q) +
                                         (live ? (e.start + token) * a.q_stride +
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     x.w += y.w;
                 }
                 if (e.whole) {
-                    const int token = (e.r0 + r) / group;
+                    const int token = token_of(e.r0 + r);
                     const int64_t row = e.start + token;
                     const int head = e.kvh * group + (e.r0 + r) - token * group;
                     const float inv = sum == 0.F ? 0.F : 1.F / sum;

@@ -45,7 +45,7 @@ struct PagedShares {
     int workers;
     // No more workers than there is work for: about `least` keys a worker.
     __device__ __forceinline__ void set(int64_t total, int group, int least, int most) {
-        const float w = static_cast<float>(total) / (static_cast<float>(group) * static_cast<float>(least));
+        const float w = __fdividef(static_cast<float>(total), static_cast<float>(group) * static_cast<float>(least));
         workers = w < static_cast<float>(most) ? max(static_cast<int>(w), 1) : most;
         size = paged_div(total, workers);
         rest = total - size * workers;
@@ -136,14 +136,14 @@ struct PagedWalk {
         kvh = next_kvh;
         q = next_q;
         item_rows = min(ROWS, rows - q * ROWS);
-        const int last_token = (q * ROWS + item_rows - 1) / group;
+        const int last_token = q == tiles_q - 1 ? n - 1 : (q * ROWS + ROWS - 1) / group;
         limit = min(max(len - n + last_token + 1, 0), p.table_width * p.page_size);
         tiles = max((limit + KT - 1) / KT, 1);
         return lo;
     }
     // the item's block in which x lies (the same expression on both sides of a cut, so the two agree)
     __device__ __forceinline__ int block_of(int64_t x, int64_t lo) const {
-        const float each = static_cast<float>(tiles) / static_cast<float>(item_end - lo);
+        const float each = __fdividef(static_cast<float>(tiles), static_cast<float>(item_end - lo));
         return x <= lo ? 0 : x >= item_end ? tiles : min(tiles, static_cast<int>(static_cast<float>(x - lo) * each));
     }
     // the next piece with a block in it
