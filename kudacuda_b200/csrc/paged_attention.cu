@@ -17,10 +17,12 @@ namespace kc {
 // serves: its tile, for a second one it reads the cache again.  It also keeps the
 // probabilities to twice the type's precision.  Decode and chunk kernel, us, 4
 // key heads of 128 bf16 dims, 1 token of 8 heads / 2 / 3:
-//   64 sequences of 500 keys    25.8, 27.6 / 28.8, 27.9 / 42.4, 28.2
-//   16 of 2000                  22.9, 23.9 / 24.8, 24.1 / 32.7, 24.5
-//   1 of 8000                   15.1, 17.8 / 15.8, 18.0 / 19.7, 18.4
-//   2 of 100000                 74.4, 79.8 / 75.9, 80.5 / 135, 81.1
+//   64 sequences of 500 keys    25.5, 26.2 / 28.4, 26.4 / 41.6, 26.5
+//   16 of 2000                  22.9, 23.3 / 24.6, 23.4 / 32.8, 23.5
+//   1 of 8000                   15.0, 17.2 / 15.8, 17.5 / 19.6, 17.7
+//   2 of 100000                 74.5, 77.5 / 76.3, 78.2 / 136, 78.4
+// (two tokens of eight heads are 16 rows: 5 to 8% lost on short caches, 3 to 10%
+// won on long ones, and the probabilities)
 constexpr int64_t kDecodeRows = 16;
 
 int64_t paged_attention_workspace_bytes(int64_t batch, int64_t rows, int64_t max_query, int64_t q_heads,

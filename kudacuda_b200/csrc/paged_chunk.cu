@@ -53,9 +53,9 @@ constexpr int kRows = 256;   // query rows of an item
 constexpr int kKeys = 128;   // keys of a block
 constexpr int kThreads = 384;
 // An item's start and end cost about as much as these keys: eight ragged batches
-// together 443 us, with 256 469, with 512 440.
+// together 414 us, with 256 430, with 512 416.
 constexpr int kOver = 384;
-constexpr int kLeast = 128;
+constexpr int kLeast = 128;  // (96, 192 and 256: within 3% on 24 batches, none better throughout)
 constexpr float kLazy = 8.F;  // how far the true maximum may exceed m
 
 template <int D>
@@ -527,7 +527,8 @@ cudaError_t launch_chunk(const PagedAttentionArgs& a, cudaStream_t s) {
     if (st != cudaSuccess) return st;
     // Blocks of the join: with about a full item of 256 rows for every two workers
     // four a worker (24 ragged sequences of 39 tokens each, 32 heads: 64.8 us in all,
-    // with two 66.2), else two (4 tokens of 8 heads over 100: 11.1 us, with four 11.8).
+    // with two 66.2, when the rest was slower), else two (4 tokens of 8 heads over 100:
+    // 11.1 us, with four 11.8).
     const int ways = static_cast<int64_t>(p.rows) * p.q_heads >= workers * (kRows / 2) ? 4 : 2;
     return launch_pdl(paged_join_kernel<DT, D, kRows, false>, dim3(workers, ways), dim3(kJoinThreads), 0, s, a);
 }

@@ -38,8 +38,11 @@ constexpr int kRows = 16;
 constexpr int kKeys = 16;
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kOver = 384;            // an item's start and end cost about as much as these keys
-constexpr int kLeast = 192;           // a worker has a block or so for every warp
+// An item's start and end cost about as much as kOver keys, and a worker has kLeast
+// or more, a block or so for every warp.  Thirteen batches together 377 us; with
+// kLeast 320 or 448 381 and 383, with both 128 380, both 256 381.
+constexpr int kOver = 384;
+constexpr int kLeast = 192;
 
 template <int D>
 struct DecodeSmem {
