@@ -209,19 +209,20 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
 //
 // The logits are read once, so memory asks 3 us of 64 rows of 151 936 16-bit
 // logits and 10 us of 333 rows of 50 257 32-bit ones.  What they do cost, rows of
-// all kinds mixed, 47 and 88 us, is instructions in the first try and in the pass
-// in index order (an exponential and two roundings an entry, three additions more
-// for every key tried), and waits: a row goes through six or so barriers of its
-// cluster, 1 to 2 us each with what lies between, and the slowest row holds up the
-// rest (64 rows, all of one kind: greedy 10 us, min-p 13, temperature alone 23,
-// top-k 29, both limits 34, top-p 62).  One row takes 16 us in 16 blocks.
+// all kinds mixed, is 47 to 60 and 88 to 97 us, depending on the rows: instructions
+// in the first try and in the pass in index order (an exponential and two roundings
+// an entry, three additions more for every key tried), and waits: a row goes
+// through six or so barriers of its cluster, 1 to 2 us each with what lies between,
+// and the slowest row holds up the rest (64 rows, all of one kind: greedy 10 us,
+// min-p 14, temperature alone 23, top-k 29, both limits 34, top-p 64).  One row
+// takes 16 us in 16 blocks.
 constexpr int kPivots = 5;
 constexpr float kFirst = 2.5F;
 constexpr int kMaxCluster = 16;  // more than 8 need the kernel's consent (launch_cluster)
 constexpr int kMaxSampleThreads = 512;
 constexpr int kList = 1024;
-constexpr int kBins = 256;
-static_assert(3 * kBins <= kList && kBins % kMaxCluster == 0);
+constexpr int kBins = 512;  // (256: 64 rows 53.4 us for 52.3, mean of eight seeds)
+static_assert(2 * kBins <= kList && kBins % kMaxCluster == 0);
 
 template <int DT>
 struct Keys {
@@ -744,14 +745,14 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
             const int at_hi = everything ? sh.at_hi : 0;
             finish(by_mass, lo, hi, everything ? 0 : above, listed, at_hi, above, target);
         } else if (hi - lo > 1) {
-            // Many entries of few keys (16-bit types): counters, one a key, in the place of
-            // the list.  Block i adds up the keys number i, i + ranks, ... of all blocks
+            // Many entries of few keys (16-bit types): counters, one a key, in the places of
+            // the list and its masses.  Block i adds up the keys number i, i + ranks, ... of all blocks
             // and tells them.
             const uint32_t span = hi - lo;
             const int per = kBins / static_cast<int>(ranks);
             uint32_t* const bin = sh.list;
             uint32_t* const got = sh.list + kBins;
-            uint32_t* const sum = sh.list + 2 * kBins;
+            uint32_t* const sum = sh.own;
             for (int i = tid; i < kBins; i += threads) bin[i] = 0;
             __syncthreads();
             hits(lo, hi, [&](uint32_t k) { atomicAdd(&bin[k - lo], 1u); });
@@ -769,28 +770,29 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
             cluster_barrier();
             // every warp: a lane has kBins / 32 keys in a row, the highest first
             constexpr int kEach = kBins / 32;
-            int64_t x[kEach], mine_sum = 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const uint32_t back = lane * kEach + i;  // keys below hi - 1
-                x[i] = back < span ? static_cast<int64_t>(sum[span - 1 - back]) : 0;
-                if constexpr (by_mass)
-                    if (x[i] != 0) x[i] *= mass(hi - 1 - back);
-                mine_sum += x[i];
-            }
+            auto part = [&](uint32_t back) {  // of the key that many below hi - 1
+                const int64_t x = back < span ? static_cast<int64_t>(sum[span - 1 - back]) : 0;
+                if constexpr (by_mass) return x * mass(hi - 1 - min(back, span - 1));
+                else return x;
+            };
+            int64_t mine_sum = 0;
+#pragma unroll 4
+            for (int i = 0; i < kEach; ++i) mine_sum += part(lane * kEach + i);
             const int64_t upto = warp_scan64(mine_sum);
             const unsigned reach = __ballot_sync(0xffffffffu, above + upto >= target);
             const int at = reach != 0 ? __ffs(reach) - 1 : 31;  // (lo reaches the target, so some lane does)
             int64_t c = above + upto - mine_sum;
             uint32_t found = lo;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const uint32_t back = lane * kEach + i;
-                if (found == lo && back + 1 < span) {
-                    if (c + x[i] >= target) found = hi - 1 - back;
-                    else c += x[i];
+            if (lane == at) {
+                for (int i = 0; i < kEach && found == lo; ++i) {
+                    const uint32_t back = lane * kEach + i;
+                    if (back + 1 >= span) break;
+                    const int64_t x = part(back);
+                    if (c + x >= target) found = hi - 1 - back;
+                    else c += x;
                 }
             }
+            __syncwarp();
             lo = __shfl_sync(0xffffffffu, found, at);
             above = __shfl_sync(0xffffffffu, c, at);
             __syncthreads();
