@@ -600,8 +600,9 @@ KUDACUDA_API int kudacuda_sm100_gqa_decode_batch(void* handle, uint64_t query, u
  *   rint(2^38 exp((x - max) / T)): the result does not depend on the batch.
  *   Order (value descending, index ascending): top-k, then the shortest prefix
  *   of mass >= top_p, then exp(..) >= min_p; drawn in order of index.
- *   temperature <= 0: the lowest index of the maximum.  NaN counts as -inf; a
- *   row with nothing above -inf gives -1. */
+ *   temperature <= 0: the lowest index of the maximum; infinite: every finite
+ *   logit is as likely as any other.  NaN counts as -inf; a row with nothing
+ *   above -inf gives -1. */
 KUDACUDA_API int kudacuda_sm100_rope_append_paged(void* handle, int dtype, uint64_t qkv, int64_t qkv_stride,
                                                   uint64_t bias, uint64_t q_out, int64_t q_stride, uint64_t k_pages,
                                                   uint64_t v_pages, uint64_t rope_cos, uint64_t rope_sin,

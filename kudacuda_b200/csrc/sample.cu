@@ -3,6 +3,7 @@
 //
 // With x the logits in 32 bits (NaN counts as -inf) and m their maximum:
 //   w_i = 1 where x_i == m, else exp((x_i - m) * (1 / T));  W_i = rint(2^38 w_i)
+// (an infinite T: w_i = 1 for every finite x_i, 0 for -inf).
 // The masses W are whole numbers, so every sum below is exact and does not
 // depend on the order in which threads or blocks add: the same row gives the
 // same token whatever shares its batch.  In the order of (x descending, index
@@ -30,6 +31,11 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
     const float x = load_elem<DT>(p, i) + 0.F;  // -0 and +0 are one value
     return x != x ? -INFINITY : x;
 }
+
+// 1 / T, never 0: for an infinite T the smallest 32-bit number stands for it, by
+// which x - m of a finite entry becomes about 0 (weight 1: the draw is uniform) and
+// that of a -inf stays -inf (weight 0), where 0 would make it NaN.
+__device__ __forceinline__ float inverse_temperature(float t) { return fmaxf(1.F / t, 1.4e-45F); }
 
 template <typename T, typename F>
 __device__ __forceinline__ T block_reduce(T v, F f, T* buf) {
@@ -76,7 +82,7 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
         }
         return;
     }
-    const float inv = 1.F / t;
+    const float inv = inverse_temperature(t);
     auto weight = [&](float x) { return x == m ? 1.F : expf((x - m) * inv); };
     auto mass = [&](float x) { return __float2ll_rn(weight(x) * kMassOne); };
     // kept: key > cut, or key == cut and index < tie_end
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
         cluster_barrier();
         return;
     }
-    const float inv = 1.F / t;
+    const float inv = inverse_temperature(t);
     // (written so that nothing branches: a branch an entry, over the exponential or
     // over the sums of a pivot, made 64 rows 60 us instead of 53)
     auto weight = [&](uint32_t k) {

@@ -452,6 +452,26 @@ def test_sample_ties_infinities_and_nan(bridge, dtype):
     check_rows(bridge, torch.tensor(rows, dtype=torch.float64).to(dtype).to(DEV), us, *cols)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 70), (BF16, 5001), (F16, 40000), (BF16, 1700001)])
+def test_sample_infinite_temperature(bridge, dtype, vocab):
+    """Every entry above -inf is as likely as any other; masked ones and NaN are never drawn."""
+
+    g = torch.Generator().manual_seed(vocab)
+    rows = 8 if vocab < 10000 else 4
+    x = 3.0 * torch.randn((rows, vocab), generator=g)
+    masked = torch.rand((rows, vocab), generator=g) < 0.6
+    x = torch.where(masked, -math.inf, x)
+    x[1::4, ::7] = math.nan
+    x[2::4, 0] = math.inf
+    x[3::4, 1:] = -math.inf  # one entry is left
+    x[3::4, 0] = 2.0
+    u = torch.rand((rows,), generator=g).tolist()
+    x = x.to(dtype).to(DEV)
+    settings = [(0, 0.5, 0.0), (0, 1.0, 0.0), (9, 1.0, 0.0), (vocab - 1, 0.9, 0.5), (0, 1.0, 1.0)]
+    for k, p, low in settings if vocab < 100000 else settings[:1]:
+        check_rows(bridge, x, u, [math.inf] * rows, [k] * rows, [p] * rows, [low] * rows)
+
+
 def test_sample_values_of_every_size(bridge):
     """bf16 values that few entries share, near 0, past 128 and far below, beside ordinary ones."""
 
