@@ -14,6 +14,7 @@ the model - the batched path's NF4 GEMMs, ``rope_append_paged``,
 from __future__ import annotations
 
 import argparse
+import contextlib
 import heapq
 import json
 import math
@@ -77,11 +78,25 @@ class PagedKVCache:
         if self._refs[page] == 0:
             heapq.heappush(self._free, page)
 
-    def _copy(self, pairs: list[tuple[int, int]], stream_ptr: int, **tables: Any) -> None:
+    def _copy(self, pairs: list[tuple[int, int]], stream_ptr: int, block_table: Any = None) -> None:
+        """Copies the pages and, with ``block_table``, points its entries at the copies."""
+
         torch = self.torch
-        self.bridge.dispatch_kv_pages_copy(self.k, self.v,
-                                           torch.tensor(pairs, dtype=torch.int32, device=self.device).view(-1, 2),
-                                           stream_ptr=stream_ptr, **tables)
+        # The lists are dropped once the copy is launched: memory of its own stream is not handed out
+        # to anyone who would write it earlier.
+        on_stream = contextlib.nullcontext()
+        if torch.device(self.device).type == "cuda":
+            on_stream = torch.cuda.stream(torch.cuda.ExternalStream(stream_ptr, device=self.device))
+        with on_stream:
+            i32 = dict(dtype=torch.int32, device=self.device)
+            tables = {}
+            if block_table is not None:
+                page_map = list(range(self.num_pages))
+                for old, new in pairs:
+                    page_map[old] = new
+                tables = {"block_table": block_table, "page_map": torch.tensor(page_map, **i32)}
+            self.bridge.dispatch_kv_pages_copy(self.k, self.v, torch.tensor(pairs, **i32).view(-1, 2),
+                                               stream_ptr=stream_ptr, **tables)
 
     def reserve(self, growth: Sequence[tuple[PagedSequence, int]], stream_ptr: int) -> None:
         """Room for each sequence's new tokens, whose lengths grow by them; all of them or none."""
@@ -138,7 +153,6 @@ class PagedKVCache:
         (a fork's pages are moved once), ``block_table`` a device table to rewrite too.  Returns the
         number of pages moved."""
 
-        torch = self.torch
         used = [p for p in range(self.num_pages) if self._refs[p] > 0]
         known = {p for s in sequences for p in s.pages}
         if known != set(used):
@@ -148,13 +162,7 @@ class PagedKVCache:
         if not pairs:
             return 0
         to = dict(pairs)
-        tables: dict[str, Any] = {}
-        if block_table is not None:
-            page_map = torch.arange(self.num_pages, dtype=torch.int32)
-            for old, new in pairs:
-                page_map[old] = new
-            tables = {"block_table": block_table, "page_map": page_map.to(self.device)}
-        self._copy(pairs, stream_ptr, **tables)
+        self._copy(pairs, stream_ptr, block_table)
         for seq in sequences:
             seq.pages = [to.get(p, p) for p in seq.pages]
         for old, new in pairs:

@@ -113,3 +113,49 @@ def test_step_refuses(setup):
     with pytest.raises(PagedCacheFull):
         gen.cache.reserve([(s, 64 * 16 + 1)], 0)
     assert s.length == 0 and gen.cache.free_pages == 64
+
+
+def test_cache_copies_on_another_stream(setup):
+    """reserve and compact on a stream that is held up, while the current stream goes on taking memory."""
+
+    from kudacuda_b200.paged_serving import PagedKVCache, PagedSequence
+
+    bridge, _, _ = setup
+    cache = PagedKVCache(bridge, layers=3, num_pages=24, kv_heads=2, head_dim=64, page_size=16, device=DEV)
+    seqs = [PagedSequence() for _ in range(4)]
+    cache.reserve([(s, 40) for s in seqs], 0)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    cache.k.copy_(torch.randn(cache.k.shape, generator=g, device=DEV))
+    cache.v.copy_(torch.randn(cache.v.shape, generator=g, device=DEV))
+
+    def contents(sequences):
+        rows = []
+        for s in sequences:
+            pages = torch.tensor(s.pages, device=DEV)
+            for x in (cache.k, cache.v):
+                rows.append(x[:, pages].permute(0, 2, 1, 3, 4).flatten(2, 3)[:, :, :40].clone())
+        return rows
+
+    forks = [cache.fork(seqs[i]) for i in (1, 3)]
+    alive = [seqs[1], seqs[3], *forks]
+    want = contents(alive)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for what in ("reserve", "compact"):
+        if what == "compact":
+            cache.free(seqs[0])
+            cache.free(seqs[2])
+        table = torch.tensor(cache.table(alive), dtype=torch.int32, device=DEV)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        if what == "reserve":
+            cache.reserve([(f, 1) for f in forks], side.cuda_stream)
+        else:
+            assert cache.compact(alive, side.cuda_stream, block_table=table) > 0
+        keep = [torch.full((n,), 5, dtype=torch.int32, device=DEV) for n in (1, 2, 4, 16, 24, 48) for _ in range(20)]
+        torch.cuda.synchronize()
+        assert bridge.error_word(clear=True) == 0 and keep
+        assert all(torch.equal(x, y) for x, y in zip(contents(alive), want))
+        if what == "compact":
+            assert table.tolist() == cache.table(alive)

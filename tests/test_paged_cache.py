@@ -160,6 +160,63 @@ def test_compaction_keeps_every_sequence_and_rewrites_tables():
     assert cache.free_pages == 12
 
 
+class StreamedTorch:
+    """torch whose tensors stay on the host; notes which stream is current as each one is made."""
+
+    def __init__(self):
+        self.current, self.made = 7, []
+        self.cuda = SimpleNamespace(ExternalStream=lambda ptr, device=None: ptr, stream=self._use)
+
+    def _use(self, stream):
+        import contextlib
+
+        @contextlib.contextmanager
+        def use():
+            self.current, before = stream, self.current
+            try:
+                yield
+            finally:
+                self.current = before
+
+        return use()
+
+    def _maker(self, make):
+        def made(*args, device=None, **kw):
+            out = make(*args, **kw)
+            self.made.append((self.current, out.data_ptr()))
+            return out
+        return made
+
+    def __getattr__(self, name):
+        value = getattr(torch, name)
+        return self._maker(value) if name in ("tensor", "arange", "zeros") else value
+
+
+def test_copies_use_memory_of_the_stream_they_run_on():
+    """The lists of a copy go back to the allocator as soon as it is launched, so they must come from the
+    stream that it runs on: another one could take their memory while the copy still reads them."""
+
+    class Streamed(Copier):
+        def dispatch_kv_pages_copy(self, k, v, pairs, *, stream_ptr, block_table=None, page_map=None):
+            lists = [t.data_ptr() for t in (pairs, page_map) if t is not None]
+            streams.append([{p: s for s, p in fake.made}[p] for p in lists])
+            assert stream_ptr == 99
+            super().dispatch_kv_pages_copy(k, v, pairs, stream_ptr=stream_ptr, block_table=block_table, page_map=page_map)
+
+    fake, streams = StreamedTorch(), []
+    cache = PagedKVCache(Streamed(), layers=1, num_pages=8, kv_heads=1, head_dim=4, page_size=16, dtype=torch.float32,
+                         device="cuda:0", torch_module=fake)
+    a, b = PagedSequence(), PagedSequence()
+    cache.reserve([(a, 5), (b, 40)], 99)
+    f = cache.fork(b)
+    cache.reserve([(f, 1)], 99)
+    assert streams == [[99]]
+    cache.free(a)
+    table = torch.tensor(cache.table([b, f]), dtype=torch.int32)
+    assert cache.compact([b, f], 99, block_table=table) == 1
+    assert streams == [[99], [99, 99]] and table.tolist() == cache.table([b, f])
+
+
 def test_rope_tables():
     cos, sin = paged_rope_tables(40, 64, 1e4)
     i, pos = 7, 33
