@@ -101,6 +101,8 @@ class PagedKVCache:
     def reserve(self, growth: Sequence[tuple[PagedSequence, int]], stream_ptr: int) -> None:
         """Room for each sequence's new tokens, whose lengths grow by them; all of them or none."""
 
+        if len({id(seq) for seq, _ in growth}) != len(growth):
+            raise ValueError("a sequence grows once in a step: its tokens come together")
         need, copies = 0, []
         for seq, tokens in growth:
             if tokens < 0:

@@ -159,3 +159,15 @@ def test_cache_copies_on_another_stream(setup):
         assert all(torch.equal(x, y) for x, y in zip(contents(alive), want))
         if what == "compact":
             assert table.tolist() == cache.table(alive)
+
+
+def test_step_refuses_a_sequence_named_twice(setup):
+    from kudacuda_b200.paged_serving import PagedSequence, Sampling
+
+    _, _, gen = setup
+    s = PagedSequence()
+    gen.step([(s, [3, 4])], [Sampling()], [0.0])
+    with pytest.raises(ValueError, match="once"):
+        gen.step([(s, [5]), (s, [6])], [Sampling()] * 2, [0.0] * 2)
+    assert s.length == 2
+    gen.cache.free(s)

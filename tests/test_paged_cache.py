@@ -135,6 +135,18 @@ def test_a_full_cache_refuses_and_changes_nothing():
         cache.truncate(a, 21)
 
 
+def test_a_sequence_named_twice_is_refused():
+    """Both entries would get the length with all tokens, and write the same place."""
+
+    cache, copier = make()
+    a, b = PagedSequence(), PagedSequence()
+    grow(cache, a, range(3))
+    with pytest.raises(ValueError, match="once"):
+        cache.reserve([(a, 1), (b, 2), (a, 1)], 0)
+    assert a.length == 3 and b.length == 0 and a.pages == [0] and cache.free_pages == 9 and not copier.calls
+    cache.reserve([(a, 1), (cache.fork(a), 1), (b, 2)], 0)  # equal, but another sequence
+
+
 def test_compaction_keeps_every_sequence_and_rewrites_tables():
     cache, copier = make(num_pages=12)
     seqs = [PagedSequence() for _ in range(4)]
