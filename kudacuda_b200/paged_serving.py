@@ -103,22 +103,23 @@ class PagedKVCache:
 
         if len({id(seq) for seq, _ in growth}) != len(growth):
             raise ValueError("a sequence grows once in a step: its tokens come together")
-        need, copies = 0, []
+        need, copies, owners = 0, [], {}
         for seq, tokens in growth:
             if tokens < 0:
                 raise ValueError("a sequence grows by zero or more tokens")
             need += -(-(seq.length + tokens) // self.page_size) - len(seq.pages)
-            partly = seq.length % self.page_size != 0 and tokens > 0
-            if partly and self._refs[seq.pages[-1]] > 1:
-                copies.append(seq)
-                need += 1
+            if tokens > 0 and seq.length % self.page_size != 0:
+                old = seq.pages[-1]
+                owners[old] = owners.get(old, self._refs[old])
+                if owners[old] > 1:  # (the last owner keeps the original)
+                    owners[old] -= 1
+                    copies.append(seq)
+                    need += 1
         if need > len(self._free):
             raise PagedCacheFull(f"{need} pages are needed, {len(self._free)} are free")
         pairs = []
         for seq in copies:
             old = seq.pages[-1]
-            if self._refs[old] == 1:  # its last other owner copied it just now
-                continue
             seq.pages[-1] = self._take()
             self._refs[old] -= 1
             pairs.append((old, seq.pages[-1]))

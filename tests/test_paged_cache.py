@@ -109,6 +109,37 @@ def test_all_owners_of_a_shared_page_growing_leave_one_with_the_original():
     assert len(copier.calls[0]) == 1 and a.pages != b.pages and cache.free_pages == 8
 
 
+@pytest.mark.parametrize("owners,tokens", [(2, 1), (3, 1), (4, 12)])
+def test_all_owners_grow_into_exactly_the_free_pages(owners, tokens):
+    # each but one copies the page of five tokens; 12 more also start a page each
+    need = owners - 1 + (owners if tokens > 11 else 0)
+    cache, copier = make(num_pages=1 + need)
+    a = PagedSequence()
+    grow(cache, a, range(5))
+    seqs = [a] + [cache.fork(a) for _ in range(owners - 1)]
+    cache.reserve([(s, tokens) for s in seqs], 0)
+    assert cache.free_pages == 0 and len(copier.calls[0]) == owners - 1
+    assert len({p for s in seqs for p in s.pages}) == 1 + need
+    assert all(read(cache, s)[:5] == list(range(5)) for s in seqs)
+    for s in seqs:
+        cache.free(s)
+    assert cache.free_pages == 1 + need
+
+
+def test_one_page_too_few_for_all_owners_changes_nothing():
+    cache, copier = make(num_pages=2)
+    a = PagedSequence()
+    grow(cache, a, range(5))
+    seqs = [a, cache.fork(a), cache.fork(a)]
+    with pytest.raises(PagedCacheFull, match="2 pages are needed, 1 are free"):
+        cache.reserve([(s, 1) for s in seqs], 0)
+    assert all(s.pages == [0] and s.length == 5 for s in seqs) and cache.free_pages == 1 and not copier.calls
+    with pytest.raises(PagedCacheFull):
+        cache.reserve([(s, 1) for s in seqs[:2]], 0)  # the third keeps the original, so both copy
+    cache.reserve([(seqs[0], 1)], 0)
+    assert cache.free_pages == 0
+
+
 def test_a_fork_of_whole_pages_copies_nothing():
     cache, copier = make()
     a = PagedSequence()
