@@ -117,18 +117,21 @@ class PagedKVCache:
                     need += 1
         if need > len(self._free):
             raise PagedCacheFull(f"{need} pages are needed, {len(self._free)} are free")
-        pairs = []
-        for seq in copies:
-            old = seq.pages[-1]
-            seq.pages[-1] = self._take()
+        pairs = [(seq.pages[-1], self._take()) for seq in copies]
+        if pairs:
+            try:
+                self._copy(pairs, stream_ptr)
+            except BaseException:
+                for _, new in pairs:
+                    self._drop(new)
+                raise
+        for seq, (old, new) in zip(copies, pairs):
+            seq.pages[-1] = new
             self._refs[old] -= 1
-            pairs.append((old, seq.pages[-1]))
         for seq, tokens in growth:
             seq.length += tokens
             while len(seq.pages) * self.page_size < seq.length:
                 seq.pages.append(self._take())
-        if pairs:
-            self._copy(pairs, stream_ptr)
 
     def fork(self, seq: PagedSequence) -> PagedSequence:
         """Another sequence with the same tokens; no page is copied yet."""
@@ -314,9 +317,10 @@ class PagedGenerator:
         """Append each entry's tokens to its sequence and draw the token after its last one.
 
         ``sampling`` and ``uniform`` (numbers in [0, 1)) have one element per entry.  Returns the drawn
-        tokens and their log-probabilities in the distribution they were drawn from."""
+        tokens and their log-probabilities in the distribution they were drawn from.  A step that raises
+        leaves the sequences at the lengths that they had."""
 
-        torch, br, c, w = self.torch, self.bridge, self.config, self.weights
+        torch = self.torch
         rows = sum(len(t) for _, t in entries)
         if not entries or any(len(t) == 0 for _, t in entries) or rows > MAX_ROWS:
             raise ValueError(f"a step takes 1 to {MAX_ROWS} tokens, at least one of each of its sequences")
@@ -326,8 +330,25 @@ class PagedGenerator:
             raise ValueError("a sequence grows past max_position")
         stream = stream if stream is not None else torch.cuda.current_stream(self.device)
         sp = int(stream.cuda_stream)
+        before = [s.length for s, _ in entries]
         with torch.cuda.stream(stream):
             self.cache.reserve([(s, len(t)) for s, t in entries], sp)
+        try:
+            return self._run(entries, sampling, uniform, stream)
+        except BaseException:
+            with contextlib.suppress(Exception):  # what was launched ends before its pages are given back
+                stream.synchronize()
+            for (s, _), length in zip(entries, before):
+                self.cache.truncate(s, length)
+            raise
+
+    def _run(self, entries: Sequence[tuple[PagedSequence, Sequence[int]]], sampling: Sequence[Sampling],
+             uniform: Sequence[float], stream: Any) -> tuple[list[int], list[float]]:
+        """The step's work, the sequences grown by their tokens."""
+
+        torch, br, c, w = self.torch, self.bridge, self.config, self.weights
+        rows, sp = sum(len(t) for _, t in entries), int(stream.cuda_stream)
+        with torch.cuda.stream(stream):
             i32 = dict(dtype=torch.int32, device=self.device)
             flat = [tok for _, t in entries for tok in t]
             state = torch.tensor([[tok, 0, 0, 0] for tok in flat], **i32)

@@ -171,3 +171,25 @@ def test_step_refuses_a_sequence_named_twice(setup):
         gen.step([(s, [5]), (s, [6])], [Sampling()] * 2, [0.0] * 2)
     assert s.length == 2
     gen.cache.free(s)
+
+
+def test_step_that_raises_can_be_taken_again(setup):
+    """The settings of the last part of a step do not fit their type: the sequence is as it was before."""
+
+    from kudacuda_b200.paged_serving import PagedSequence, Sampling
+
+    _, _, gen = setup
+    free = gen.cache.free_pages
+    seq, other = PagedSequence(), PagedSequence()
+    ids = prompt(33, 77)
+    gen.step([(seq, ids[:20])], [Sampling()], [0.0])
+    gen.step([(other, ids[:20])], [Sampling()], [0.0])
+    with pytest.raises((RuntimeError, OverflowError, TypeError)):
+        gen.step([(seq, ids[20:])], [Sampling(temperature=1.0, top_k=1 << 40)], [0.0])
+    assert seq.length == 20 and gen.cache.free_pages == free - 4
+    again, _ = gen.step([(seq, ids[20:])], [Sampling()], [0.0])
+    x = gen.x[12].clone()
+    first, _ = gen.step([(other, ids[20:])], [Sampling()], [0.0])
+    assert again == first and torch.equal(gen.x[12], x)
+    gen.cache.free(seq)
+    gen.cache.free(other)

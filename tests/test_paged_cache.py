@@ -10,7 +10,8 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from kudacuda_b200.kudacuda_sidecar import KudaCudaBridge  # noqa: E402
-from kudacuda_b200.paged_serving import PagedCacheFull, PagedKVCache, PagedSequence, paged_rope_tables  # noqa: E402
+from kudacuda_b200.paged_serving import (  # noqa: E402
+    PagedCacheFull, PagedGenerator, PagedKVCache, PagedSequence, Sampling, paged_rope_tables)
 
 
 class Copier:
@@ -164,6 +165,52 @@ def test_a_full_cache_refuses_and_changes_nothing():
         cache.reserve([(a, -1)], 0)
     with pytest.raises(ValueError):
         cache.truncate(a, 21)
+
+
+def test_a_copy_that_fails_changes_nothing():
+    cache, copier = make()
+    a = PagedSequence()
+    grow(cache, a, range(5))
+    b = cache.fork(a)
+
+    def fail(*args, **kw):
+        raise RuntimeError("no copy")
+
+    copier.dispatch_kv_pages_copy = fail
+    with pytest.raises(RuntimeError, match="no copy"):
+        cache.reserve([(a, 30), (b, 1)], 0)
+    assert a.pages == b.pages == [0] and a.length == b.length == 5 and cache.free_pages == 9
+    cache.free(a)
+    cache.free(b)
+    assert cache.free_pages == 10
+
+
+def test_a_step_that_raises_leaves_its_sequences_as_they_were():
+    cache, copier = make()
+    gen = PagedGenerator.__new__(PagedGenerator)
+    gen.torch = StreamedTorch()
+    gen.cache, gen.device, gen.cos = cache, "cpu", torch.zeros((100, 2))
+    gen.config = SimpleNamespace(layers=0, hidden=4, vocab=9, eps=1e-6)
+    gen.weights = SimpleNamespace(layers=[], embedding=None)
+    gen.q = gen.attn = gen.qkv_out = gen.x = torch.zeros((64, 4))
+    done = []
+
+    def fail(*args, **kw):
+        raise RuntimeError("no embedding")
+
+    gen.bridge = SimpleNamespace(dispatch_batch_embedding=fail)
+    a = PagedSequence()
+    grow(cache, a, range(20))
+    b = cache.fork(a)
+    stream = SimpleNamespace(cuda_stream=0, synchronize=lambda: done.append(1))
+    with pytest.raises(RuntimeError, match="no embedding"):
+        gen.step([(a, [1] * 30), (b, [2]), (PagedSequence(), [3])], [Sampling()] * 3, [0.5] * 3, stream)
+    # (one of the two owners may keep its copy of the page they shared)
+    assert a.length == b.length == 20 and len(a.pages) == len(b.pages) == 2 and cache.free_pages >= 7 and done
+    assert read(cache, a) == read(cache, b) == list(range(20))
+    cache.free(a)
+    cache.free(b)
+    assert cache.free_pages == 10
 
 
 def test_a_sequence_named_twice_is_refused():
