@@ -403,10 +403,19 @@ class PagedGenerator:
             raise NativeCudaError(f"paged step raised device error word {word:#x}")
         return tokens, logprobs
 
+    def _most_pages(self, prompt: int, new_tokens: int, answers: int) -> int:
+        """Pages of a prompt and its answers when all are finished: the first answer has all of its own, the
+        others share the whole pages before the prompt's last token.  (The last token drawn is not fed.)"""
+
+        size = self.cache.page_size
+        whole = -(-(prompt + new_tokens - 1) // size)
+        return whole + (answers - 1) * (whole - (prompt - 1) // size)
+
     def generate(self, prompts: Sequence[Sequence[int]], new_tokens: int, sampling: Sampling = Sampling(), *,
                  answers: int = 1, seed: int = 0, stream: Any = None) -> list[list[list[int]]]:
         """``answers`` continuations of every prompt: each prompt is fed once, in pieces that share steps with
-        the sequences that already decode, and then forked.  Returns tokens [prompt][answer]."""
+        the sequences that already decode, and then forked.  A prompt waits until the pages that it and its
+        answers will need are free.  Returns tokens [prompt][answer]."""
 
         if new_tokens < 1 or answers < 1 or any(len(p) == 0 for p in prompts):
             raise ValueError("prompts have tokens, and at least one new token and one answer are asked for")
@@ -414,21 +423,37 @@ class PagedGenerator:
             raise ValueError(f"at most {MAX_ROWS} answers of a prompt")
         rng = random.Random(seed)
         waiting = [(i, PagedSequence(), list(p)) for i, p in enumerate(prompts)][::-1]  # the next one last
-        decoding: list[tuple[list[int], PagedSequence]] = []
+        decoding: list[tuple[int, list[int], PagedSequence]] = []
         out: list[list[list[int]]] = [[] for _ in prompts]
         live: list[PagedSequence] = []
+        budget = self.cache.free_pages
+        claims: dict[int, int] = {}  # pages of the prompts that have begun, at their most
+        unfinished = [answers] * len(prompts)
+
+        def done(i: int, seq: PagedSequence) -> None:
+            self.cache.free(seq)
+            live.remove(seq)
+            unfinished[i] -= 1
+            if unfinished[i] == 0:
+                del claims[i]
+
         try:
             while waiting or decoding:
                 room = MAX_ROWS
                 batch: list[tuple[Any, PagedSequence, list[int]]] = []
-                for got, seq in decoding[:room]:
+                for _, got, seq in decoding[:room]:
                     batch.append((got, seq, [got[-1]]))
                 room -= len(batch)
                 fed = []
                 while waiting and room > 0:
-                    i, seq, left = waiting.pop()
-                    if not seq.pages:
+                    i, seq, left = waiting[-1]
+                    if i not in claims:
+                        pages = self._most_pages(len(left), new_tokens, answers)
+                        if claims and sum(claims.values()) + pages > budget:
+                            break
+                        claims[i] = pages
                         live.append(seq)
+                    waiting.pop()
                     batch.append((i, seq, left[:room]))
                     room -= len(left[:room])
                     fed.append((i, seq, left[len(batch[-1][2]):]))
@@ -436,13 +461,12 @@ class PagedGenerator:
                 tokens, _ = self.step([(s, t) for _, s, t in batch], [d[0] for d in draws], [d[1] for d in draws],
                                       stream)
                 still = []
-                for (got, seq), token in zip(decoding[:MAX_ROWS], tokens):
+                for (i, got, seq), token in zip(decoding[:MAX_ROWS], tokens):
                     got.append(token)
                     if len(got) < new_tokens:
-                        still.append((got, seq))
+                        still.append((i, got, seq))
                     else:
-                        self.cache.free(seq)
-                        live.remove(seq)
+                        done(i, seq)
                 decoding = decoding[MAX_ROWS:] + still
                 for (i, seq, left), token in zip(fed, tokens[len(batch) - len(fed):]):
                     if left:
@@ -463,10 +487,9 @@ class PagedGenerator:
                         got = [first]
                         out[i].append(got)
                         if new_tokens > 1:
-                            decoding.append((got, owner))
+                            decoding.append((i, got, owner))
                         else:
-                            self.cache.free(owner)
-                            live.remove(owner)
+                            done(i, owner)
         finally:
             for seq in live:
                 self.cache.free(seq)

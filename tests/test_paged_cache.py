@@ -213,6 +213,54 @@ def test_a_step_that_raises_leaves_its_sequences_as_they_were():
     assert cache.free_pages == 10
 
 
+class Counting(PagedGenerator):
+    """A generator whose steps only take pages; the token drawn is the sequence's length."""
+
+    def __init__(self, num_pages, page=16):
+        self.cache, self.copier = make(num_pages, page)
+        self.steps, self.least = 0, num_pages
+
+    def step(self, entries, sampling, uniform, stream=None):
+        self.cache.reserve([(s, len(t)) for s, t in entries], 0)
+        self.steps += 1
+        self.least = min(self.least, self.cache.free_pages)
+        return [s.length for s, _ in entries], [0.0] * len(entries)
+
+
+@pytest.mark.parametrize("pages,lengths,new,answers", [
+    (4, [16] * 5, 5, 1), (3, [1, 33, 2, 40], 8, 1), (10, [16, 17, 15, 1, 31], 20, 3), (40, [100, 200, 7], 50, 4),
+    (5, [64, 64, 10], 17, 1), (7, [33, 16], 1, 5),
+])
+def test_prompts_wait_until_their_pages_are_free(pages, lengths, new, answers):
+    gen = Counting(pages)
+    out = gen.generate([[1] * n for n in lengths], new, answers=answers)
+    assert out == [[[n + t for t in range(new)]] * answers for n in lengths]
+    assert gen.cache.free_pages == pages
+
+
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 33, 50])
+@pytest.mark.parametrize("new", [1, 2, 15, 16, 17, 40])
+@pytest.mark.parametrize("answers", [1, 2, 5])
+def test_pages_of_a_prompt_and_its_answers(length, new, answers):
+    gen = Counting(100)
+    gen.generate([[1] * length], new, answers=answers)
+    most = gen._most_pages(length, new, answers)
+    assert 100 - gen.least == most
+    Counting(most).generate([[1] * length], new, answers=answers)
+    with pytest.raises(PagedCacheFull):  # one alone that does not fit is refused, and leaves nothing behind
+        gen = Counting(most)
+        held = PagedSequence()
+        gen.cache.reserve([(held, 1)], 0)
+        gen.generate([[1] * length], new, answers=answers)
+    assert gen.cache.free_pages == most - 1
+
+
+def test_prompts_that_fit_together_share_steps():
+    gen = Counting(100)
+    gen.generate([[1] * 10] * 5, 6)
+    assert gen.steps == 6
+
+
 def test_a_sequence_named_twice_is_refused():
     """Both entries would get the length with all tokens, and write the same place."""
 
