@@ -1601,8 +1601,9 @@ class KudaCudaBridge:
             raise ValueError("k_pages and v_pages must be contiguous")
         if pairs.dtype is not int32 or pairs.dim() != 2 or pairs.shape[1] != 2 or not pairs.is_contiguous():
             raise ValueError("pairs must be contiguous int32 [n, 2]")
-        size, num_pages = k_pages.element_size(), shape[1]
-        layer_bytes = k_pages.stride(0) * size
+        # (from the shape: the stride of a single layer may be anything, contiguous or not)
+        num_pages = shape[1]
+        page_bytes = math.prod(shape[2:]) * k_pages.element_size()
         table = (0, 0, 0, 0)
         if (block_table is None) != (page_map is None):
             raise ValueError("a block table and a page map come together")
@@ -1618,8 +1619,8 @@ class KudaCudaBridge:
                 raise ValueError("page_map must be contiguous int32 [num_pages]")
             table = (block_table.data_ptr(), stride if rows > 1 else width, rows, width)
         self._require_device(k_pages, v_pages, pairs, block_table, page_map)
-        self._call("kudacuda_sm100_kv_pages_copy", k_pages.data_ptr(), v_pages.data_ptr(), shape[0], layer_bytes,
-                   num_pages, layer_bytes // max(1, num_pages), pairs.data_ptr(), pairs.shape[0], *table,
+        self._call("kudacuda_sm100_kv_pages_copy", k_pages.data_ptr(), v_pages.data_ptr(), shape[0],
+                   num_pages * page_bytes, num_pages, page_bytes, pairs.data_ptr(), pairs.shape[0], *table,
                    0 if page_map is None else page_map.data_ptr(), stream_ptr & 0xFFFFFFFFFFFFFFFF)
 
     def dispatch_sample(self, logits: Any, tokens: Any, uniform: Any, *, temperature: Any = None, top_k: Any = None,

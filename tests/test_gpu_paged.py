@@ -360,6 +360,18 @@ def test_kv_pages_copy(bridge, layers, pages, shape, moves, tables):
         assert torch.equal(wide, want)
 
 
+def test_kv_pages_copy_of_one_layer_whose_stride_is_a_page(bridge):
+    g = torch.Generator(device=DEV).manual_seed(11)
+    k, v = (torch.randn((9, 1, 2, 16, 64), generator=g, device=DEV).to(BF16).transpose(0, 1) for _ in range(2))
+    want_k, want_v = k.clone(), v.clone()
+    for a, b in ((8, 0), (3, 7)):
+        want_k[:, b], want_v[:, b] = k[:, a], v[:, a]
+    bridge.dispatch_kv_pages_copy(k, v, torch.tensor([[8, 0], [3, 7]], dtype=torch.int32, device=DEV),
+                                  stream_ptr=int(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert bridge.error_word(clear=True) == 0 and torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
 def test_kv_pages_copy_skips_pages_out_of_range(bridge):
     k = torch.randn((2, 6, 1, 16, 64), device=DEV).to(BF16)
     v = k + 1

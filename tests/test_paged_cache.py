@@ -507,6 +507,15 @@ def test_pages_copy_passes_and_refuses(bridge):
     assert not bridge.lib.calls
 
 
+def test_pages_copy_of_one_layer_goes_by_its_shape(bridge):
+    """The stride of the single layer is a page's; the tensor is contiguous all the same."""
+
+    k, v = (torch.zeros((4, 1, 2, 16, 64), dtype=BF16).transpose(0, 1) for _ in range(2))
+    assert k.is_contiguous() and k.stride(0) == 2048
+    bridge.br.dispatch_kv_pages_copy(k, v, torch.zeros((1, 2), dtype=torch.int32), stream_ptr=0)
+    assert bridge.lib.calls[-1][1][3:7] == (1, 4 * 4096, 4, 4096)
+
+
 def test_sample_passes_and_refuses(bridge):
     x, u, tok = torch.zeros((3, 20), dtype=BF16)[:, 4:14], torch.zeros(3), torch.zeros(3, dtype=torch.int32)
     bridge.br.dispatch_sample(x, tok, u, top_k=tok, stream_ptr=0)
