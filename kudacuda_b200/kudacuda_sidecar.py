@@ -1578,6 +1578,8 @@ class KudaCudaBridge:
         if lse is not None and (lse.dtype is not self._types[2] or lse.shape != (rows, heads)
                                 or not lse.is_contiguous()):
             raise ValueError("lse must be contiguous float32 [rows, q_heads]")
+        if not workspace.is_contiguous():  # (an expanded one has fewer bytes than it says)
+            raise ValueError("workspace must be contiguous")
         self._require_device(query, k_pages, v_pages, output, query_start, kv_len, block_table, workspace, lse)
         self._call("kudacuda_sm100_paged_attention", code, query.data_ptr(), stride, k_pages.data_ptr(),
                    v_pages.data_ptr(), output.data_ptr(), out_stride, 0 if lse is None else lse.data_ptr(),

@@ -456,6 +456,12 @@ def test_paged_attention_refuses(bridge, kw):
     assert not bridge.lib.calls
 
 
+def test_paged_attention_refuses_a_workspace_smaller_than_it_says(bridge):
+    with pytest.raises(ValueError, match="workspace"):
+        attend(bridge.br, attention_args(ws=torch.zeros(1, dtype=torch.uint8).expand(4096)))
+    assert not bridge.lib.calls
+
+
 def append_args(**kw):
     a = dict(qkv=torch.zeros((3, 8 * 64), dtype=BF16), q=torch.zeros((3, 4, 64), dtype=BF16),
              cos=torch.zeros((9, 16)), sin=torch.zeros((9, 16)), bias=None)
