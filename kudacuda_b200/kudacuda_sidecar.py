@@ -1526,6 +1526,8 @@ class KudaCudaBridge:
         if out_rows != rows or cols != out_cols + 2 * kv_heads * head_dim or q_out.dtype is not dtype:
             raise ValueError("q_out must hold the query heads of qkv's rows in its dtype")
         max_pos = rotary = cos = sin = 0
+        if (rope_cos is None) != (rope_sin is None):
+            raise ValueError("rope_cos and rope_sin come together")
         if rope_cos is not None:
             f32 = self._types[2]
             if (rope_cos.dtype is not f32 or rope_sin.dtype is not f32 or rope_cos.dim() != 2

@@ -494,6 +494,13 @@ def test_rope_append_refuses(bridge, kw):
     assert not bridge.lib.calls
 
 
+@pytest.mark.parametrize("kw", [dict(cos=None), dict(sin=None)])
+def test_rope_append_refuses_one_table_without_the_other(bridge, kw):
+    with pytest.raises(ValueError, match="together"):
+        append(bridge.br, append_args(**kw))
+    assert not bridge.lib.calls
+
+
 def test_pages_copy_passes_and_refuses(bridge):
     k, v = torch.zeros((3, 7, 2, 16, 8), dtype=BF16), torch.zeros((3, 7, 2, 16, 8), dtype=BF16)
     pairs = torch.zeros((2, 2), dtype=torch.int32)
