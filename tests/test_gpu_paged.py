@@ -611,3 +611,17 @@ def test_native_refusals(bridge):
                                x[:, 0].contiguous(), stream_ptr=0)
     torch.cuda.synchronize()
     assert bridge.error_word(clear=True) == 0
+
+
+@pytest.mark.parametrize("kw,word", [(dict(num_pages=1 << 60), "num_pages"), (dict(num_pages=(1 << 59) + 1), "num_pages"),
+                                     (dict(width=1 << 60), "table_width"), (dict(width=(1 << 60) + 1), "table_width")])
+def test_native_refuses_sizes_whose_products_wrap(bridge, kw, word):
+    k, v, table, _, _ = R.make_cache([40], 2, 16, 128, BF16, DEV, 95)
+    start, kv = R.starts([1], DEV), torch.tensor([40], dtype=torch.int32, device=DEV)
+    q = torch.zeros((1, 16, 128), dtype=BF16, device=DEV)
+    out, ws = torch.empty_like(q), bridge.paged_attention_workspace(q, k, table, max_query=1)
+    width, pages = kw.get("width", table.shape[1]), kw.get("num_pages", k.shape[0])
+    rc = bridge.lib.kudacuda_sm100_paged_attention(
+        bridge.engine_handle, 2, q.data_ptr(), 2048, k.data_ptr(), v.data_ptr(), out.data_ptr(), 2048, 0, ws.data_ptr(),
+        ws.nbytes, start.data_ptr(), kv.data_ptr(), table.data_ptr(), width, width, 1, 1, 1, 16, 2, 128, pages, 16, 0.1, 0)
+    assert rc == 1 and word in bridge.lib.kudacuda_last_error(bridge.engine_handle).decode()
