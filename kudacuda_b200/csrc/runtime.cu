@@ -1735,9 +1735,10 @@ const char* paged_batch(kc::PagedBatch* p, Handle* h, int dtype, uint64_t k_page
     // (each factor by itself first: the products must not wrap)
     if (num_pages < 1 || num_pages > (int64_t{1} << 31) || num_pages * kv_heads * page_size > (int64_t{1} << 31) - 1)
         return "requires num_pages >= 1 and num_pages * kv_heads * page_size < 2^31";
-    if (table_width < 1 || table_width > (int64_t{1} << 27) || table_width * page_size > (int64_t{1} << 27) || table_stride < table_width)
+    if (table_width < (batch > 0 ? 1 : 0) || table_width > (int64_t{1} << 27) || table_width * page_size > (int64_t{1} << 27) || table_stride < table_width)
         return "requires table_width >= 1, table_width * page_size <= 2^27 and table_stride >= table_width";
-    if (k_pages == 0 || v_pages == 0 || query_start == 0 || kv_len == 0 || block_table == 0)
+    // (a batch of no sequences has no lengths and no table)
+    if (k_pages == 0 || v_pages == 0 || query_start == 0 || (batch > 0 && (kv_len == 0 || block_table == 0)))
         return "requires non-null device pointers";
     if (k_pages % 16 != 0 || v_pages % 16 != 0) return "the pages must be 16-byte aligned";
     p->query_start = P<const int32_t>(query_start);

@@ -219,6 +219,19 @@ def test_attention_no_rows(bridge):
     assert out.shape[0] == 0 and bridge.error_word(clear=True) == 0
 
 
+@pytest.mark.parametrize("width", [0, 4])
+def test_a_batch_of_no_sequences(bridge, width):
+    k, v = (torch.zeros((3, 2, 16, 128), dtype=BF16, device=DEV) for _ in range(2))
+    q, qkv = torch.empty((0, 16, 128), dtype=BF16, device=DEV), torch.empty((0, 20 * 128), dtype=BF16, device=DEV)
+    table, lens = torch.empty((0, width), dtype=torch.int32, device=DEV), torch.empty((0,), dtype=torch.int32, device=DEV)
+    start = torch.zeros((1,), dtype=torch.int32, device=DEV)
+    ws = bridge.paged_attention_workspace(q, k, table, max_query=0)
+    bridge.dispatch_paged_attention(q, k, v, torch.empty_like(q), start, lens, table, ws, max_query=0, stream_ptr=0)
+    bridge.dispatch_rope_append_paged(qkv, q, k, v, None, None, start, lens, table, stream_ptr=0)
+    torch.cuda.synchronize()
+    assert bridge.error_word(clear=True) == 0 and not k.any() and not v.any()
+
+
 def test_attention_offsets_past_32_bits(bridge):
     """A cache of more than 2^32 elements whose sequences live at its end."""
 
