@@ -124,6 +124,41 @@ def test_attention_scores_far_apart(bridge, new, lens):
     check_attention(q, new, lens, keys, vals, out, lse, 1 / math.sqrt(d))
 
 
+def small_weights(bridge, dtype, heads, below, step, n=20_032, d=64):
+    """The first key takes almost all of the weight but its value is 0: the output is that of the others, each
+    ``below`` nats less.  As many equal sequences as the device has SMs, so that one running maximum goes
+    through a sequence's whole length.  ``step``: half of the spacing of the smallest f16 weights, as a part
+    of the largest weight, by which each may be off beside its rounding (bf16 has no such end)."""
+
+    g = torch.Generator().manual_seed(int(10 * below) + heads)
+    kk = (0.01 * torch.randn((1, n, d), generator=g)).to(dtype)
+    vv = (64 * (0.5 + torch.rand((1, n, d), generator=g))).to(dtype)
+    kk[:, 0, :] = 0
+    kk[:, :, 0] = 0
+    kk[:, 0, 0] = 8.0
+    vv[:, 0] = 0
+    q = 0.3 * torch.randn((1, heads, d), generator=g)
+    q[:, :, 0] = below * math.sqrt(d) / 8.0
+    q = q.to(dtype)
+    batch = torch.cuda.get_device_properties(0).multi_processor_count
+    k, v = (x.view(n // 64, 1, 64, d).to(DEV) for x in (kk, vv))
+    table = torch.arange(n // 64, dtype=torch.int32, device=DEV).repeat(batch, 1)
+    out, _ = attend(bridge, q.to(DEV).repeat(batch, 1, 1), k, v, table, [1] * batch, [n] * batch)
+    assert bridge.error_word(clear=True) == 0
+    ref, _, mag, _ = R.attention(q, [1], [n], [kk.double()], [vv.double()], 1 / math.sqrt(d))
+    u = R.UNIT[dtype]
+    bound = u * ref.abs() + (u + 2.0**-14) * mag + (n * step * 96 + 2.0**-25 if dtype == F16 else 0)
+    for r in (0, 1, batch // 2, batch - 1):
+        worst = ((out[r:r + 1].double().cpu() - ref).abs() / bound).max()
+        assert worst <= 1, f"{float(worst)} of the bound"
+
+
+@pytest.mark.parametrize("dtype,heads", [(F16, 1), (BF16, 1), (F16, 12)])
+@pytest.mark.parametrize("below", [12.0, 17.4, 19.0])
+def test_attention_small_weights_beside_a_large_one(bridge, dtype, heads, below):
+    small_weights(bridge, dtype, heads, below, 2.0**-40)
+
+
 @pytest.mark.parametrize("new,lens", [([1, 1, 1], [70, 300, 129]), ([90, 3], [200, 77])])
 def test_attention_strided_rows_scale_stream_and_wide_table(bridge, new, lens):
     """Rows that are a slice of a wider buffer, a table that is a slice of a wider one, a scale of the
