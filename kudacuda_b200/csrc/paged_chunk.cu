@@ -9,8 +9,8 @@
 //   O_t += P_t V_j    (P from tensor memory, V from shared memory, MN-major)
 // with the running maximum m in the log2 domain (c = scale log2 e).  A thread
 // owns one row, so maximum and sum need no exchange.  m only follows the true
-// maximum when that has grown by more than 8 (a factor of 256, far inside fp32
-// and both 16-bit types): O is then rescaled in tensor memory, which is rare.
+// maximum when that has grown by more than kLazy (a factor of 256, far inside fp32
+// and bf16, or of 16 in f16): O is then rescaled in tensor memory, which is rare.
 // The final O / l does not depend on m.
 //
 // Warps: 0-3 and 4-7 softmax, tile 0 and 1; 8 K/V producer (TMA, one box per
@@ -21,7 +21,8 @@
 //
 // P is rounded to the cache's type because that is what the matrix instruction
 // takes (its error, half a step of the type, is that of the output's own rounding;
-// sum and maximum are of the unrounded values).  The two tiles take turns: while
+// sum and maximum are of the unrounded values).  f16 P are scaled up, or the small
+// ones would not be there (kShift).  The two tiles take turns: while
 // one's scores are exponentiated the other's products run, and the first half of
 // P multiplies while the second is made.  Two tiles fill the tensor memory (S 2 x
 // 128, O 2 x 128 columns).
@@ -56,7 +57,15 @@ constexpr int kThreads = 384;
 // together 414 us, with 256 430, with 512 416.
 constexpr int kOver = 384;
 constexpr int kLeast = 128;  // (96, 192 and 256: within 3% on 24 batches, none better throughout)
-constexpr float kLazy = 8.F;  // how far the true maximum may exceed m
+// m is a running maximum less kShift, and the true one, less kShift too, may exceed it
+// by kLazy.  f16 ends at 2^16 and 2^-25: with P up to 2^15, what rounds to nothing is a
+// weight below 2^-36 of the largest (with kShift 0 below 2^-25, and 131071 keys of 2^-25.1
+// beside one of 1 were lost: 0.4% of O).  f16 with kLazy 8, 6, 4, 2, 0: the large case 441, 439,
+// 441, 468, 485 us, 24 mixed sequences 56.8, 56.8, 56.9, 58.9, 59.3.
+template <int DT>
+constexpr float kLazy = DT == kF16 ? 4.F : 8.F;
+template <int DT>
+constexpr float kShift = DT == kF16 ? 15.F - kLazy<DT> : 0.F;
 
 template <int D>
 struct ChunkSmem {
@@ -390,9 +399,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mx[0] = max3(mx[0], s[i], s[i + 1]);
                     mx[1] = max3(mx[1], s[i + 2], s[i + 3]);
                 }
-                const float top = max3(max3(mx[0], s[kKeys - 2], s[kKeys - 1]), mx[1], mx[1]) * c;
+                const float top = fmaf(max3(max3(mx[0], s[kKeys - 2], s[kKeys - 1]), mx[1], mx[1]), c, -kShift<DT>);
                 if (top != top) l = top;  // a NaN score makes the row NaN
-                const bool grow = top > m + kLazy;  // from -inf: any finite maximum
+                const bool grow = top > m + kLazy<DT>;  // from -inf: any finite maximum
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mn = grow ? top : m;
                     const float f = grow ? ex2(m - mn) : 1.F;

@@ -159,6 +159,12 @@ def test_attention_small_weights_beside_a_large_one(bridge, dtype, heads, below)
     small_weights(bridge, dtype, heads, below, 2.0**-40)
 
 
+@pytest.mark.parametrize("dtype,heads", [(F16, 32), (BF16, 32), (F16, 17)])
+@pytest.mark.parametrize("below", [12.0, 17.4, 19.0])
+def test_attention_small_weights_with_many_rows(bridge, dtype, heads, below):
+    small_weights(bridge, dtype, heads, below, 2.0**-36)
+
+
 @pytest.mark.parametrize("new,lens", [([1, 1, 1], [70, 300, 129]), ([90, 3], [200, 77])])
 def test_attention_strided_rows_scale_stream_and_wide_table(bridge, new, lens):
     """Rows that are a slice of a wider buffer, a table that is a slice of a wider one, a scale of the
