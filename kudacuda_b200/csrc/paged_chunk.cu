@@ -133,6 +133,23 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
 }
+// A wait that may last for whole pieces (one of 2^20 blocks takes a second, 2^17
+// tries end after 0.2): it gives up when no block has been fetched for as long as
+// any other wait would last (the ring holds a few).
+__device__ __forceinline__ bool bar_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                              const volatile int* beat) {
+    for (int round = 0, seen = 0;; ++round) {
+        for (uint32_t i = 0; i < (1u << 17); ++i) {
+            if (mbar_try_wait(bar, parity)) return true;
+            if (*abort_flag) return false;
+        }
+        const int now = *beat;
+        if (round > 0 && now == seen) break;
+        seen = now;
+    }
+    *abort_flag = 1;
+    return false;
+}
 // the item's last block has rows without a key
 __device__ __forceinline__ bool has_tail(int limit) { return limit % kKeys != 0 || limit == 0; }
 
@@ -153,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) ChunkBars bars;
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, beat_count;
     __shared__ int64_t sums[kThreads / 32], place_at;
     __shared__ int place_seq;
     const PagedBatch& p = a.p;
@@ -181,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.p_ready[i], 128);
             mbar_init(&bars.o_done[i], 1);
         }
-        abort_flag = 0;
+        abort_flag = beat_count = 0;
         fence_mbar_init();
     }
     tc_fence_before();
@@ -194,6 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_launch_dependents();
     const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_slot);
     volatile int* const abort_p = &abort_flag;
+    volatile int* const beat = &beat_count;  // blocks fetched
     W w;
     w.begin(p, group, shares, worker, place_seq, place_at);
 
@@ -226,7 +244,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tail_use = tail ? tail_use | 1u << s : tail_use & ~(1u << s);
                         if (tail) tail_parity ^= 1u << s;
                         uint64_t* const full = tail ? &bars.v_tail[s] : &bars.kv_full[s];
-                        if (lane == 0) mbar_arrive_expect_tx(full, pages * p.page_size * 128 * M::kHalves);
+                        if (lane == 0) {
+                            *beat = static_cast<int>(seq);
+                            mbar_arrive_expect_tx(full, pages * p.page_size * 128 * M::kHalves);
+                        }
                         __syncwarp();
                         if (mine)
                             tma_load_2d(ring + s * M::kTile + half * (128 * 128) + part * p.page_size * 128,
@@ -308,8 +329,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t items = 0, seq = 0, tail_parity = 0;
             const uint16_t* q = static_cast<const uint16_t*>(a.q);
             while (w.next(p, group)) {
-                // (a long wait: the whole of the piece before)
-                if (items > 0 && !bar_wait(&bars.q_empty, (items - 1) & 1, abort_p, true, 1u << 22)) break;
+                // (the whole of the piece before)
+                if (items > 0 && !bar_wait_long(&bars.q_empty, (items - 1) & 1, abort_p, beat)) break;
                 const int r_all = w.item_rows > 128 ? 256 : 128;
                 if (q_by_tma) {  // 128 / group whole tokens a tile (rows past the item are other tokens': not stored)
                     if (lane == 0) mbar_arrive_expect_tx(&bars.q_full, r_all * D * 2);
@@ -343,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 seq += 2 * (w.t1 - w.t0);
                 if (w.t1 == w.tiles && has_tail(w.limit)) {
                     const uint32_t sv = (seq - 1) % M::kStages;  // the piece's last V block
-                    if (!bar_wait(&bars.v_tail[sv], tail_parity >> sv & 1, abort_p, true, 1u << 22)) break;
+                    if (!bar_wait_long(&bars.v_tail[sv], tail_parity >> sv & 1, abort_p, beat)) break;
                     tail_parity ^= 1u << sv;
                     const int from = w.limit - (w.tiles - 1) * kKeys;  // rows from here on hold no key
                     uint8_t* v = ring + sv * M::kTile;
@@ -376,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool idle = !__any_sync(0xffffffffu, live);  // a warp of rows past the item: it only keeps step
             float m = -INFINITY, l = 0.F;
             for (int j = w.t0; j < w.t1; ++j) {
-                bar_wait(&bars.s_full[t], ns++ & 1, abort_p);
+                // (the second tile's first block: the whole of every piece without that tile)
+                bar_wait_long(&bars.s_full[t], ns++ & 1, abort_p, beat);
                 tc_fence_after();
                 if (idle) {  // (what its lanes of P hold reaches no row of the item)
                     tc_fence_before();

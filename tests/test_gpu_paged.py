@@ -273,6 +273,28 @@ def test_a_batch_of_no_sequences(bridge, width):
     assert bridge.error_word(clear=True) == 0 and not k.any() and not v.any()
 
 
+def test_attention_second_tile_idle_for_a_long_time(bridge):
+    """Items of one tile first, for longer than 2^17 tries of a barrier last (0.2 s), then items of two: 64
+    sequences of 2^27 keys, the same page over and over, for one token of 32 heads, and at the end 300 tokens
+    over 400 keys, all in the last worker's share."""
+
+    page, d, n, long = 128, 64, 1 << 27, 64
+    g = torch.Generator().manual_seed(83)
+    k, v, small, keys, vals = R.make_cache([400], 1, page, d, BF16, DEV, 84)
+    table = torch.full((long + 1, n // page), int(small[0, 0]), dtype=torch.int32, device=DEV)
+    table[-1, :small.shape[1]] = small[0]
+    q = torch.randn((long + 300, 32, d), generator=g).to(BF16).to(DEV)
+    out, lse = attend(bridge, q, k, v, table, [1] * long + [300], [n] * long + [400])
+    assert bridge.error_word(clear=True) == 0
+    check_attention(q[-300:], [300], [400], keys, vals, out[-300:], lse[-300:], 1 / math.sqrt(d))
+    # a long sequence attends to 128 keys, to each as often; its 32-bit sums are of that many blocks, and
+    # each addition may be off by 2^-23 of the sum
+    want, _ = attend(bridge, q[:long], k, v, small[:, :1].repeat(long, 1), [1] * long, [page] * long)
+    blocks = long * (n // 128) / (torch.cuda.get_device_properties(0).multi_processor_count - 1)
+    bound = (2 * blocks * 2.0**-23 + 2.0**-7) * v[small[0, 0]].abs().max().double()
+    assert ((out[:long].double() - want.double()).abs() <= bound).all()
+
+
 def test_attention_offsets_past_32_bits(bridge):
     """A cache of more than 2^32 elements whose sequences live at its end."""
 
