@@ -512,9 +512,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         v.begin(p, group, shares, worker, place_seq, place_at);
         Part::cuts(a.workspace)[worker] = v.record(p, group, shares, worker);
     }
-    if (tid == 0 && *abort_p && p.err != nullptr) atomicOr(p.err, 16);
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && *abort_p && p.err != nullptr) atomicOr(p.err, 16);  // (every wait is over)
     if (warp == 8) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
