@@ -20,6 +20,9 @@
 // Items of at most 8 rows put lo into the fragment's other 8 rows, whose sum with the first 8 is
 // taken at the end: half of the products, and the tensor cores keep time to
 // spare while the cache arrives.
+// A value that is not finite reaches the rows that attend it alone: where a block has
+// keys past some row's own, it is looked through for one first, and if there is one
+// the product is taken row by row.
 //
 // Measured (128 dims): 2 sequences of 70 001 to 130 001 keys, 8 key heads of 4: 131 us,
 // 5.9 TB/s of the card's 6.55 (the join of the pieces, 4 us, does not overlap); 64
@@ -92,9 +95,30 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+// the halves of a word that hold keys `key` and `key` + 1, where these are below `left`
+__device__ __forceinline__ uint32_t keep_below(int key, int left) {
+    return (key < left ? 0xffffu : 0u) | (key + 1 < left ? 0xffff0000u : 0u);
+}
+// Whether one of the first `keys` rows of a warp's V block holds an infinity or a NaN.
+template <int DT, int D>
+__device__ __forceinline__ bool not_finite(uint32_t block, int keys) {
+    constexpr uint32_t kTop = DT == kBF16 ? 0x7f80u : 0x7c00u;
+    bool found = false;
+    for (int i = threadIdx.x & 31; i < D / 64 * kKeys * 8; i += 32) {  // 16-byte words, eight a row of 64 dims
+        uint32_t x[4];
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                     : "r"(block + 16 * i));
+        if ((i >> 3) % kKeys >= keys) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) found = found || (x[k] & kTop) == kTop || (x[k] >> 16 & kTop) == kTop;
+    }
+    return __any_sync(0xffffffffu, found);
+}
+
 // What the warps need of a piece; thread 0 lists them, kList at a time.
 struct Piece {
-    int b, start, n, len, kvh, r0, rows, limit, t0, t1;
+    int b, start, n, len, kvh, r0, rows, limit, least, t0, t1;
     int whole;
 };
 constexpr int kList = 12;
@@ -155,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 e.r0 = w.q * kRows;
                 e.rows = w.item_rows;
                 e.limit = w.limit;
+                e.least = w.least;
                 e.t0 = w.t0;
                 e.t1 = w.t1;
                 e.whole = w.whole() ? 1 : 0;
@@ -329,6 +354,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (narrow && h == 0) ph[n >> 1][2 * (n & 1) + 1] = lo;
                         pl[n >> 1][2 * (n & 1) + h] = lo;
                     }
+                if (e.least < min(key0 + kKeys, e.limit) && not_finite<DT, D>(vb, valid)) {
+                    // (rare) a value that only some of the rows may see, and 0 times it is not 0: the product
+                    // is taken for each row by itself, with the values past its keys left out
+#pragma unroll 1
+                    for (int r = 0; r < e.rows; ++r) {
+                        const int left = __shfl_sync(0xffffffffu, r < 8 ? row_keys[0] : row_keys[1], 4 * (r & 7)) - key0;
+                        if (left <= 0) continue;
+                        const bool mine = g == (r & 7);
+#pragma unroll
+                        for (int d = 0; d < D / 16; ++d) {
+                            const int key = lane & 15, word = 2 * (d & 3) + (lane >> 4);
+                            uint32_t b[4];
+                            ldsm4t(b, vb + key * 128 + (d >> 2) * (kKeys * 128) + ((word ^ (key & 7)) << 4));
+                            const uint32_t keep0 = keep_below(2 * t4, left), keep1 = keep_below(2 * t4 + 8, left);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                float one[4] = {0.F, 0.F, 0.F, 0.F};
+                                mma16816<DT>(one, ph[0], b[2 * x] & keep0, b[2 * x + 1] & keep1);
+                                if (!narrow) mma16816<DT>(one, pl[0], b[2 * x] & keep0, b[2 * x + 1] & keep1);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (mine && (narrow || i >> 1 == r >> 3)) o[2 * d + x][i] += one[i];
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    continue;
+                }
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk) {
                     const int key = 16 * kk + (lane & 15);
@@ -337,9 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int left = valid - 16 * kk;
                     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
                     if (left < 16) {
-                        const int k0 = 2 * t4, k1 = 2 * t4 + 8;
-                        keep0 = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
-                        keep1 = (k1 < left ? 0xffffu : 0u) | (k1 + 1 < left ? 0xffff0000u : 0u);
+                        keep0 = keep_below(2 * t4, left);
+                        keep1 = keep_below(2 * t4 + 8, left);
                     }
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d) {

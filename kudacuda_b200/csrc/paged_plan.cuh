@@ -82,7 +82,7 @@ struct PagedWalk {
     int next_kvh, next_q;
     // the piece at hand
     int piece_b, piece_start, piece_n, piece_len;
-    int kvh, q, item_rows, limit, t0, t1, tiles;
+    int kvh, q, item_rows, limit, least, t0, t1, tiles;  // limit, least: keys of the last row and of the first
     int64_t item_end;
 
     // cost of the first k tiles of a key head
@@ -138,6 +138,7 @@ struct PagedWalk {
         item_rows = min(ROWS, rows - q * ROWS);
         const int last_token = q == tiles_q - 1 ? n - 1 : (q * ROWS + ROWS - 1) / group;
         limit = min(max(len - n + last_token + 1, 0), p.table_width * p.page_size);
+        least = min(max(len - n + q * ROWS / group + 1, 0), limit);
         tiles = max((limit + KT - 1) / KT, 1);
         return lo;
     }

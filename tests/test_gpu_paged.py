@@ -253,6 +253,37 @@ def test_attention_nan_reaches_the_rows_that_attend_it_alone(bridge, new):
     assert torch.equal(out[new[0]:], good[new[0]:]) and torch.equal(lse[new[0]:], good_lse[new[0]:])
 
 
+def values_not_finite(bridge, dtype, heads, kv_heads, d, new, lens, back, value):
+    """One element of the value of the key ``back`` places before sequence 0's last one: the rows that attend
+    it get it, in its dim alone, and no other row sees it."""
+
+    k, v, table, keys, vals = R.make_cache(lens, kv_heads, 16, d, dtype, DEV, 67)
+    q = torch.randn((sum(new), heads, d), generator=torch.Generator().manual_seed(68)).to(dtype)
+    pos, dim = lens[0] - 1 - back, d - 3
+    v[int(table[0, pos // 16]), kv_heads - 1, pos % 16, dim] = value
+    vals[0][kv_heads - 1, pos, dim] = value
+    out, lse = attend(bridge, q.to(DEV), k, v, table, new, lens)
+    assert bridge.error_word(clear=True) == 0
+    scale = 1 / math.sqrt(d)
+    ref, ref_lse, mag, reach = R.attention(q, new, lens, keys, vals, scale)
+    got, u = out.double().cpu(), R.UNIT[dtype]
+    hit = ~torch.isfinite(ref)
+    assert hit.any() and not hit[..., :dim].any() and not torch.isfinite(got[hit]).any()
+    assert ((got - ref).abs() <= u * ref.abs() + (u + 2.0**-14) * mag)[~hit].all()
+    assert ((lse.double().cpu() - ref_lse).abs() <= d * 2.0**-24 * reach + 2.0**-18).all()
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("case", [
+    # dtype, heads, kv_heads, d, new, lengths, back: few rows a key head
+    (BF16, 8, 1, 128, [2, 1], [37, 20], 0), (F16, 2, 2, 64, [16], [16], 7), (BF16, 10, 2, 128, [3, 2], [600, 17], 1),
+    (F16, 4, 2, 128, [4, 1, 3], [129, 5, 64], 0), (BF16, 5, 5, 64, [9], [9], 8), (F16, 16, 2, 64, [2], [4098], 0),
+    (BF16, 6, 3, 128, [8], [33], 3),
+])
+def test_attention_values_that_are_not_finite_few_rows(bridge, case, value):
+    values_not_finite(bridge, *case, value)
+
+
 def test_attention_no_rows(bridge):
     k, v, table, _, _ = R.make_cache([5], 2, 16, 128, BF16, DEV, 71)
     q = torch.empty((0, 16, 128), dtype=BF16, device=DEV)
