@@ -14,9 +14,11 @@
 // The final O / l does not depend on m.
 //
 // Warps: 0-3 and 4-7 softmax, tile 0 and 1; 8 K/V producer (TMA, one box per
-// page and 64 dims, 128-byte swizzle); 9 MMA issuer; 10 fetches Q and clears the
-// rows of the last V block past the item's last key (their P is 0, but 0 times
-// a NaN in an unused slot is not); 11 only writes the record of the item that goes
+// page and 64 dims, 128-byte swizzle); 9 MMA issuer; 10 fetches Q and cleans the
+// rows of V that not every row of the item attends: their P is 0 for those that do
+// not, but 0 times a NaN is not.  Rows past the item's last key go to 0; the others
+// are looked through for values that are not finite, which are taken out and in the
+// end added to the rows that attend them; 11 only writes the record of the item that goes
 // on into this stretch.
 //
 // P is rounded to the cache's type because that is what the matrix instruction
@@ -150,12 +152,22 @@ __device__ __forceinline__ bool bar_wait_long(uint64_t* bar, uint32_t parity, vo
     *abort_flag = 1;
     return false;
 }
-// the item's last block has rows without a key
-__device__ __forceinline__ bool has_tail(int limit) { return limit % kKeys != 0 || limit == 0; }
+// whether block j has rows that not every row of the item attends, as its last ones
+__device__ __forceinline__ bool is_tail(int j, int least) { return (j + 1) * kKeys > least; }
+// 16-bit values from this magnitude on are not finite
+template <int DT>
+constexpr uint32_t kNotFinite = DT == kBF16 ? 0x7f80u : 0x7c00u;
+// the two 16-bit values of x, 0 where not finite
+template <int DT>
+__device__ __forceinline__ uint32_t finite_only(uint32_t x) {
+    const uint32_t size = x & 0x7fff7fffu;
+    return x & ((size & 0xffffu) >= kNotFinite<DT> ? 0xffff0000u : 0xffffffffu) &
+           (size >> 16 >= kNotFinite<DT> ? 0xffffu : 0xffffffffu);
+}
 
 struct ChunkBars {
     uint64_t kv_full[8], kv_empty[8];
-    uint64_t v_tail[8];  // the last V block of an item has landed, rows past its last key not cleared yet
+    uint64_t v_tail[8];  // a block of V has landed whose last rows are to be looked at first
     uint64_t q_full, q_empty;
     uint64_t s_full[2], p_half[2], p_ready[2], o_done[2];
 };
@@ -171,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ __align__(8) ChunkBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, beat_count;
+    __shared__ int odd_first, odd_last;  // the pieces from whose V something was taken out
     __shared__ int64_t sums[kThreads / 32], place_at;
     __shared__ int place_seq;
     const PagedBatch& p = a.p;
@@ -199,6 +212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.o_done[i], 1);
         }
         abort_flag = beat_count = 0;
+        odd_first = 0x7fffffff;
+        odd_last = -1;
         fence_mbar_init();
     }
     tc_fence_before();
@@ -239,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int s = seq % M::kStages;
                         if (seq >= M::kStages) ok = bar_wait(&bars.kv_empty[s], (seq / M::kStages - 1) & 1, abort_p);
                         if (!ok) break;
-                        // the tail of V goes through warp 10, which then completes kv_full
-                        const bool tail = v == 1 && j == w.tiles - 1 && has_tail(w.limit);
+                        // a tail of V goes through warp 10, which then completes kv_full
+                        const bool tail = v == 1 && is_tail(j, w.least);
                         tail_use = tail ? tail_use | 1u << s : tail_use & ~(1u << s);
                         if (tail) tail_parity ^= 1u << s;
                         uint64_t* const full = tail ? &bars.v_tail[s] : &bars.kv_full[s];
@@ -361,21 +376,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) bar_arrive(&bars.q_full);
                 }
                 ++items;
-                seq += 2 * (w.t1 - w.t0);
-                if (w.t1 == w.tiles && has_tail(w.limit)) {
-                    const uint32_t sv = (seq - 1) % M::kStages;  // the piece's last V block
-                    if (!bar_wait_long(&bars.v_tail[sv], tail_parity >> sv & 1, abort_p, beat)) break;
+                bool ok = true;
+                for (int j = max(w.t0, w.least / kKeys); j < w.t1; ++j) {
+                    const uint32_t sv = (seq + 2 * (j - w.t0) + 1) % M::kStages;
+                    ok = bar_wait_long(&bars.v_tail[sv], tail_parity >> sv & 1, abort_p, beat);
+                    if (!ok) break;
                     tail_parity ^= 1u << sv;
-                    const int from = w.limit - (w.tiles - 1) * kKeys;  // rows from here on hold no key
-                    uint8_t* v = ring + sv * M::kTile;
-                    for (int i = from * 8 + lane; i < 128 * 8; i += 32)
+                    // rows from `some` on are attended by some rows of the item, from `none` on by none
+                    const int some = max(w.least - j * kKeys, 0), none = min(w.limit - j * kKeys, kKeys);
+                    uint4* const v = reinterpret_cast<uint4*>(ring + sv * M::kTile);
+                    uint32_t most = 0;  // the largest magnitude of either half
+#pragma unroll 4
+                    for (int i = some * 8 + lane; i < none * 8; i += 32)
 #pragma unroll
-                        for (int h = 0; h < M::kHalves; ++h)
-                            *reinterpret_cast<uint4*>(v + h * (128 * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+                        for (int h = 0; h < M::kHalves; ++h) {
+                            const uint4 x = v[h * (128 * 8) + i];
+                            most = __vmaxu2(most, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu));
+                            most = __vmaxu2(most, __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+                        }
+                    if (__any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) >= kNotFinite<DT>)) {
+                        for (int i = some * 8 + lane; i < none * 8; i += 32)
+                            for (int h = 0; h < M::kHalves; ++h) {
+                                const uint4 x = v[h * (128 * 8) + i];
+                                v[h * (128 * 8) + i] = make_uint4(finite_only<DT>(x.x), finite_only<DT>(x.y),
+                                                                  finite_only<DT>(x.z), finite_only<DT>(x.w));
+                            }
+                        odd_first = min(odd_first, static_cast<int>(items) - 1);
+                        odd_last = static_cast<int>(items) - 1;
+                    }
+                    for (int i = none * 8 + lane; i < kKeys * 8; i += 32)
+#pragma unroll
+                        for (int h = 0; h < M::kHalves; ++h) v[h * (128 * 8) + i] = make_uint4(0, 0, 0, 0);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&bars.kv_full[sv]);
                 }
+                if (!ok) break;
+                seq += 2 * (w.t1 - w.t0);
             }
             if (q_by_tma && items > 0) bar_wait(&bars.q_full, (items - 1) & 1, abort_p, false);  // Q has landed
         }
@@ -518,6 +555,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 8) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+    // (rare) what was taken out of V, to the rows that attend it: thread = row, as above
+    if (odd_first > odd_last || warp >= 8) return;
+    W v;
+    v.begin(p, group, shares, worker, place_seq, place_at);
+#pragma unroll 1
+    for (int piece = 0; piece <= odd_last && v.next(p, group); ++piece) {
+        const int token = (v.q * kRows + tid) / group;
+        if (piece < odd_first || tid >= v.item_rows) continue;
+        const int end = min(min(max(v.piece_len - v.piece_n + token + 1, 0), v.limit), v.t1 * kKeys);
+        uint16_t* const out = static_cast<uint16_t*>(a.out) + (v.piece_start + token) * a.out_stride +
+                              static_cast<int64_t>(v.kvh * group + (v.q * kRows + tid) % group) * D;
+        float* const part = Part::slot(a.workspace, gridDim.x, worker, v.t0 > 0 ? 0 : 1) + 2 * kRows + tid * 4;
+#pragma unroll 1
+        for (int key = max(v.t0 * kKeys, v.least); key < end; ++key) {
+            const int page = p.table[v.piece_b * p.table_stride + key / p.page_size];
+            if (page < 0 || page >= p.num_pages) continue;
+            const uint16_t* const x = static_cast<const uint16_t*>(a.v_pages) +
+                                      ((static_cast<int64_t>(page) * p.kv_heads + v.kvh) * p.page_size +
+                                       (key & (p.page_size - 1))) * D;
+#pragma unroll 1
+            for (int i = 0; i < D; ++i) {
+                if ((x[i] & 0x7fffu) < kNotFinite<DT>) continue;
+                const float y = DT == kBF16 ? bf16_bits_to_f32(x[i]) : f16_bits_to_f32(x[i]);
+                float* const at = part + (i >> 2) * (kRows * 4) + (i & 3);
+                if (v.whole()) {
+                    const float z = DT == kBF16 ? bf16_bits_to_f32(out[i]) : f16_bits_to_f32(out[i]);
+                    out[i] = static_cast<uint16_t>(pack2<DT>(z + y, 0.F));
+                } else {
+                    *at += y;
+                }
+            }
+        }
     }
 }
 

@@ -190,6 +190,8 @@ struct PagedWalk {
         c.kvh = kvh;
         return c;
     }
+    // whether some rows of the piece do not attend all of its keys
+    __device__ __forceinline__ bool uneven() const { return least < min(limit, t1 * KT); }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
 

@@ -284,6 +284,17 @@ def test_attention_values_that_are_not_finite_few_rows(bridge, case, value):
     values_not_finite(bridge, *case, value)
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("case", [
+    # many rows a key head: blocks of 128 keys, items of 256 rows, pieces cut from a long sequence
+    (BF16, 8, 1, 128, [130], [130], 0), (F16, 8, 2, 64, [40, 9], [300, 9], 13), (BF16, 16, 2, 128, [70, 3], [200, 77], 19),
+    (F16, 2, 2, 128, [257], [400], 130), (BF16, 10, 2, 128, [50], [4000], 2), (F16, 17, 1, 128, [9], [128], 0),
+    (BF16, 40, 1, 64, [30, 50], [30, 51], 28), (BF16, 32, 8, 128, [200, 60, 1], [1000, 60, 500], 140),
+])
+def test_attention_values_that_are_not_finite_many_rows(bridge, case, value):
+    values_not_finite(bridge, *case, value)
+
+
 def test_attention_no_rows(bridge):
     k, v, table, _, _ = R.make_cache([5], 2, 16, 128, BF16, DEV, 71)
     q = torch.empty((0, 16, 128), dtype=BF16, device=DEV)
