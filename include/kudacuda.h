@@ -586,8 +586,15 @@ KUDACUDA_API int kudacuda_sm100_gqa_decode_batch(void* handle, uint64_t query, u
  *   pages.  32-bit arithmetic, one rounding.
  * paged_attention: out[r][h] = softmax(scale q k^T) V over keys at positions
  *   <= the row's own, lse (optional, fp32 [rows][q_heads]) the natural log of
- *   the sum of exponentials; a row without keys gives 0 and -inf.  max_query
- *   is the largest number of rows of a sequence.  workspace_bytes(max_kv =
+ *   the sum of exponentials; a row without keys gives 0 and -inf.  Scores,
+ *   sums and accumulators have 32 bits.  max_query, the largest number of rows
+ *   of a sequence, chooses the kernel for the whole batch: with max_query *
+ *   q_heads / kv_heads <= 16 the one that keeps the probabilities to twice the
+ *   type's precision, else one that rounds each to the type (half a step of
+ *   it, as the output's own rounding).  A smaller max_query than the rows are
+ *   is allowed: the first kernel then takes them too, re-reading the cache for
+ *   every 16 rows.  How the work is cut depends on the whole batch, so a row's
+ *   last bits do too; the same call gives the same bits.  workspace_bytes(max_kv =
  *   table_width * page_size) once; the contents need no initialisation, and
  *   calls that may overlap need a workspace each.
  * kv_pages_copy: page pairs[i][0] -> page pairs[i][1] (int32 device pairs) of

@@ -15,7 +15,11 @@ namespace kc {
 
 // Query rows a key head (of the longest sequence) up to which the decode kernel
 // serves: its tile, for a second one it reads the cache again.  It also keeps the
-// probabilities to twice the type's precision.  Decode and chunk kernel, us, 4
+// probabilities to twice the type's precision, where the chunk kernel rounds them to
+// the type: against 64 bits the relative error is 0.0022 (24 mixed sequences) and
+// 0.0023 (4 x 2048 tokens over 8192 keys) where the output's rounding alone makes
+// 0.0017.  max_query is the caller's, who may name a smaller one to have the decode
+// kernel.  Decode and chunk kernel, us, 4
 // key heads of 128 bf16 dims, 1 token of 8 heads / 2 / 3:
 //   64 sequences of 500 keys    25.5, 26.2 / 28.4, 26.4 / 41.6, 26.5
 //   16 of 2000                  22.9, 23.3 / 24.6, 23.4 / 32.8, 23.5

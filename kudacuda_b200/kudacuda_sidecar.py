@@ -1567,7 +1567,9 @@ class KudaCudaBridge:
         """Causal attention of a ragged batch of new tokens over a paged cache that holds them already.
 
         ``query`` / ``output`` [rows, q_heads, head_dim] (rows may be strided), ``lse`` float32
-        [rows, q_heads] or None; see kudacuda_sm100_paged_attention in include/kudacuda.h."""
+        [rows, q_heads] or None.  ``max_query`` (at most the rows of the longest sequence) times the query heads
+        a key head up to 16 keeps the probabilities to twice the dtype's precision, more rounds each to it; see
+        kudacuda_sm100_paged_attention in include/kudacuda.h."""
 
         dtype = query.dtype
         code, (num_pages, kv_heads, page_size, head_dim), batch = self._paged_batch(

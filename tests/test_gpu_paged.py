@@ -220,6 +220,36 @@ def test_attention_does_not_depend_on_the_batch_and_repeats(bridge, new):
     assert bridge.error_word(clear=True) == 0
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("new,lens,heads,kv_heads", [([1, 70, 3], [900, 333, 40], 16, 2), ([300, 1], [300, 4000], 4, 1)])
+def test_attention_with_a_smaller_max_query_keeps_the_probabilities(bridge, dtype, new, lens, heads, kv_heads):
+    """The kernel that max_query = 1 chooses takes any number of rows, and rounds the output alone to the type."""
+
+    k, v, table, keys, vals = R.make_cache(lens, kv_heads, 32, 128, dtype, DEV, 57)
+    q = torch.randn((sum(new), heads, 128), generator=torch.Generator().manual_seed(58)).to(dtype)
+    out, lse = attend(bridge, q.to(DEV), k, v, table, new, lens, max_query=1)
+    assert bridge.error_word(clear=True) == 0
+    check_attention(q, new, lens, keys, vals, out, lse, 128**-0.5)
+    ref, _, mag, _ = R.attention(q, new, lens, keys, vals, 128**-0.5)
+    assert ((out.double().cpu() - ref).abs() <= R.UNIT[dtype] * ref.abs() + 2.0**-14 * mag).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [60, 1, 17, 1], [3, 1, 200, 2]])
+def test_attention_of_a_part_of_the_batch(bridge, new):
+    """Sequences alone, in twos and all together give the same rows, within the bound of either."""
+
+    lens = [600, 77, 1500, 300]
+    k, v, table, keys, vals = R.make_cache(lens, 2, 32, 128, BF16, DEV, 53)
+    q = torch.randn((sum(new), 16, 128), generator=torch.Generator().manual_seed(54)).to(BF16).to(DEV)
+    at = [sum(new[:i]) for i in range(5)]
+    for part in ([0], [1], [2], [3], [0, 1], [1, 3], [2, 3], [0, 1, 2, 3]):
+        rows = torch.cat([q[at[i]:at[i + 1]] for i in part])
+        some = [[x[i] for i in part] for x in (new, lens, keys, vals)]
+        out, lse = attend(bridge, rows, k, v, table[part], some[0], some[1])
+        assert bridge.error_word(clear=True) == 0
+        check_attention(rows, *some, out, lse, 128**-0.5)
+
+
 @pytest.mark.parametrize("new", [[1, 1], [40, 3]])
 def test_attention_flags_a_missing_page_and_spares_the_others(bridge, new):
     lens = [200, 150]
