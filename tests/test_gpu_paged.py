@@ -714,6 +714,109 @@ def test_sample_row_does_not_depend_on_its_batch(bridge):
         assert one[0] == whole[r] and lo[0] == lw[r]
 
 
+# ------------------------------------------------------------------ in a captured graph
+def captured(work):
+    """Runs ``work`` once, captures it, and returns the replay."""
+
+    work()
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        work()
+
+    def replay():
+        graph.replay()
+        torch.cuda.synchronize()
+
+    return replay
+
+
+def current():
+    return int(torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", [(BF16, 1, 151936), (BF16, 64, 20000), (torch.float32, 300, 777),
+                                              (F16, 3, 40001), (torch.float32, 2, 900001)])
+def test_sample_in_a_graph(bridge, dtype, rows, vocab):
+    """One block a row, clusters of up to 16 and rows that no cluster holds; every replay on new inputs."""
+
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.empty((rows, vocab), dtype=dtype, device=DEV)
+    u, temperature, top_p = (torch.empty((rows,), device=DEV) for _ in range(3))
+    top_k = torch.empty((rows,), dtype=torch.int32, device=DEV)
+
+    def fill():
+        x.copy_(3.0 * torch.randn((rows, vocab), generator=g, device=DEV))
+        for t, low, high in ((u, 0.0, 1.0), (temperature, -0.3, 1.5), (top_p, 0.5, 1.1)):
+            t.copy_(low + (high - low) * torch.rand((rows,), generator=g, device=DEV))
+        top_k.copy_(torch.randint(0, 60, (rows,), generator=g, device=DEV))
+
+    def into(tokens, logp):
+        bridge.dispatch_sample(x, tokens, u, temperature=temperature, top_k=top_k, top_p=top_p, logprobs=logp,
+                               stream_ptr=current())
+
+    fill()
+    tokens, logp = torch.zeros((rows,), dtype=torch.int32, device=DEV), torch.zeros((rows,), device=DEV)
+    want, want_logp = torch.zeros_like(tokens), torch.zeros_like(logp)
+    replay = captured(lambda: into(tokens, logp))
+    for _ in range(3):
+        fill()
+        replay()
+        into(want, want_logp)
+        torch.cuda.synchronize()
+        assert torch.equal(tokens, want) and torch.equal(logp, want_logp)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [700, 1, 30]])
+def test_rope_append_in_a_graph(bridge, new):
+    """The lengths are device data: a replay appends where they say."""
+
+    lens = [800, 40, 90]
+    k, v, table, _, _ = R.make_cache([n + 20 for n in lens], 2, 16, 128, BF16, DEV, 97, junk=0.0)
+    start, kv = R.starts(new, DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    qkv = torch.randn((sum(new), 20 * 128), generator=torch.Generator(device=DEV).manual_seed(98), device=DEV).to(BF16)
+    ang = torch.rand((900, 64), generator=torch.Generator(device=DEV).manual_seed(99), device=DEV) * 6.28
+    cos, sin = ang.cos(), ang.sin()
+    q = torch.zeros((sum(new), 16, 128), dtype=BF16, device=DEV)
+
+    def into(q, k, v):
+        bridge.dispatch_rope_append_paged(qkv, q, k, v, cos, sin, start, kv, table, stream_ptr=current())
+
+    replay = captured(lambda: into(q, k, v))
+    for step in range(3):
+        kv.add_(step + 1)
+        qkv.mul_(0.5)
+        want_q, want_k, want_v = q.clone(), k.clone(), v.clone()
+        into(want_q, want_k, want_v)
+        replay()
+        assert torch.equal(q, want_q) and torch.equal(k, want_k) and torch.equal(v, want_v)
+    assert bridge.error_word(clear=True) == 0
+
+
+def test_kv_pages_copy_in_a_graph(bridge):
+    g = torch.Generator(device=DEV).manual_seed(21)
+    k, v = (torch.randn((3, 12, 2, 16, 64), generator=g, device=DEV).to(BF16) for _ in range(2))
+    pairs = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    table = torch.randint(-1, 12, (3, 5), generator=g, device=DEV, dtype=torch.int32)
+    page_map = torch.arange(12, dtype=torch.int32, device=DEV)
+
+    def into(k, v, table):
+        bridge.dispatch_kv_pages_copy(k, v, pairs, block_table=table, page_map=page_map, stream_ptr=current())
+
+    replay = captured(lambda: into(k, v, table))
+    for new in ([[4, 5], [6, 0]], [[11, 2], [8, 9]]):
+        pairs.copy_(torch.tensor(new, dtype=torch.int32))
+        page_map.copy_(torch.arange(12, dtype=torch.int32))
+        for a, b in new:
+            page_map[a] = b
+        want = k.clone(), v.clone(), table.clone()
+        into(*want)
+        replay()
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1]) and torch.equal(table, want[2])
+        assert torch.equal(k[:, new[0][1]], k[:, new[0][0]])
+    assert bridge.error_word(clear=True) == 0
+
+
 # ------------------------------------------------------------------ refusals of the C entries
 def test_native_refusals(bridge):
     from kudacuda_b200.kudacuda_sidecar import NativeCudaError
