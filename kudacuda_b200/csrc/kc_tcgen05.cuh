@@ -1,7 +1,7 @@
 // kc_tcgen05.cuh -- the 5th-generation tensor core's plumbing shared by the
-// batched GEMM (batched.cu) and the paged attention (paged_attention.cu):
-// matrix instructions, tensor-memory access, shared-memory descriptors, 2D
-// TMA loads and bounded mbarrier waits.
+// batched GEMM (batched.cu) and the paged attention (paged_chunk.cu; the loads
+// also paged_decode.cu): matrix instructions, shared-memory descriptors, 2D and
+// 3D TMA loads and bounded mbarrier waits.
 #pragma once
 
 #include <cuda.h>

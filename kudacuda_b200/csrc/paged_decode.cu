@@ -57,7 +57,7 @@ constexpr float kShift = DT == kF16 ? 15.F : 0.F;
 template <int D>
 struct DecodeSmem {
     static constexpr int kHalves = D / 64;
-    static constexpr int kBlock = kHalves * kKeys * 128;  // [D / 64][32][128 B]
+    static constexpr int kBlock = kHalves * kKeys * 128;  // [D / 64][16][128 B]
     static constexpr int kStages = D == 128 ? 3 : 6;
     static constexpr int kWarpBytes = kStages * 2 * kBlock;
     static constexpr int kMeet = kWarps / 2 * kRows * D * 4;  // accumulators of half of the warps
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     continue;
                 }
                 const uint32_t kb = smem_u32(ring + s * 2 * M::kBlock), vb = kb + M::kBlock;
-                // S: 16 rows x 32 keys, four tiles of 8 keys
+                // S: 16 rows x 16 keys, two tiles of 8 keys
                 float sc[kKeys / 8][4], sc2[kKeys / 8][4];  // even and odd steps of 16 dims: two chains
 #pragma unroll
                 for (int n = 0; n < kKeys / 8; ++n)
