@@ -160,8 +160,12 @@ class PagedKVCache:
         number of pages moved."""
 
         used = [p for p in range(self.num_pages) if self._refs[p] > 0]
-        known = {p for s in sequences for p in s.pages}
-        if known != set(used):
+        sequences = list({id(s): s for s in sequences}.values())
+        owners = [0] * self.num_pages
+        for s in sequences:
+            for p in s.pages:
+                owners[p] += 1
+        if owners != self._refs:  # (a fork left out would keep pages that have moved)
             raise ValueError("compact needs all of the cache's sequences")
         low = [p for p in range(len(used)) if self._refs[p] == 0]
         pairs = list(zip([p for p in used if p >= len(used)], low))

@@ -330,6 +330,20 @@ class StreamedTorch:
         return self._maker(value) if name in ("tensor", "arange", "zeros") else value
 
 
+def test_compaction_needs_the_forks_too():
+    cache, copier = make()
+    a, b = PagedSequence(), PagedSequence()
+    grow(cache, a, range(20))
+    grow(cache, b, range(100, 120))
+    fork = cache.fork(b)
+    cache.free(a)
+    with pytest.raises(ValueError, match="all of the cache's sequences"):
+        cache.compact([b], 0)  # its pages are all that are in use, but the fork would be left behind
+    assert b.pages == fork.pages == [2, 3] and not copier.calls
+    assert cache.compact([b, fork, b], 0) == 2 and b.pages == fork.pages == [0, 1]
+    assert read(cache, b) == read(cache, fork) == list(range(100, 120))
+
+
 def test_copies_use_memory_of_the_stream_they_run_on():
     """The lists of a copy go back to the allocator as soon as it is launched, so they must come from the
     stream that it runs on: another one could take their memory while the copy still reads them."""
