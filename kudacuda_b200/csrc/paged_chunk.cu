@@ -30,9 +30,9 @@
 // 128, O 2 x 128 columns).
 //
 // Measured, 4 prompts of 2048 tokens of 16 heads over 8192 keys (2 key heads of 128
-// bf16 dims; 0.48 Tflop): 374 us on a cool card, 1.29 Pflop/s (the library's
-// largest product: 1.63), and 432 us after a second of it, when the power limit
-// brings the clocks down (1.11, the library's product: 1.36).  A step of both
+// bf16 dims; 0.48 Tflop): 375 us on a cool card, 1.28 Pflop/s (the library's
+// largest product: 1.63), and 431 us after a second of it, when the power limit
+// brings the clocks down (1.12, the library's product: 1.36).  A step of both
 // tiles takes 3550 clocks, of which the products could use 2048; the rest is the
 // chain from a score to its product with V (load from tensor memory 60, maximum
 // 300, exponentials and stores 1250) and six barrier waits of about 180.  Without

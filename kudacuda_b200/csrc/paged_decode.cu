@@ -24,11 +24,11 @@
 // keys past some row's own, it is looked through for one first, and if there is one
 // the product is taken row by row.
 //
-// Measured (128 dims): 2 sequences of 70 001 to 130 001 keys, 8 key heads of 4: 131 us,
-// 5.9 TB/s of the card's 6.55 (the join of the pieces, 4 us, does not overlap); 64
+// Measured (128 dims): 2 sequences of 70 001 to 130 001 keys, 8 key heads of 4: 130 us,
+// 6.0 TB/s of the card's 6.55 (the join of the pieces, 4 us, does not overlap); 64
 // of 32 to 2048 keys, 2 key heads of 8: 19.4 us, 30 MB, of which the loop takes 8:
 // the rest is the chain before it (lengths, shares, page numbers) and after it
-// (meeting, pieces, join) and two launches.  1 of 509 keys: 12.3 us.
+// (meeting, pieces, join) and two launches.  1 of 509 keys: 12.5 us.
 #include "kc_common.cuh"
 #include "kc_launch.h"
 #include "kc_tcgen05.cuh"
@@ -123,7 +123,7 @@ struct Piece {
 };
 constexpr int kList = 12;
 
-// (one block an SM, said aloud, gives the loop 238 registers instead of 175: 64
+// (one block an SM, said aloud, gives the loop 244 registers instead of 175: 64
 // sequences of 500 keys, 4 key heads, take 21.8 us instead of 24.0)
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads, 1)
