@@ -33,8 +33,7 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
 }
 
 // 1 / T, never 0: for an infinite T the smallest 32-bit number stands for it, by
-// which x - m of a finite entry becomes about 0 (weight 1: the draw is uniform) and
-// that of a -inf stays -inf (weight 0), where 0 would make it NaN.
+// which x - m of a -inf stays -inf (weight 0), where 0 would make it NaN.
 __device__ __forceinline__ float inverse_temperature(float t) { return fmaxf(1.F / t, 1.4e-45F); }
 
 template <typename T, typename F>
@@ -83,7 +82,8 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
         return;
     }
     const float inv = inverse_temperature(t);
-    auto weight = [&](float x) { return x == m ? 1.F : expf((x - m) * inv); };
+    const float full = t == INFINITY && m < INFINITY ? -3.402823466e38F : m;  // from here on the weight is 1
+    auto weight = [&](float x) { return x >= full ? 1.F : expf((x - m) * inv); };
     auto mass = [&](float x) { return __float2ll_rn(weight(x) * kMassOne); };
     // kept: key > cut, or key == cut and index < tie_end
     uint32_t cut = 0;
@@ -483,11 +483,13 @@ __global__ void __launch_bounds__(kMaxSampleThreads, 2) sample_cluster_kernel(co
         return;
     }
     const float inv = inverse_temperature(t);
+    // keys from here on weigh 1: the maximum, for an infinite T every finite one
+    const uint32_t full = t == INFINITY && m < INFINITY ? K::near(-INFINITY) + 1 : top;
     // (written so that nothing branches: a branch an entry, over the exponential or
     // over the sums of a pivot, made 64 rows 60 us instead of 53)
     auto weight = [&](uint32_t k) {
         const float e = expf((K::value(k) - m) * inv);
-        return k == top ? 1.F : e;
+        return k >= full ? 1.F : e;
     };
     auto mass = [&](uint32_t k) {
         int hi, lo;

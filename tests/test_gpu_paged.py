@@ -632,6 +632,22 @@ def test_sample_infinite_temperature(bridge, dtype, vocab):
         check_rows(bridge, x, u, [math.inf] * rows, [k] * rows, [p] * rows, [low] * rows)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, F16])
+def test_sample_infinite_temperature_and_the_lowest_value(bridge, dtype):
+    """A mask of the type's lowest value is finite, so it is as likely as any; min-p of 1 keeps it too."""
+
+    g = torch.Generator().manual_seed(12)
+    info = torch.finfo(dtype)
+    x = 3.0 * torch.randn((6, 501), generator=g, dtype=torch.float64)
+    x = torch.where(torch.rand((6, 501), generator=g) < 0.5, info.min, x)
+    x[2::3, ::9] = info.max
+    x[1::3, ::5] = -math.inf
+    x = x.to(dtype).to(DEV)
+    for k, p, low in ((0, 1.0, 0.0), (0, 1.0, 1.0), (0, 0.7, 0.3), (400, 0.9, 1.0)):
+        u = torch.rand((6,), generator=g).tolist()
+        check_rows(bridge, x, u, [math.inf] * 6, [k] * 6, [p] * 6, [low] * 6)
+
+
 def test_sample_values_of_every_size(bridge):
     """bf16 values that few entries share, near 0, past 128 and far below, beside ordinary ones."""
 
