@@ -215,7 +215,8 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const SampleArgs a) {
 //
 // The logits are read once, so memory asks 3 us of 64 rows of 151 936 16-bit
 // logits and 10 us of 333 rows of 50 257 32-bit ones.  What they do cost, rows of
-// all kinds mixed, is 47 to 60 and 88 to 97 us, depending on the rows: instructions
+// all kinds mixed, is 41 to 75 and 90 to 103 us, depending on the rows (means of 16
+// draws 51 and 95): instructions
 // in the first try and in the pass in index order (an exponential and two roundings
 // an entry, three additions more for every key tried), and waits: a row goes
 // through six or so barriers of its cluster, 1 to 2 us each with what lies between,
